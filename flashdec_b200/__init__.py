@@ -30,6 +30,9 @@ __all__ = [
     "device_status",
     "reserve_workspace",
     "copy_async",
+    "window_attention",
+    "scored_decode",
+    "evict_tokens",
 ]
 
 __version__ = "0.2.0"
@@ -75,6 +78,10 @@ def _resolve(name):
             "paged_decode_attention": paged_decode.paged_decode_attention,
             "paged_decode_attention_into": paged_decode.paged_decode_attention_into,
         }[name]
+    if name in ("window_attention", "scored_decode", "evict_tokens"):
+        from .kernels import bounded_cache
+
+        return getattr(bounded_cache, name)
     if name == "copy_async":
         # the C++ function itself: one cudaMemcpyAsync per call, no Python
         # frame in between (a missing host-path module raises here)

@@ -93,11 +93,46 @@ class RopeKVAppendArgs(ctypes.Structure):
     ]
 
 
+class StreamAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", _i32), ("dtype", _i32), ("num_seqs", _i32), ("num_tokens", _i32),
+        ("num_q_heads", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("block_size", _i32),
+        ("num_blocks", _i32), ("max_blocks_per_seq", _i32),
+        ("window", _i64), ("sinks", _i64), ("max_query_len", _i32), ("sm_scale", _f32),
+        ("q", _vp), ("q_stride", _I64x3), ("out", _vp), ("out_stride", _I64x3),
+        ("k_cache", _vp), ("k_stride", _I64x4), ("v_cache", _vp), ("v_stride", _I64x4),
+        ("block_tables", _vp), ("block_tables_stride", _I64x2),
+        ("seq_lens", _vp), ("seq_lens_stride", _i64),
+        ("query_start_loc", _vp), ("query_start_loc_stride", _i64),
+        ("block_tables_index", _i32), ("seq_lens_index", _i32), ("query_start_loc_index", _i32),
+        ("reserved", _i32),
+        ("scores", _vp), ("scores_stride", _I64x3), ("scratch", _vp), ("scratch_bytes", _sz),
+    ]
+
+
+class EvictTokensArgs(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", _i32), ("elem_bytes", _i32), ("num_seqs", _i32), ("num_kv_heads", _i32),
+        ("head_dim", _i32), ("block_size", _i32), ("num_blocks", _i32),
+        ("max_blocks_per_seq", _i32), ("max_new_blocks_per_seq", _i32),
+        ("budget", _i32), ("sinks", _i32), ("recent", _i32),
+        ("k_cache", _vp), ("k_stride", _I64x4), ("v_cache", _vp), ("v_stride", _I64x4),
+        ("scores", _vp), ("scores_stride", _I64x3),
+        ("block_tables", _vp), ("block_tables_stride", _I64x2),
+        ("seq_lens", _vp), ("seq_lens_stride", _i64),
+        ("new_block_tables", _vp), ("new_block_tables_stride", _I64x2),
+        ("block_tables_index", _i32), ("seq_lens_index", _i32), ("new_block_tables_index", _i32),
+        ("new_seq_lens_index", _i32), ("kept", _vp), ("new_seq_lens", _vp),
+    ]
+
+
 # Exported symbols declared in include/flashdec_b200.h
 EXPORTED_SYMBOLS = (
     "fd_paged_decode_workspace", "fd_paged_decode", "fd_split_kv_reduce", "fd_rope_kv_append",
     "fd_error_string", "fd_version", "fd_device_status", "fd_num_sms", "fd_paged_decode_static",
     "fd_selftest_wait_timeout", "fd_cascade_workspace", "fd_cascade_decode",
+    "fd_window_attention_workspace", "fd_window_attention", "fd_scored_decode_workspace",
+    "fd_scored_decode", "fd_evict_tokens",
 )
 
 _lock = threading.Lock()
@@ -146,7 +181,14 @@ def load_library():
         lib.fd_device_status.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
         lib.fd_num_sms.argtypes = []
         lib.fd_selftest_wait_timeout.argtypes = [ctypes.c_int64, _vp]
-        for name in ("fd_paged_decode_workspace", "fd_paged_decode", "fd_paged_decode_static",
+        for name in ("fd_window_attention", "fd_scored_decode"):
+            getattr(lib, name).argtypes = [ctypes.POINTER(StreamAttentionArgs), _vp]
+            getattr(lib, name + "_workspace").argtypes = [ctypes.POINTER(StreamAttentionArgs),
+                                                          ctypes.POINTER(_sz)]
+            getattr(lib, name + "_workspace").restype = ctypes.c_int
+        lib.fd_evict_tokens.argtypes = [ctypes.POINTER(EvictTokensArgs), _vp]
+        for name in ("fd_window_attention", "fd_scored_decode", "fd_evict_tokens",
+                     "fd_paged_decode_workspace", "fd_paged_decode", "fd_paged_decode_static",
                      "fd_split_kv_reduce", "fd_selftest_wait_timeout",
                      "fd_rope_kv_append", "fd_version", "fd_device_status", "fd_num_sms"):
             getattr(lib, name).restype = ctypes.c_int
@@ -174,8 +216,15 @@ def load_hostpath():
         if hp.ARGS_BYTES != ctypes.sizeof(PagedDecodeArgs):
             raise RuntimeError("flashdec_b200._hostpath was built against another "
                                "fd_paged_decode_args layout: rebuild it")
+        if (hp.STREAM_ARGS_BYTES != ctypes.sizeof(StreamAttentionArgs)
+                or hp.EVICT_ARGS_BYTES != ctypes.sizeof(EvictTokensArgs)):
+            raise RuntimeError("flashdec_b200._hostpath was built against another layout of the "
+                               "bounded-cache argument structs: rebuild it")
         hp.set_entry_points(ctypes.cast(lib.fd_paged_decode, ctypes.c_void_p).value,
                             ctypes.cast(lib.fd_cascade_decode, ctypes.c_void_p).value)
+        hp.set_stream_entry_points(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in (
+            lib.fd_window_attention, lib.fd_window_attention_workspace, lib.fd_scored_decode,
+            lib.fd_scored_decode_workspace, lib.fd_evict_tokens, lib.fd_error_string)))
         _hostpath = hp
         return hp
 

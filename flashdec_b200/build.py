@@ -24,7 +24,8 @@ CSRC = PKG / "csrc"
 INCLUDE = REPO / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libflashdec_b200.so"
-SOURCES = ["fd_host.cu", "fd_attention.cu", "fd_wave_decode.cu", "fd_rope_append.cu", "fd_static.cu", "fd_selftest.cu"]
+SOURCES = ["fd_host.cu", "fd_attention.cu", "fd_wave_decode.cu", "fd_rope_append.cu", "fd_static.cu", "fd_selftest.cu",
+           "fd_stream_attention.cu", "fd_evict.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
          "-I", str(INCLUDE), "-I", str(CSRC)]
@@ -64,6 +65,8 @@ def _compile(src: str, verbose: bool) -> Path:
 
 
 HOSTPATH_SRC = CSRC / "fd_hostpath.cpp"
+HOSTPATH_SOURCES = [HOSTPATH_SRC, CSRC / "fd_stream_host.cpp"]
+HOSTPATH_HEADERS = [INCLUDE / "flashdec_b200.h", CSRC / "fd_stream_host.h"]
 HOSTPATH = PKG / ("_hostpath" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
@@ -73,7 +76,7 @@ def build_hostpath(verbose: bool = False, force: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    newest = max(HOSTPATH_SRC.stat().st_mtime, (INCLUDE / "flashdec_b200.h").stat().st_mtime)
+    newest = max(f.stat().st_mtime for f in HOSTPATH_SOURCES + HOSTPATH_HEADERS)
     if HOSTPATH.exists() and HOSTPATH.stat().st_mtime >= newest and not force:
         return HOSTPATH
     incs = cpp_extension.include_paths(device_type="cuda") + [sysconfig.get_paths()["include"],
@@ -84,7 +87,7 @@ def build_hostpath(verbose: bool = False, force: bool = False) -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_hostpath",
            "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{d}" for d in incs],
-           str(HOSTPATH_SRC), "-o", str(tmp), *[f"-L{d}" for d in libs],
+           *map(str, HOSTPATH_SOURCES), "-o", str(tmp), *[f"-L{d}" for d in libs],
            "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lcudart",
            *[f"-Wl,-rpath,{d}" for d in libs]]
     if verbose:

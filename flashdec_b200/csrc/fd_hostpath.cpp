@@ -32,6 +32,8 @@
 //    stream-ordered cudaMemcpyAsync between a host tensor and a device
 //    tensor (or two device tensors) on the device's current stream.
 //
+//  * the bounded-cache operators of fd_stream_host.cpp.
+//
 // The entry points are taken as addresses from the already-loaded
 // libflashdec_b200.so (set_entry_points), so both paths call the same
 // library.  Every function runs with the GIL held, which serialises the
@@ -48,6 +50,7 @@
 #include <unordered_map>
 #include <vector>
 
+#include "fd_stream_host.h"
 #include "flashdec_b200.h"
 
 namespace {
@@ -434,4 +437,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("copy_async", &copy_async, py::arg("dst"), py::arg("src"),
         "dst <- src on the current stream of the CUDA side's device (one cudaMemcpyAsync); "
         "keep both tensors alive until the stream has passed the copy");
+  bind_stream_operators(m);
 }

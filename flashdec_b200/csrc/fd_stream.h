@@ -1,0 +1,81 @@
+// Shared by the bounded-cache attention kernels (fd_window_attention,
+// fd_scored_decode): launch parameters and the key range of a block of query
+// rows.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace fd {
+
+struct StreamParams {
+  const void* q;
+  int64_t qs0, qs1, qs2;
+  void* out;
+  int64_t os0, os1, os2;
+  const void* k;
+  int64_t ks0, ks1, ks2, ks3;
+  const void* v;
+  int64_t vs0, vs1, vs2, vs3;
+  const void* bt;
+  int64_t bts0, bts1;
+  const void* sl;
+  int64_t sls;
+  const void* qstart;  // null: one query per sequence
+  int64_t qss;
+  float* scores;  // null: no scores kept
+  int64_t scs0, scs1, scs2;
+  int bt64, sl64, qs64;
+  int num_seqs, num_tokens, hq, hkv, group;
+  int bs_log2, num_blocks, max_blocks;
+  int window, sinks;
+  int row_blocks;  // grid extent of the row-block axis
+  int splits;      // CTAs per (sequence, KV head, row block)
+  int vec;         // rows of K and V are 16-byte aligned and contiguous
+  float scale_log2;
+  float* part_acc;  // [row = token * hq + head][split][D]
+  float* part_ml;   // [row][split][2]: max (base 2), sum
+  float* raw;       // [row][raw_tokens]: scaled scores (base 2)
+  float* lse;       // [row]: max + log2(sum)
+  int64_t raw_tokens;
+  int* status;
+};
+
+// The sequence's queries: rows [q0, q0 + qlen) of q, tokens [n - qlen, n).
+struct StreamSeq {
+  int q0, qlen, n;
+};
+
+// The keys that rows [r0, r1) of a sequence's (query, group head) rows can
+// see, as a list of cache pages: `sink_pages` from position 0, then the pages
+// from `win_page` to the one of the last query.  Adjoining ranges are one
+// (sink_pages 0, win_page 0), so no key is listed twice.
+struct StreamRange {
+  int pos0, pos1;      // positions of the first and the last row's query
+  int lo;              // first key in the first row's window
+  int sink_end;        // sinks seen: [0, sink_end)
+  int sink_pages, win_page, pages;
+
+  __host__ __device__ StreamRange(const StreamSeq& s, int r0, int r1, int group, int window,
+                                  int sinks, int bs_log2) {
+    pos0 = s.n - s.qlen + r0 / group;
+    pos1 = s.n - s.qlen + (r1 - 1) / group;
+    lo = pos0 - window + 1 > 0 ? pos0 - window + 1 : 0;
+    sink_end = sinks < pos1 + 1 ? sinks : pos1 + 1;
+    sink_pages = (sink_end + (1 << bs_log2) - 1) >> bs_log2;
+    win_page = lo >> bs_log2;
+    if (pos1 < 0) {  // no row sees a key
+      sink_end = sink_pages = win_page = pages = 0;
+      return;
+    }
+    if (sink_pages >= win_page) {
+      if (sink_pages > 0) win_page = 0;
+      sink_pages = 0;
+    }
+    pages = sink_pages + (pos1 >> bs_log2) + 1 - win_page;
+  }
+  // logical page of list entry i
+  __host__ __device__ int page(int i) const { return i < sink_pages ? i : i - sink_pages + win_page; }
+};
+
+}  // namespace fd

@@ -282,6 +282,114 @@ typedef struct fd_rope_kv_append_args {
 
 int fd_rope_kv_append(const fd_rope_kv_append_args* args, void* cuda_stream);
 
+/* ---- attention over a bounded cache --------------------------------------
+ * No counterpart in the reference: serving streams longer than their cache.
+ * Both entry points take this struct.
+ *
+ * fd_window_attention: the last q_len(b) of sequence b's seq_len(b) cached
+ * tokens are its queries (their K/V are in the cache already).  A query at
+ * position p sees key j iff j <= p and (j > p - window or j < sinks).
+ * query_start_loc [num_seqs + 1] gives the rows of q (q_len(b) = start[b + 1] -
+ * start[b]); NULL: one query per sequence (num_tokens == num_seqs).  Rows of
+ * q outside every sequence are not written; a query that sees no key (q_len >
+ * seq_len) gets zeros.  Only pages that hold a visible key are read: entries
+ * of block_tables before the window (and past the sinks) may be stale.
+ * max_query_len sizes the launch; longer queries are still computed.
+ *
+ * fd_scored_decode: one query per sequence over all its tokens (window,
+ * sinks, query_start_loc, max_query_len and num_tokens are not read), and
+ * scores[block, kv_head, offset] += the softmax weight the token got, summed
+ * over the query heads of the KV head.  The newest token's score is set, not
+ * added to: what its slot held before is not read.  No two sequences may share
+ * a page (their updates would race). */
+typedef struct fd_stream_attention_args {
+  int32_t struct_size;   /* = sizeof(fd_stream_attention_args) */
+  int32_t dtype;         /* FD_DTYPE_F16 or FD_DTYPE_BF16 */
+  int32_t num_seqs;
+  int32_t num_tokens;    /* rows of q */
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;      /* 64 or 128 */
+  int32_t block_size;    /* 8, 16 or 32 */
+  int32_t num_blocks;
+  int32_t max_blocks_per_seq;
+  int64_t window;        /* >= 1 */
+  int64_t sinks;         /* >= 0 */
+  int32_t max_query_len; /* >= 1 */
+  float sm_scale;
+  const void* q;         /* [num_tokens, num_q_heads, head_dim] */
+  int64_t q_stride[3];
+  void* out;             /* as q */
+  int64_t out_stride[3];
+  const void* k_cache;   /* [block, kv_head, token, dim] */
+  int64_t k_stride[4];
+  const void* v_cache;
+  int64_t v_stride[4];
+  const void* block_tables; /* [num_seqs, max_blocks_per_seq] */
+  int64_t block_tables_stride[2];
+  const void* seq_lens;  /* [num_seqs] */
+  int64_t seq_lens_stride;
+  const void* query_start_loc; /* [num_seqs + 1] or NULL */
+  int64_t query_start_loc_stride;
+  int32_t block_tables_index;  /* FD_INDEX_I32 / FD_INDEX_I64 */
+  int32_t seq_lens_index;
+  int32_t query_start_loc_index;
+  int32_t reserved;
+  float* scores;         /* [block, kv_head, token] fp32; fd_scored_decode only */
+  int64_t scores_stride[3];
+  void* scratch;         /* fd_*_workspace bytes, 16-byte aligned, no initialisation */
+  size_t scratch_bytes;
+} fd_stream_attention_args;
+
+int fd_window_attention_workspace(const fd_stream_attention_args* args, size_t* scratch_bytes);
+int fd_window_attention(const fd_stream_attention_args* args, void* cuda_stream);
+int fd_scored_decode_workspace(const fd_stream_attention_args* args, size_t* scratch_bytes);
+int fd_scored_decode(const fd_stream_attention_args* args, void* cuda_stream);
+
+/* fd_evict_tokens: per sequence b and KV head, copy at most `budget` of the
+ * cached tokens' K, V and score to the pages new_block_tables[b] names, in
+ * their order: all of them when seq_len <= budget, else the first `sinks`, the
+ * last `recent` and the budget - sinks - recent best-scored of the rest (equal
+ * scores: the lower position first; NaN ranks above every number, -0 equals
+ * +0).  kept[b, head, i] = the position that went to place i (-1 from
+ * new_seq_lens[b] = min(seq_len, budget) on).  The source pages stay as they
+ * are; no new page may be a source page of any sequence or a new page of
+ * another. */
+typedef struct fd_evict_tokens_args {
+  int32_t struct_size;   /* = sizeof(fd_evict_tokens_args) */
+  int32_t elem_bytes;    /* of K and V: 2 */
+  int32_t num_seqs;
+  int32_t num_kv_heads;
+  int32_t head_dim;      /* 64 or 128 */
+  int32_t block_size;    /* 8, 16 or 32 */
+  int32_t num_blocks;
+  int32_t max_blocks_per_seq;
+  int32_t max_new_blocks_per_seq;  /* * block_size >= min(budget, longest seq_len) */
+  int32_t budget;        /* >= 1 */
+  int32_t sinks;         /* >= 0 */
+  int32_t recent;        /* >= 0, sinks + recent <= budget */
+  void* k_cache;
+  int64_t k_stride[4];
+  void* v_cache;
+  int64_t v_stride[4];
+  float* scores;
+  int64_t scores_stride[3];
+  const void* block_tables;
+  int64_t block_tables_stride[2];
+  const void* seq_lens;
+  int64_t seq_lens_stride;
+  const void* new_block_tables; /* [num_seqs, max_new_blocks_per_seq] */
+  int64_t new_block_tables_stride[2];
+  int32_t block_tables_index;
+  int32_t seq_lens_index;
+  int32_t new_block_tables_index;
+  int32_t new_seq_lens_index;
+  int32_t* kept;         /* [num_seqs, num_kv_heads, budget], contiguous */
+  void* new_seq_lens;    /* [num_seqs], contiguous */
+} fd_evict_tokens_args;
+
+int fd_evict_tokens(const fd_evict_tokens_args* args, void* cuda_stream);
+
 /* ---- misc ---------------------------------------------------------------- */
 const char* fd_error_string(int code);
 int fd_version(void);
