@@ -25,7 +25,7 @@ INCLUDE = REPO / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libflashdec_b200.so"
 SOURCES = ["fd_host.cu", "fd_attention.cu", "fd_wave_decode.cu", "fd_rope_append.cu", "fd_static.cu", "fd_selftest.cu",
-           "fd_stream_attention.cu", "fd_evict.cu"]
+           "fd_stream_attention.cu", "fd_prompt_attention.cu", "fd_evict.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr",
          "-I", str(INCLUDE), "-I", str(CSRC)]

@@ -218,7 +218,8 @@ bool get_cache_tensor_map(const CacheDesc& d, CUtensorMap* out, int perm[4]) {
   std::stable_sort(ax.begin(), ax.end(),
                    [](const Axis& a, const Axis& b) { return a.stride_bytes < b.stride_bytes; });
   const bool halves =
-      d.head_dim == 128 && (d.block_size == 16 || d.block_size == 8 || d.plane_box != 0);
+      d.head_dim == 128 && d.plane_box >= 0 &&
+      (d.block_size == 16 || d.block_size == 8 || d.plane_box != 0);
   std::array<Axis, 4> all;
   int n = 0;
   for (const Axis& a : ax) {

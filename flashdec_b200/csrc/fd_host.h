@@ -33,7 +33,8 @@ struct CacheDesc {
   int num_blocks;
   int64_t stride[4];    // block, head, token, dim (elements)
   int plane_box = 0;    // head_dim 128: the half axis for every page size, so one
-                        // box moves a whole page plane (also 32-token pages)
+                        // box moves a whole page plane (also 32-token pages);
+                        // -1: for none, one box per (page, 64-dim half)
 };
 
 // Encode (or fetch from the cache) a tiled tensor map over `d` with 128B

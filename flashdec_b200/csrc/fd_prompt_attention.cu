@@ -1,0 +1,598 @@
+// fd_window_attention for many queries per sequence (prompt chunks), on the
+// 5th-generation tensor cores.
+#include <algorithm>
+#include <cstring>
+#include <type_traits>
+
+#include "../../include/flashdec_b200.h"
+#include "fd_host.h"
+#include "fd_ptx.cuh"
+#include "fd_stream.h"
+#include "fd_stream.cuh"
+#include "fd_tile.cuh"
+
+namespace fd {
+namespace {
+
+// One CTA: 256 query rows (row = query x head of the group) of a (sequence, KV
+// head) as two groups of 128, against the list of cache pages they see in
+// tiles of 128 keys.  Per group: S = Q K^T (M 128, N 128) into TMEM, one
+// thread per row takes it from there, writes P = exp2(S - m) back over S in the
+// cache's type, and O += P V accumulates in TMEM with P as the TMEM operand.
+// The two groups alternate, so the tensor pipe works on one while the other
+// does its softmax.
+//
+//   warp 0      TMA producer: K and V tiles alternate through a ring of slots
+//   warp 1      issues the tcgen05.mma (one thread)
+//   warp 2      V tiles with keys that some row does not see: rows that no row
+//               sees are zeroed, and an infinity or NaN in another raises the
+//               CTA's `careful` flag
+//   warps 4-7   softmax and epilogue of rows 0-127
+//   warps 8-11  the same of rows 128-255
+//
+// TMEM columns: S/P of group g at 128 g, O of group g at 256 + 128 g.
+constexpr int kPromptThreads = 384;
+constexpr int kRows = 256;
+constexpr int kKeys = 128;
+
+template <int D>
+struct PromptSmem {
+  static constexpr int kSlots = D == 128 ? 4 : 8;
+  static constexpr uint32_t kHalf = 128 * 128;             // [128 rows][64 dims]
+  static constexpr uint32_t kOperand = (D / 64) * kHalf;   // a Q group or a K or V tile
+  static constexpr uint32_t kRing = 2 * kOperand;          // offset: two Q groups first
+  static constexpr uint32_t kBars = kRing + kSlots * kOperand;
+  static constexpr size_t kBytes = kBars + 512 + 1024;     // barriers; alignment
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 128 consecutive fp32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+#define R4(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
+#define R16(i) R4(i), R4(i + 4), R4(i + 8), R4(i + 12)
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : R16(0), R16(16), R16(32), R16(48), R16(64), R16(80), R16(96), R16(112)
+      : "r"(taddr)
+      : "memory");
+#undef R16
+#undef R4
+}
+
+// 32 columns of this thread's TMEM lane <- registers.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// D[tmem] (+)= A[tmem] x B[smem desc]; issued by one thread.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+}
+
+// The first x bits, clamped to [0, 32].
+__device__ __forceinline__ uint32_t low_bits(int x) {
+  return x <= 0 ? 0u : (x >= 32 ? 0xffffffffu : (1u << x) - 1u);
+}
+
+// Wait for a barrier's phase whatever the abort flag says: copies in flight
+// have to land before the CTA's shared memory is given up.
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < kWaitLimitNs) {
+  }
+}
+
+// What a row sees, in list coordinates (entry i of tile t is key list place
+// 128 t + i): [0, sink_end) and [w0, w1].
+struct RowView {
+  int sink_end, w0, w1;
+};
+__device__ __forceinline__ RowView view_of(const StreamParams& p, const StreamRange& rg, int pos) {
+  const int shift = (rg.sink_pages - rg.win_page) << p.bs_log2;
+  RowView v;
+  v.sink_end = min(p.sinks, pos + 1);
+  v.w0 = max(pos - p.window + 1, 0) + shift;
+  v.w1 = pos + shift;
+  return v;
+}
+
+// One row at a time by one warp, key by key, with plain loads: the way out
+// when a page id is bad or a value that part of the rows must not see is not
+// finite.  Same result as the tiles up to rounding.
+template <typename T, int D>
+__device__ __noinline__ void careful_rows(const StreamParams& p, const StreamSeq& s, int b, int h, int row0,
+                                          int rows, int lane) {
+  for (int r = row0; r < row0 + rows; ++r) {
+    const int qt = r / p.group;
+    const int head = h * p.group + r - qt * p.group;
+    const int pos = s.n - s.qlen + qt;
+    float q[D / 32], o[D / 32], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      q[i] = to_f32<T>(static_cast<const T*>(p.q)[(s.q0 + qt) * p.qs0 + head * p.qs1 + (lane + 32 * i) * p.qs2]);
+      o[i] = 0.f;
+    }
+    const int lo = max(pos - p.window + 1, 0);
+    for (int key = min(p.sinks, lo) > 0 ? 0 : lo; key <= pos; ++key) {
+      if (key >= p.sinks && key < lo) key = lo;
+      const int64_t id =
+          load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(key >> p.bs_log2) * p.bts1);
+      if (id < 0 || id >= p.num_blocks) continue;
+      const int off = key & ((1 << p.bs_log2) - 1);
+      const T* k = static_cast<const T*>(p.k) + id * p.ks0 + h * p.ks1 + off * p.ks2;
+      const T* v = static_cast<const T*>(p.v) + id * p.vs0 + h * p.vs1 + off * p.vs2;
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) x += q[i] * to_f32<T>(k[(lane + 32 * i) * p.ks3]);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      x *= p.scale_log2;
+      const float mn = fmaxf(m, x);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float alpha = exp2f(m - base), w = exp2f(x - base);
+      m = mn;
+      l = l * alpha + w;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) o[i] = o[i] * alpha + w * to_f32<T>(v[(lane + 32 * i) * p.vs3]);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + (lane + 32 * i) * p.os2] =
+          from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_kernel(const __grid_constant__ StreamParams p, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const int4 kperm, const int4 vperm) {
+  using SM = PromptSmem<D>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kSlots = SM::kSlots;
+  constexpr int kHalves = D / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + SM::kBars);
+  uint64_t* full = bars;                // [slot] TMA bytes
+  uint64_t* empty = full + kSlots;      // [slot] the products that read it are done
+  uint64_t* v_ready = empty + kSlots;   // [slot] V checked
+  uint64_t* q_ready = v_ready + kSlots; // [group]
+  uint64_t* s_full = q_ready + 2;       // [group] S in TMEM
+  uint64_t* p_ready = s_full + 2;       // [group] P in TMEM (and O rescaled)
+  uint64_t* pv_done = p_ready + 2;      // [group] O holds the tile
+  uint64_t* drained = pv_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+  volatile int* careful = abort_flag + 1;  // [2], by parity of the row block
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const int h = blockIdx.y;
+  const int b = blockIdx.z;
+
+  if (tid == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(smem_u32(&full[i]), 1);
+      mbar_init(smem_u32(&empty[i]), 1);
+      mbar_init(smem_u32(&v_ready[i]), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(smem_u32(&q_ready[g]), 128);
+      mbar_init(smem_u32(&s_full[g]), 1);
+      mbar_init(smem_u32(&p_ready[g]), 128);
+      mbar_init(smem_u32(&pv_done[g]), 1);
+    }
+    mbar_init(smem_u32(drained), 1);
+    fence_mbar_init();
+    *abort_flag = 0;
+    careful[0] = careful[1] = 0;
+  }
+  if (warp == 3) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&tmap_k);
+    prefetch_tensormap(&tmap_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  const StreamSeq s = sequence_of(p, b);
+  const int rows_all = s.qlen * p.group;
+  const int bs = 1 << p.bs_log2;
+  const int tile_pages = kKeys >> p.bs_log2;
+  auto range_of = [&](int rb) {
+    return StreamRange(s, rb * kRows, min(rb * kRows + kRows, rows_all), p.group, p.window, p.sinks, p.bs_log2);
+  };
+  // every row of the block sees every key of tile t
+  auto interior = [&](const StreamRange& rg, int t) {
+    const RowView first = view_of(p, rg, rg.pos0), last = view_of(p, rg, rg.pos1);
+    return rg.pos0 >= 0 && ((t + 1) * kKeys <= first.sink_end ||
+                            (t * kKeys >= last.w0 && (t + 1) * kKeys - 1 <= first.w1));
+  };
+
+  if (warp == 0) {
+    // ======== producer: lane = (page of the tile, 64-dim half) ========
+    const uint64_t policy = l2_policy_evict_first();
+    const int my_half = lane & (kHalves - 1);
+    const int my_page = lane / kHalves;
+    uint32_t n = 0;  // tiles of either kind issued so far
+    bool ok = true;
+    for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
+      const StreamRange rg = range_of(rb);
+      const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      auto look = [&](int t) -> int64_t {  // -2: no page there
+        const int i = t * tile_pages + my_page;
+        if (my_page >= tile_pages || i >= rg.pages) return -2;
+        return load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(rg.page(i)) * p.bts1);
+      };
+      int64_t next = look(0);
+      for (int t = 0; ok && t < tiles; ++t) {
+        const int64_t id = next;
+        if (t + 1 < tiles) next = look(t + 1);
+        const bool valid = id >= 0 && id < p.num_blocks;
+        if (id != -2 && !valid) {
+          careful[round & 1] = round + 1;
+          atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
+        }
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, valid));
+        for (int kind = 0; ok && kind < 2; ++kind, ++n) {
+          const int slot = n % kSlots;
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[slot]), ((n / kSlots) & 1) ^ 1, p.status, abort_flag));
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&full[slot]);
+          if (lane == 0) mbar_arrive_expect_tx(bar, boxes * (bs * 128));
+          __syncwarp();
+          if (valid) {
+            const int4 perm = kind ? vperm : kperm;
+            const int blk = static_cast<int>(id);
+            tma_load_4d(smem_u32(smem + SM::kRing + slot * SM::kOperand + my_half * SM::kHalf) + my_page * (bs * 128),
+                        kind ? &tmap_v : &tmap_k, bar, my_half * 64, tmap_coord(perm.x, h, blk),
+                        tmap_coord(perm.y, h, blk), tmap_coord(perm.z, h, blk), policy);
+          }
+        }
+      }
+    }
+    if (*abort_flag) {
+      for (uint32_t i = n > kSlots ? n - kSlots : 0; i < n; ++i)
+        drain_wait(smem_u32(&full[i % kSlots]), (i / kSlots) & 1);
+    }
+  } else if (warp == 1) {
+    // ======== tcgen05.mma, one thread ========
+    if (lane == 0) {
+      constexpr uint32_t kIdO = umma_idesc_f16(kBf16, true, 128, D);
+      uint32_t n = 0, it = 0;  // slots taken, tiles done (per group)
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = ok && mbar_wait(smem_u32(bar), parity, p.status, abort_flag);
+        return ok;
+      };
+      for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
+        const StreamRange rg = range_of(rb);
+        const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+        const int groups = rows_all - rb * kRows > 128 ? 2 : 1;
+        auto keys16 = [&](int t) {  // 16-key steps of tile t
+          return (min(kKeys, (rg.pages << p.bs_log2) - t * kKeys) + 15) >> 4;
+        };
+        auto issue_s = [&](int g, int t, uint32_t slot) {
+          const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, 16 * keys16(t));
+          const uint32_t qa = smem_u32(smem + g * SM::kOperand);
+          const uint32_t ka = smem_u32(smem + SM::kRing + slot * SM::kOperand);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = (k >> 2) * SM::kHalf + (k & 3) * 32u;
+            umma_f16(tmem + 128 * g, umma_smem_desc(qa + off, 16, 1024, 2),
+                     umma_smem_desc(ka + off, 16, 1024, 2), idesc, k > 0);
+          }
+          umma_commit(smem_u32(&s_full[g]));
+        };
+        if (tiles == 0) continue;
+        for (int g = 0; ok && g < groups; ++g) wait(&q_ready[g], round & 1);
+        if (!wait(&full[n % kSlots], (n / kSlots) & 1)) break;
+        tc_fence_after();
+        for (int g = 0; g < groups; ++g) issue_s(g, 0, n % kSlots);
+        umma_commit(smem_u32(&empty[n % kSlots]));
+        ++n;
+        for (int t = 0; t < tiles; ++t, ++it) {
+          const uint32_t vs = n % kSlots, ks = (n + 1) % kSlots;
+          if (!wait(&v_ready[vs], (n / kSlots) & 1)) break;
+          if (t + 1 < tiles && !wait(&full[ks], ((n + 1) / kSlots) & 1)) break;
+          const uint32_t va = smem_u32(smem + SM::kRing + vs * SM::kOperand);
+          for (int g = 0; ok && g < groups; ++g) {
+            if (!wait(&p_ready[g], it & 1)) break;
+            tc_fence_after();
+            const int steps = keys16(t);
+            for (int k = 0; k < steps; ++k)
+              umma_f16_ts(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k,
+                          umma_smem_desc(va + k * 2048, SM::kHalf, 1024, 2), kIdO, t > 0 || k > 0);
+            umma_commit(smem_u32(&pv_done[g]));
+            // The tensor pipe takes this thread's products in order: S of the
+            // next tile lands on P only after the product above has read it.
+            if (t + 1 < tiles) issue_s(g, t + 1, ks);
+          }
+          if (!ok) break;
+          umma_commit(smem_u32(&empty[vs]));
+          if (t + 1 < tiles) umma_commit(smem_u32(&empty[ks]));
+          n += t + 1 < tiles ? 2 : 1;
+        }
+      }
+      if (*abort_flag) {  // products in flight still read shared memory and write TMEM
+        umma_commit(smem_u32(drained));
+        drain_wait(smem_u32(drained), 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ======== V tiles on the edge of what the rows see ========
+    constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
+    uint32_t n = 0;
+    bool ok = true;
+    for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
+      const StreamRange rg = range_of(rb);
+      const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      const int shift = (rg.sink_pages - rg.win_page) << p.bs_log2;
+      for (int t = 0; ok && t < tiles; ++t) {
+        ++n;  // K
+        const int slot = n % kSlots;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), (n / kSlots) & 1, p.status, abort_flag));
+        if (!ok) break;
+        if (!interior(rg, t)) {
+          uint8_t* v = smem + SM::kRing + slot * SM::kOperand;
+          const int end = min(kKeys, (((rg.pages << p.bs_log2) - t * kKeys) + 15) & ~15);
+          bool odd = false;
+          for (int k0 = 0; k0 < end; k0 += 4) {
+            const int key = k0 + (lane >> 3);  // 8 lanes per 128-byte row
+            const int place = t * kKeys + key;
+            // seen by some row of the block
+            const bool seen = place < (rg.pages << p.bs_log2) &&
+                              (place < rg.sink_end || (place >= rg.lo + shift && place <= rg.pos1 + shift));
+#pragma unroll
+            for (int hf = 0; hf < kHalves; ++hf) {
+              uint4* x = reinterpret_cast<uint4*>(v + hf * SM::kHalf + key * 128 + (lane & 7) * 16);
+              if (!seen) {
+                *x = make_uint4(0u, 0u, 0u, 0u);
+              } else {
+                const uint4 y = *x;
+                odd |= nonfinite16(y.x, kExp) | nonfinite16(y.y, kExp) | nonfinite16(y.z, kExp) |
+                       nonfinite16(y.w, kExp);
+              }
+            }
+          }
+          if (__any_sync(0xffffffffu, odd) && lane == 0) careful[round & 1] = round + 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(smem_u32(&v_ready[slot]));
+        ++n;  // V
+      }
+    }
+  } else if (warp >= 4) {
+    // ======== softmax: thread = row = TMEM lane ========
+    const int g = (warp - 4) >> 2;
+    const int gt = tid - 128 - 128 * g;  // row of the group
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lane_addr + 128 * g, o_addr = lane_addr + 256 + 128 * g;
+    // a scale of 0 (uniform weights) stays above it: -inf * 0 is NaN
+    const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
+    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // the scale's sign goes to q
+    uint32_t it = 0;
+    bool ok = true;
+    for (int rb = blockIdx.x, round = 0; ok && rb * kRows + 128 * g < rows_all; rb += gridDim.x, ++round) {
+      const StreamRange rg = range_of(rb);
+      const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      const int grow0 = rb * kRows + 128 * g;
+      // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane ----
+      constexpr int kChunks = D / 8;
+#pragma unroll
+      for (int i = 0; i < kChunks; ++i) {
+        const int e = gt + 128 * i;
+        const int r = e / kChunks, c = e % kChunks;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (grow0 + r < rows_all) {
+          const int qt = (grow0 + r) / p.group;
+          const int head = h * p.group + (grow0 + r) - qt * p.group;
+          const T* src = static_cast<const T*>(p.q) + (s.q0 + qt) * p.qs0 + head * p.qs1 + c * 8 * p.qs2;
+          x = p.qs2 == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0
+                  ? *reinterpret_cast<const uint4*>(src)
+                  : gather8(src, p.qs2);
+          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+        }
+        *reinterpret_cast<uint4*>(smem + g * SM::kOperand + (c >> 3) * SM::kHalf + r * 128 +
+                                  (((c & 7) ^ (r & 7)) << 4)) = x;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(&q_ready[g]));
+
+      const int row = grow0 + gt;
+      const int qt = min(row, rows_all - 1) / p.group;
+      const RowView view = view_of(p, rg, s.n - s.qlen + qt);
+      float m = -INFINITY, l = 0.f;  // m in score units: P = exp2((S - m) scale)
+      for (int t = 0; t < tiles; ++t, ++it) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[g]), it & 1, p.status, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        float v[128];
+        tmem_ld128(s_addr, v);
+        if (!interior(rg, t)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int at = t * kKeys + 32 * c;
+            const uint32_t on = low_bits(view.sink_end - at) |
+                                (low_bits(view.w1 + 1 - at) & ~low_bits(view.w0 - at));
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[32 * c + j] = (on >> j) & 1u ? v[32 * c + j] : -INFINITY;
+          }
+        }
+        float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // The reference maximum follows the running one only when it is 2^8
+        // behind: P stays below 2^8, and O is rescaled rarely.
+        const bool first = m == -INFINITY;
+        const bool behind = !first && (top - m) * scale > 8.f;
+        float alpha = 1.f;
+        if (first) m = top;
+        if (behind) {
+          alpha = ex2((m - top) * scale);
+          m = top;
+          l *= alpha;
+        }
+        if (__any_sync(0xffffffffu, behind)) {
+          // PV of the tile before has to be in O first
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[g]), (it - 1) & 1, p.status, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_ld32(o_addr + 32 * c, o);
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(o[j] * alpha);
+            tmem_st32(o_addr + 32 * c, w);
+          }
+          tmem_wait_st();
+        }
+        const float base = m == -INFINITY ? 0.f : m * scale;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float a = ex2(fmaf(v[64 * c + 2 * j], scale, -base));
+            const float e = ex2(fmaf(v[64 * c + 2 * j + 1], scale, -base));
+            sum[(2 * j) & 3] += a;
+            sum[(2 * j + 1) & 3] += e;
+            w[j] = pack2<T>(a, e);
+          }
+          tmem_st32(s_addr + 32 * c, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&p_ready[g]));
+      }
+      if (ok && tiles > 0)
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[g]), (it - 1) & 1, p.status, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      if (careful[round & 1] == round + 1) {
+        const int w0 = grow0 + (warp & 3) * 32;
+        careful_rows<T, D>(p, s, b, h, w0, max(0, min(32, rows_all - w0)), lane);
+        continue;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int head = h * p.group + row - qt * p.group;
+      T* dst = static_cast<T*>(p.out) + (s.q0 + qt) * p.os0 + head * p.os1;
+      const bool wide = p.os2 == 1 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0;
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (tiles > 0) {
+          tmem_ld32(o_addr + 32 * c, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = l == 0.f ? 0.f : o[j] * inv;
+        if (row < rows_all) {
+          if (wide) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<uint4*>(dst + 32 * c + 8 * j) =
+                  make_uint4(pack2<T>(o[8 * j], o[8 * j + 1]), pack2<T>(o[8 * j + 2], o[8 * j + 3]),
+                             pack2<T>(o[8 * j + 4], o[8 * j + 5]), pack2<T>(o[8 * j + 6], o[8 * j + 7]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) dst[(32 * c + j) * p.os2] = from_f32<T>(o[j]);
+          }
+        }
+      }
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 3) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D>
+int launch(const StreamParams& p, const CUtensorMap& mk, const CUtensorMap& mv, const int (&kp)[4],
+           const int (&vp)[4], dim3 grid, cudaStream_t stream) {
+  auto kern = prompt_kernel<T, D>;
+  constexpr size_t smem = PromptSmem<D>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e == cudaSuccess)
+    e = launch_pdl(kern, grid, dim3(kPromptThreads), smem, stream, p, mk, mv, make_int4(kp[0], kp[1], kp[2], 0),
+                   make_int4(vp[0], vp[1], vp[2], 0));
+  return cuda_status(e);
+}
+
+}  // namespace
+
+bool prompt_attention(const StreamParams& p, bool bf16, int D, int64_t max_query_len, cudaStream_t stream,
+                      int* rc) {
+  CacheDesc kd;
+  kd.base = p.k;
+  kd.elem_bytes = 2;
+  kd.is_bf16 = bf16;
+  kd.head_dim = D;
+  kd.block_size = 1 << p.bs_log2;
+  kd.num_heads = p.hkv;
+  kd.num_blocks = p.num_blocks;
+  kd.plane_box = -1;
+  CacheDesc vd = kd;
+  vd.base = p.v;
+  const int64_t ks[4] = {p.ks0, p.ks1, p.ks2, p.ks3}, vs[4] = {p.vs0, p.vs1, p.vs2, p.vs3};
+  std::copy(ks, ks + 4, kd.stride);
+  std::copy(vs, vs + 4, vd.stride);
+  CUtensorMap mk, mv;
+  int kp[4], vp[4];
+  if (!get_cache_tensor_map(kd, &mk, kp) || !get_cache_tensor_map(vd, &mv, vp)) return false;
+  const int64_t blocks = (max_query_len * p.group + kRows - 1) / kRows;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 20)), p.hkv, p.num_seqs);
+  if (D == 128) {
+    *rc = bf16 ? launch<__nv_bfloat16, 128>(p, mk, mv, kp, vp, grid, stream)
+               : launch<__half, 128>(p, mk, mv, kp, vp, grid, stream);
+  } else {
+    *rc = bf16 ? launch<__nv_bfloat16, 64>(p, mk, mv, kp, vp, grid, stream)
+               : launch<__half, 64>(p, mk, mv, kp, vp, grid, stream);
+  }
+  return true;
+}
+
+}  // namespace fd

@@ -78,4 +78,10 @@ struct StreamRange {
   __host__ __device__ int page(int i) const { return i < sink_pages ? i : i - sink_pages + win_page; }
 };
 
+// fd_window_attention on tcgen05, for many rows per (sequence, KV head).  False
+// when no tensor map describes the caches (nothing is launched); else *rc is
+// the launch's status.
+bool prompt_attention(const StreamParams& p, bool bf16, int head_dim, int64_t max_query_len,
+                      cudaStream_t stream, int* rc);
+
 }  // namespace fd

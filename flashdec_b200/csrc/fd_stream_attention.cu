@@ -8,6 +8,7 @@
 #include "../../include/flashdec_b200.h"
 #include "fd_host.h"
 #include "fd_ptx.cuh"
+#include "fd_stream.cuh"
 #include "fd_stream.h"
 
 namespace fd {
@@ -29,24 +30,6 @@ constexpr size_t split_smem_bytes() {
   return ring_bytes<D>() + static_cast<size_t>(kM) * 16 * D * 2;
 }
 
-__device__ __forceinline__ StreamSeq sequence_of(const StreamParams& p, int b) {
-  StreamSeq s;
-  const int64_t cap = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
-  const int64_t n = load_index(p.sl, p.sl64, b * p.sls);
-  s.n = static_cast<int>(min(max(n, int64_t(0)), cap));
-  s.q0 = b;
-  s.qlen = 1;
-  if (p.qstart) {
-    const int64_t a = load_index(p.qstart, p.qs64, b * p.qss);
-    const int64_t z = load_index(p.qstart, p.qs64, (b + 1) * p.qss);
-    const int64_t nt = p.num_tokens;
-    const int64_t a1 = min(max(a, int64_t(0)), nt);
-    s.q0 = static_cast<int>(a1);
-    s.qlen = static_cast<int>(min(max(z, a1), nt) - a1);
-  }
-  return s;
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
@@ -65,19 +48,6 @@ __device__ __forceinline__ void cp_async_wait() {
 template <int D>
 __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
   return r * (D * 2) + ((c ^ (r & 7)) << 4);
-}
-
-// 8 elements of a strided row as one 16-byte value.
-template <typename T>
-__device__ __forceinline__ uint4 gather8(const T* src, int64_t stride) {
-  __align__(16) T el[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) el[i] = src[i * stride];
-  return *reinterpret_cast<const uint4*>(el);
-}
-
-__device__ __forceinline__ bool nonfinite16(uint32_t w, uint32_t exp_mask) {
-  return (w & exp_mask) == exp_mask || ((w >> 16) & exp_mask) == exp_mask;
 }
 
 // ---------------------------------------------------------------------------
@@ -508,6 +478,8 @@ struct StreamPlan {
   int m16;         // 16-row tiles per CTA: 1 or 2
   int row_blocks;  // grid extent
   int splits;
+  bool prompt;     // many rows: prompt_attention, where it takes the layout
+  int64_t max_query;
   int64_t raw_tokens;
   size_t acc_bytes, ml_bytes, raw_bytes, lse_bytes;
   size_t bytes() const { return acc_bytes + ml_bytes + raw_bytes + lse_bytes; }
@@ -551,6 +523,8 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
                          ? 1
                          : std::min<int64_t>(a->max_query_len, std::max<int64_t>(tokens, 1));
   const int64_t rows = mq * group;
+  pl.max_query = mq;
+  pl.prompt = rows >= 256;
   pl.m16 = rows > 16 ? 2 : 1;
   const int per = 16 * pl.m16;
   pl.row_blocks = static_cast<int>(
@@ -671,6 +645,7 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   p.status = status;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   const bool bf16 = a->dtype == FD_DTYPE_BF16;
+  if (pl.prompt && prompt_attention(p, bf16, a->head_dim, pl.max_query, stream, &rc)) return rc;
   if (a->head_dim == 128) {
     rc = bf16 ? launch_typed<__nv_bfloat16, 128>(p, pl, stream) : launch_typed<__half, 128>(p, pl, stream);
   } else {
