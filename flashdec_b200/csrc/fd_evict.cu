@@ -28,7 +28,8 @@ struct EvictParams {
   int bt64, sl64, nbt64, nl64;
   int hkv, bs_log2, num_blocks, max_blocks, max_new_blocks;
   int budget, sinks, recent;
-  int vec;  // rows are 16-byte aligned and contiguous
+  int vec;        // rows are 16-byte aligned and contiguous
+  int score_vec;  // four scores of a page: one 16-byte load
   int* status;
 };
 
@@ -59,149 +60,317 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 }
 
 constexpr int kSelectThreads = 1024;
+constexpr int kBins = 2048;
+constexpr int kMaxCluster = 8;
+constexpr int kSelectWords = 3 * kBins;  // histograms of the three digits
 
-// One CTA per (KV head, sequence).  The threshold key is found digit by digit
-// (four 8-bit histograms over the tokens that are neither sinks nor recent);
-// then one pass in order keeps the protected tokens, the keys above the
-// threshold and the first of the keys equal to it.
-__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
-  __shared__ int hist[256];
-  __shared__ int pick[2];  // digit, keys still to take among that digit's
-  __shared__ int wsum[2][32];
+// Exclusive sum over the threads of a CTA (in thread order) and the total.
+__device__ __forceinline__ int block_exclusive(int x, int* warp_sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int y = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, y, d);
+    if (lane >= d) y += z;
+  }
+  if (lane == 31) warp_sums[warp] = y;
+  __syncthreads();
+  int w = warp_sums[lane];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, w, d);
+    if (lane >= d) w += z;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  __syncthreads();  // warp_sums may be written again
+  return (warp > 0 ? before : 0) + y - x;
+}
+
+// One cluster per (KV head, sequence), each CTA a run of its tokens, whose keys
+// it keeps in shared memory when they fit (`key_cap`).  The threshold key is
+// found digit by digit (11, 11 and 10 bits): each CTA counts its keys, the
+// cluster's counts are added through distributed shared memory, and every CTA
+// finds the same digit.  Then one pass in order keeps the protected tokens
+// (sinks and recent), the keys above the threshold and the first of the keys
+// equal to it.  The counts are whole numbers: no order of the atomics changes
+// the result.
+__global__ void __launch_bounds__(kSelectThreads)
+    evict_select_kernel(const __grid_constant__ EvictParams p, int key_cap) {
+  extern __shared__ __align__(16) int dyn[];
+  int* hist = dyn;                                                // [3][kBins]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(dyn + kSelectWords);  // [key_cap]
+  __shared__ int warp_sums[32];
+  __shared__ int pick[2];    // digit, keys still to take among that digit's
+  __shared__ int counts[2];  // this CTA's sure keeps and threshold keys
   const int tid = threadIdx.x;
-  const int warp = tid >> 5;
-  const int lane = tid & 31;
-  const int h = blockIdx.x;
-  const int b = blockIdx.y;
+  const int ranks = gridDim.x;  // the cluster
+  const int rank = blockIdx.x;
+  const int h = blockIdx.y;
+  const int b = blockIdx.z;
+  for (int i = tid; i < kSelectWords; i += kSelectThreads) hist[i] = 0;
   pdl_wait();
   pdl_launch_dependents();
   const int n = length_of(p, b);
   const int m = kept_of(p, n);
   int* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
-  if (h == 0 && tid == 0) {
+  if (h == 0 && rank == 0 && tid == 0) {
     if (p.nl64) {
       static_cast<int64_t*>(p.new_lens)[b] = m;
     } else {
       static_cast<int*>(p.new_lens)[b] = m;
     }
   }
-  for (int i = m + tid; i < p.budget; i += kSelectThreads) kept[i] = -1;
-  if (n <= m) {
-    for (int i = tid; i < m; i += kSelectThreads) kept[i] = i;
+  for (int i = m + rank * kSelectThreads + tid; i < p.budget; i += ranks * kSelectThreads) kept[i] = -1;
+  if (n <= m) {  // the whole cluster
+    for (int i = rank * kSelectThreads + tid; i < m; i += ranks * kSelectThreads) kept[i] = i;
     return;
   }
   const int sinks = min(p.sinks, m);
   const int recent = min(p.recent, m - sinks);
   const int mid0 = sinks, mid1 = n - recent;
-  auto key_of = [&](int t) -> uint32_t {
+  const int run = ((n + ranks - 1) / ranks + 7) & ~7;
+  const int t0 = min(rank * run, n), t1 = min(t0 + run, n);
+  const bool cached = run <= key_cap;
+  const int mask = (1 << p.bs_log2) - 1;
+  // keys of the four tokens from t (t % 4 == 0: they share a page)
+  auto load4 = [&](int t, uint32_t(&k)[4]) {
     const int64_t id =
         page_of(p, p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(t >> p.bs_log2) * p.bts1);
-    if (id < 0) return 0u;
-    return score_key(p.scores[id * p.scs0 + h * p.scs1 + (t & ((1 << p.bs_log2) - 1)) * p.scs2]);
+    if (id < 0) {
+      k[0] = k[1] = k[2] = k[3] = 0u;
+      return;
+    }
+    const float* src = p.scores + id * p.scs0 + h * p.scs1 + (t & mask) * p.scs2;
+    if (p.score_vec) {
+      const float4 x = *reinterpret_cast<const float4*>(src);
+      k[0] = score_key(x.x);
+      k[1] = score_key(x.y);
+      k[2] = score_key(x.z);
+      k[3] = score_key(x.w);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = score_key(src[i * p.scs2]);
+    }
   };
-  // the (m - sinks - recent)-th greatest key of [mid0, mid1)
+  auto four = [&](int t, uint32_t(&k)[4]) {
+    if (cached) {
+      const uint4 x = *reinterpret_cast<const uint4*>(keys + (t - t0));
+      k[0] = x.x;
+      k[1] = x.y;
+      k[2] = x.z;
+      k[3] = x.w;
+    } else {
+      load4(t, k);
+    }
+  };
+  if (cached) {
+    for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {
+      uint32_t k[4];
+      load4(t, k);
+      *reinterpret_cast<uint4*>(keys + (t - t0)) = make_uint4(k[0], k[1], k[2], k[3]);
+    }
+  }
+  __syncthreads();
+  // ---- the (m - sinks - recent)-th greatest key of [mid0, mid1) ----
   int need = m - sinks - recent;
+  const bool any_mid = need > 0;
   uint32_t prefix = 0;
-  for (int shift = 24; need > 0 && shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int t = mid0 + tid; t < mid1; t += kSelectThreads) {
-      const uint32_t k = key_of(t);
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))
-        atomicAdd(&hist[(k >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int left = need, d = 255;
-      while (d > 0 && hist[d] < left) left -= hist[d--];
-      pick[0] = d;
-      pick[1] = left;
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(pick[0]) << shift;
-    need = pick[1];
-    __syncthreads();
-  }
-  // `need` keys equal to `prefix` are kept, all greater ones
-  const bool any_mid = m - sinks - recent > 0;
-  int base = 0, ties = 0;  // kept and equal keys before this chunk
-  for (int c = 0; c < n; c += kSelectThreads) {
-    const int t = c + tid;
-    const bool mid = t >= mid0 && t < mid1;
-    const uint32_t k = mid && any_mid ? key_of(t) : 0u;
-    const bool sure = t < n && (!mid || (any_mid && k > prefix));
-    const bool tie = mid && any_mid && k == prefix;
-    const uint32_t below = (1u << lane) - 1u;
-    const uint32_t bs = __ballot_sync(0xffffffffu, sure), bt = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) {
-      wsum[0][warp] = __popc(bs);
-      wsum[1][warp] = __popc(bt);
-    }
-    __syncthreads();
-    int ws = 0, wt = 0, all_s = 0, all_t = 0;
-    for (int w = 0; w < kSelectThreads / 32; ++w) {
-      if (w < warp) {
-        ws += wsum[0][w];
-        wt += wsum[1][w];
+  if (any_mid) {
+#pragma unroll 1
+    for (int digit = 0; digit < 3; ++digit) {
+      const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0);
+      const int above = digit == 0 ? 32 : (digit == 1 ? 21 : 10);  // bits found so far lie above
+      int* mine = hist + digit * kBins;
+      for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {
+        uint32_t k[4];
+        four(t, k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t + i >= mid0 && t + i < mid1 && (above == 32 || (k[i] >> above) == (prefix >> above)))
+            atomicAdd(&mine[(k[i] >> shift) & (above - shift == 11 ? 2047 : 1023)], 1);
       }
-      all_s += wsum[0][w];
-      all_t += wsum[1][w];
+      cluster_arrive();
+      cluster_wait();
+      // bins from the top: thread i has bins 2047 - 2 i and 2046 - 2 i
+      const int hi = kBins - 1 - 2 * tid;
+      int c_hi = 0, c_lo = 0;
+      for (int r = 0; r < ranks; ++r) {
+        uint32_t at = map_to_rank(smem_u32(mine + hi - 1), r);
+        int x, y;
+        asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(at) : "memory");
+        c_lo += x;
+        c_hi += y;
+      }
+      int total;
+      const int before = block_exclusive(c_hi + c_lo, warp_sums, total);
+      if (before < need && need <= before + c_hi + c_lo) {  // exactly one thread
+        const bool up = need <= before + c_hi;
+        pick[0] = up ? hi : hi - 1;
+        pick[1] = need - before - (up ? 0 : c_hi);
+      }
+      __syncthreads();
+      prefix |= static_cast<uint32_t>(pick[0]) << shift;
+      need = pick[1];
+      __syncthreads();
     }
-    const int tie_rank = ties + wt + __popc(bt & below);
-    const int ties_before = min(tie_rank, need) - min(ties, need);  // kept ties before t in this chunk
-    const int at = base + ws + __popc(bs & below) + ties_before;
-    if (sure || (tie && tie_rank < need)) {
-      if (at < m) kept[at] = t;
-    }
-    base += all_s + min(ties + all_t, need) - min(ties, need);
-    ties += all_t;
-    __syncthreads();
   }
+  // ---- keep `need` of the keys equal to `prefix` and all greater ones ----
+  auto flags = [&](int t, uint32_t& sure, uint32_t& tie) {
+    uint32_t k[4] = {0u, 0u, 0u, 0u};
+    if (t < t1) four(t, k);
+    sure = tie = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = t + i < t1;
+      const bool mid = t + i >= mid0 && t + i < mid1;
+      sure |= (in && (!mid || (any_mid && k[i] > prefix)) ? 1u : 0u) << i;
+      tie |= (in && mid && any_mid && k[i] == prefix ? 1u : 0u) << i;
+    }
+  };
+  int sure_n = 0, tie_n = 0;
+  for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {
+    uint32_t sure, tie;
+    flags(t, sure, tie);
+    sure_n += __popc(sure);
+    tie_n += __popc(tie);
+  }
+  int total_sure, total_tie;
+  block_exclusive(sure_n, warp_sums, total_sure);
+  block_exclusive(tie_n, warp_sums, total_tie);
+  if (tid == 0) {
+    counts[0] = total_sure;
+    counts[1] = total_tie;
+  }
+  cluster_arrive();
+  cluster_wait();
+  int base = 0, ties = 0;  // sure keeps and threshold keys before this CTA's run
+  for (int r = 0; r < rank; ++r) {
+    int x, y;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(map_to_rank(smem_u32(&counts[0]), r)) : "memory");
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(y) : "r"(map_to_rank(smem_u32(&counts[1]), r)) : "memory");
+    base += x;
+    ties += y;
+  }
+  cluster_arrive();  // nobody reads this CTA's shared memory after the matching wait
+  for (int c = t0; c < t1; c += 4 * kSelectThreads) {
+    uint32_t sure, tie;
+    flags(c + 4 * tid, sure, tie);
+    int total;  // both counts in one sum: at most 4096 of each
+    const int before = block_exclusive(__popc(sure) | (__popc(tie) << 16), warp_sums, total);
+    int s = base + (before & 0xffff), w = ties + (before >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool is_sure = (sure >> i) & 1u, is_tie = (tie >> i) & 1u;
+      if (is_sure || (is_tie && w < need)) kept[s + min(w, need)] = c + 4 * tid + i;
+      s += is_sure;
+      w += is_tie;
+    }
+    base += total & 0xffff;
+    ties += total >> 16;
+  }
+  cluster_wait();
 }
 
 constexpr int kCopyThreads = 256;
+constexpr int kCopyRows = 8;  // rows a warp has in flight
 
-// One warp per kept row: K, V and the score go to the new page.
+// A warp copies K, V and score of 8 kept tokens at a time: lane i < 8 looks up
+// row i's pages, then all rows' loads go out before the first store.
 template <int D>
 __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_constant__ EvictParams p) {
   const int lane = threadIdx.x & 31;
   const int h = blockIdx.y;
   const int b = blockIdx.z;
+  const int mask = (1 << p.bs_log2) - 1;
   pdl_wait();
   pdl_launch_dependents();
   const int m = kept_of(p, length_of(p, b));
-  const int mask = (1 << p.bs_log2) - 1;
   const int* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
-  for (int i = blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); i < m;
-       i += gridDim.x * (kCopyThreads / 32)) {
-    const int t = kept[i];
-    const int64_t src =
-        page_of(p, p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(t >> p.bs_log2) * p.bts1);
-    const int64_t dst =
-        page_of(p, p.nbt, p.nbt64, b * p.nbts0 + static_cast<int64_t>(i >> p.bs_log2) * p.nbts1);
-    if (src < 0 || dst < 0) continue;
-    const uint8_t* k0 = p.k + src * p.ks0 + h * p.ks1 + (t & mask) * p.ks2;
-    uint8_t* k1 = p.k + dst * p.ks0 + h * p.ks1 + (i & mask) * p.ks2;
-    const uint8_t* v0 = p.v + src * p.vs0 + h * p.vs1 + (t & mask) * p.vs2;
-    uint8_t* v1 = p.v + dst * p.vs0 + h * p.vs1 + (i & mask) * p.vs2;
-    if (p.vec) {
-      constexpr int kChunks = D / 8;  // 16-byte chunks of a row
-      if (lane < kChunks) {
-        *reinterpret_cast<uint4*>(k1 + lane * 16) = *reinterpret_cast<const uint4*>(k0 + lane * 16);
-      } else if (lane - kChunks < kChunks) {
-        *reinterpret_cast<uint4*>(v1 + (lane - kChunks) * 16) =
-            *reinterpret_cast<const uint4*>(v0 + (lane - kChunks) * 16);
-      }
-    } else {
-      for (int d = lane; d < D; d += 32) {
-        *reinterpret_cast<uint16_t*>(k1 + d * p.ks3) = *reinterpret_cast<const uint16_t*>(k0 + d * p.ks3);
-        *reinterpret_cast<uint16_t*>(v1 + d * p.vs3) = *reinterpret_cast<const uint16_t*>(v0 + d * p.vs3);
+  const int step = gridDim.x * (kCopyThreads / 32) * kCopyRows;
+  for (int i0 = (blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5)) * kCopyRows; i0 < m; i0 += step) {
+    int64_t src = -1, dst = -1;
+    int t = 0;
+    const int i = i0 + lane;
+    if (lane < kCopyRows && i < m) {
+      t = kept[i];
+      src = page_of(p, p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(t >> p.bs_log2) * p.bts1);
+      dst = page_of(p, p.nbt, p.nbt64, b * p.nbts0 + static_cast<int64_t>(i >> p.bs_log2) * p.nbts1);
+      if (src < 0 || dst < 0) {
+        src = dst = -1;
+      } else {
+        p.scores[dst * p.scs0 + h * p.scs1 + (i & mask) * p.scs2] =
+            p.scores[src * p.scs0 + h * p.scs1 + (t & mask) * p.scs2];
       }
     }
-    if (lane == 0)
-      p.scores[dst * p.scs0 + h * p.scs1 + (i & mask) * p.scs2] =
-          p.scores[src * p.scs0 + h * p.scs1 + (t & mask) * p.scs2];
+    if (p.vec) {
+      constexpr int kChunks = D / 8;      // 16-byte chunks of a row
+      constexpr int kSide = 16 / kChunks; // rows a half warp moves at once: lanes 0-15 K, 16-31 V
+      const bool is_v = lane >= 16;
+      const int c = lane & (kChunks - 1);
+      const int sub = (lane & 15) / kChunks;
+      uint8_t* base = is_v ? p.v : p.k;
+      const int64_t s0 = is_v ? p.vs0 : p.ks0, s1 = is_v ? p.vs1 : p.ks1, s2 = is_v ? p.vs2 : p.ks2;
+      uint4 x[kCopyRows / kSide];
+#pragma unroll
+      for (int j = 0; j < kCopyRows / kSide; ++j) {
+        const int r = j * kSide + sub;
+        const int64_t from = __shfl_sync(0xffffffffu, src, r);
+        const int tok = __shfl_sync(0xffffffffu, t, r);
+        if (from >= 0) x[j] = __ldcs(reinterpret_cast<const uint4*>(base + from * s0 + h * s1 + (tok & mask) * s2 + c * 16));
+      }
+#pragma unroll
+      for (int j = 0; j < kCopyRows / kSide; ++j) {
+        const int r = j * kSide + sub;
+        const int64_t to = __shfl_sync(0xffffffffu, dst, r);
+        if (to >= 0) *reinterpret_cast<uint4*>(base + to * s0 + h * s1 + ((i0 + r) & mask) * s2 + c * 16) = x[j];
+      }
+    } else {
+      for (int r = 0; r < kCopyRows; ++r) {
+        const int64_t from = __shfl_sync(0xffffffffu, src, r), to = __shfl_sync(0xffffffffu, dst, r);
+        const int tok = __shfl_sync(0xffffffffu, t, r);
+        if (to < 0) continue;
+        const uint8_t* k0 = p.k + from * p.ks0 + h * p.ks1 + (tok & mask) * p.ks2;
+        uint8_t* k1 = p.k + to * p.ks0 + h * p.ks1 + ((i0 + r) & mask) * p.ks2;
+        const uint8_t* v0 = p.v + from * p.vs0 + h * p.vs1 + (tok & mask) * p.vs2;
+        uint8_t* v1 = p.v + to * p.vs0 + h * p.vs1 + ((i0 + r) & mask) * p.vs2;
+        for (int d = lane; d < D; d += 32) {
+          *reinterpret_cast<uint16_t*>(k1 + d * p.ks3) = *reinterpret_cast<const uint16_t*>(k0 + d * p.ks3);
+          *reinterpret_cast<uint16_t*>(v1 + d * p.vs3) = *reinterpret_cast<const uint16_t*>(v0 + d * p.vs3);
+        }
+      }
+    }
   }
+}
+
+// Tokens a CTA of the selection holds: about 4096, and no more than a cluster
+// of 8 has to.
+int select(const EvictParams& p, int num_seqs, cudaStream_t stream) {
+  const int64_t cap = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
+  int ranks = 1;
+  while (ranks < kMaxCluster && cap > 4096 * ranks) ranks *= 2;
+  const int64_t run = ((cap + ranks - 1) / ranks + 7) & ~int64_t(7);
+  // past this the keys are read again for every digit
+  const int key_cap = run <= 48 * 1024 ? static_cast<int>(run) : 0;
+  const size_t smem = sizeof(int) * (kSelectWords + static_cast<size_t>(key_cap));
+  cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(smem));
+  if (e != cudaSuccess) return cuda_status(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ranks, p.hkv, num_seqs);
+  cfg.blockDim = dim3(kSelectThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cuda_status(cudaLaunchKernelEx(&cfg, evict_select_kernel, p, key_cap));
 }
 
 }  // namespace
@@ -265,13 +434,14 @@ extern "C" int fd_evict_tokens(const fd_evict_tokens_args* a, void* cuda_stream)
   p.vec = aligned(a->k_cache, a->k_stride) && aligned(a->v_cache, a->v_stride);
   p.status = status;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  int rc = cuda_status(launch_pdl(evict_select_kernel, dim3(p.hkv, a->num_seqs), dim3(kSelectThreads), 0,
-                                  stream, p));
+  p.score_vec = reinterpret_cast<uintptr_t>(a->scores) % 16 == 0 && a->scores_stride[0] % 4 == 0 &&
+                a->scores_stride[1] % 4 == 0 && a->scores_stride[2] == 1;
+  int rc = select(p, a->num_seqs, stream);
   if (rc != FD_OK) return rc;
   const int64_t most = std::min<int64_t>(
       std::min<int64_t>(p.budget, static_cast<int64_t>(p.max_new_blocks) << p.bs_log2),
       static_cast<int64_t>(p.max_blocks) << p.bs_log2);
-  const int per = kCopyThreads / 32;
+  const int per = kCopyThreads / 32 * kCopyRows;
   const int blocks = static_cast<int>(std::min<int64_t>((most + per - 1) / per, 1 << 20));
   const dim3 grid(std::max(blocks, 1), p.hkv, a->num_seqs);
   return cuda_status(a->head_dim == 128
