@@ -33,11 +33,12 @@ struct StreamParams {
   int splits;      // CTAs per (sequence, KV head, row block)
   int vec;         // rows of K and V are 16-byte aligned and contiguous
   float scale_log2;
+  int cluster;      // the splits of a unit form a cluster
+  int min_tiles;    // tiles a split holds at least
   float* part_acc;  // [row = token * hq + head][split][D]
   float* part_ml;   // [row][split][2]: max (base 2), sum
   float* raw;       // [row][raw_tokens]: scaled scores (base 2)
-  float* lse;       // [row]: max + log2(sum)
-  int64_t raw_tokens;
+  int64_t raw_tokens;  // row length of raw, or of its copy in shared memory
   int* status;
 };
 

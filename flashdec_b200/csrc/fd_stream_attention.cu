@@ -18,21 +18,27 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTok = 16;    // tokens per warp tile
 constexpr int kStages = 3;  // tiles in flight per warp
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 128;
+constexpr int kMaxCluster = 8;      // splits that merge inside a cluster
+constexpr int kRawBytes = 10 << 10; // scores a CTA may keep in shared memory
 
 template <int D>
 constexpr size_t ring_bytes() {
   return static_cast<size_t>(kWarps) * kStages * 2 * kTok * D * 2;
 }
+// ring (later the merge buffer: kWarps x rows x (D + 2) floats), q, the CTA's
+// (max, sum) and the cluster's weights per row
 template <int D, int kM>
 constexpr size_t split_smem_bytes() {
-  // ring (later the merge buffer: kWarps x rows x (D + 2) floats) and q
-  return ring_bytes<D>() + static_cast<size_t>(kM) * 16 * D * 2;
+  return ring_bytes<D>() + static_cast<size_t>(kM) * 16 * (D * 2 + 2 * sizeof(float) + (kMaxCluster + 1) * sizeof(float));
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -40,6 +46,16 @@ __device__ __forceinline__ void cp_async_commit() {
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
+  return x;
 }
 
 // Byte offset of 16-byte chunk `c` of row `r` in a [rows][D] 16-bit tile: the
@@ -54,8 +70,11 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 // One CTA: rows [16 kM rb, +16 kM) of a (sequence, KV head), split `blockIdx.x`
 // of the pages they see.  Row r is head r % group of query r / group, so K and
 // V are read once for the whole group.  Tile i of 16 tokens goes to warp i % 4;
-// each warp keeps three tiles in flight with cp.async and its own running
-// max and sum (base 2), and the four merge at the end.
+// each warp keeps three tiles in flight with cp.async and its own maximum and
+// sum (base 2, the maximum followed only when a score passes it by 2^8), and
+// the four merge at the end.  The splits merge through distributed shared
+// memory when they form a cluster (p.cluster), else through fp32 partials and
+// stream_finish_kernel.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int kM>
 __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_constant__ StreamParams p) {
@@ -64,6 +83,10 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   constexpr uint32_t kTileBytes = kTok * D * 2;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* qsm = smem + ring_bytes<D>();
+  float* cml = reinterpret_cast<float*>(qsm + kRows * D * 2);  // [row][2] this CTA's max and sum
+  float* weight = cml + kRows * 2;                             // [split][row] of the cluster
+  float* lse = weight + kMaxCluster * kRows;                   // [row]
+  float* raw = reinterpret_cast<float*>(smem + split_smem_bytes<D, kM>());  // [row][raw_tokens]
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -74,20 +97,41 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   const int split = blockIdx.x;
   const int h = blockIdx.y / p.row_blocks;
   const int b = blockIdx.z;
+  const int mask = (1 << p.bs_log2) - 1;
+  // a scale of 0 (uniform weights) stays above it: -inf * 0 is NaN; its sign goes to q
+  const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
 
   pdl_wait();
   pdl_launch_dependents();
   const StreamSeq s = sequence_of(p, b);
   const int rows_all = s.qlen * p.group;
   uint8_t* const kring = smem + warp * (kStages * 2 * kTileBytes);
+  // this lane's part of a tile copy: chunk `cc` of rows cr, cr + kStep, ...
+  constexpr int kStep = 32 / kChunks;
+  const int cr = lane / kChunks, cc = lane % kChunks;
+  const uint32_t copy_off = tile_chunk<D>(cr, cc);
+  const uint32_t k_off = tile_chunk<D>((mi >> 1) * 8 + r8, mi & 1);
+  const uint32_t v_off = tile_chunk<D>((mi & 1) * 8 + r8, mi >> 1);
 
   for (int rb = blockIdx.y - h * p.row_blocks; rb * kRows < rows_all; rb += p.row_blocks) {
     const int row0 = rb * kRows;
     const int rows = min(kRows, rows_all - row0);
     const StreamRange rg(s, row0, row0 + rows, p.group, p.window, p.sinks, p.bs_log2);
     const int tiles = ((rg.pages << p.bs_log2) + kTok - 1) / kTok;
-    const int t0 = static_cast<int>(static_cast<int64_t>(split) * tiles / p.splits);
-    const int t1 = static_cast<int>(static_cast<int64_t>(split + 1) * tiles / p.splits);
+    const int per = max((tiles + p.splits - 1) / p.splits, p.min_tiles);
+    const int t0 = min(split * per, tiles);
+    const int t1 = min(t0 + per, tiles);
+
+    if (!p.cluster && p.splits > 1 && t0 >= t1 && split > 0) {  // nothing left for this split
+      if (tid < rows) {
+        const int qt = (row0 + tid) / p.group;
+        const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + h * p.group + (row0 + tid) - qt * p.group;
+        p.part_ml[(row * p.splits + split) * 2] = -INFINITY;
+        p.part_ml[(row * p.splits + split) * 2 + 1] = 0.f;
+      }
+      continue;
+    }
 
     // lanes 0 and 1 hold the (at most two) pages of a tile: {block, position of its first token}
     auto fetch = [&](int t, int& blk, int& pos) {
@@ -96,8 +140,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       const int i = p.bs_log2 >= 4 ? (t * kTok) >> p.bs_log2 : 2 * t + lane;
       if (lane < 2 && t < t1 && i < rg.pages) {
         const int page = rg.page(i);
-        pos = p.bs_log2 >= 4 ? (page << p.bs_log2) + ((t * kTok) & ((1 << p.bs_log2) - 1))
-                             : page << p.bs_log2;
+        pos = p.bs_log2 >= 4 ? (page << p.bs_log2) + ((t * kTok) & mask) : page << p.bs_log2;
         const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + page * p.bts1);
         if (id >= 0 && id < p.num_blocks) {
           blk = static_cast<int>(id);
@@ -113,33 +156,67 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       const bool seen = pos <= rg.pos1 && (pos >= rg.lo || pos < rg.sink_end);
       return (second ? blk1 : blk0) >= 0 && seen ? pos : -1;
     };
+    // all 16 tokens seen by some row (`all`: by every row) and their pages good
+    auto whole = [&](int blk0, int blk1, int pos0, int pos1, bool all) -> bool {
+      const int hi = all ? rg.pos0 : rg.pos1;
+      const int lo = all ? max(rg.pos1 - p.window + 1, 0) : rg.lo;
+      const int se = all ? min(p.sinks, rg.pos0 + 1) : rg.sink_end;
+      auto run_ok = [&](int first, int n) { return first + n <= se || (first >= lo && first + n - 1 <= hi); };
+      if (p.bs_log2 == 3) return blk0 >= 0 && blk1 >= 0 && run_ok(pos0, 8) && run_ok(pos1, 8);
+      return blk0 >= 0 && run_ok(pos0, kTok);
+    };
     auto issue = [&](int t, int blk, int pos) {
       const int blk0 = __shfl_sync(0xffffffffu, blk, 0), blk1 = __shfl_sync(0xffffffffu, blk, 1);
       const int pp0 = __shfl_sync(0xffffffffu, pos, 0), pp1 = __shfl_sync(0xffffffffu, pos, 1);
       if (t < t1) {
         uint8_t* kt = kring + ((t / kWarps) % kStages) * (2 * kTileBytes);
-        uint8_t* vt = kt + kTileBytes;
-        const int mask = (1 << p.bs_log2) - 1;
-#pragma unroll
-        for (int i = 0; i < kTok * kChunks / 32; ++i) {
-          const int tok = (lane + 32 * i) / kChunks;
-          const int c = (lane + 32 * i) % kChunks;
-          const int tp = token_pos(tok, blk0, blk1, pp0, pp1);
-          const int64_t blkid = p.bs_log2 == 3 && tok >= 8 ? blk1 : blk0;
-          const T* ks = static_cast<const T*>(p.k);
-          const T* vs = static_cast<const T*>(p.v);
-          if (tp >= 0) {
-            ks += blkid * p.ks0 + h * p.ks1 + (tp & mask) * p.ks2 + c * 8 * p.ks3;
-            vs += blkid * p.vs0 + h * p.vs1 + (tp & mask) * p.vs2 + c * 8 * p.vs3;
+        constexpr int kN = kTok / kStep;
+        if (p.vec && whole(blk0, blk1, pp0, pp1, false)) {
+          const T* k0 = static_cast<const T*>(p.k) + blk0 * p.ks0 + h * p.ks1 + ((pp0 & mask) + cr) * p.ks2 + cc * 8;
+          const T* v0 = static_cast<const T*>(p.v) + blk0 * p.vs0 + h * p.vs1 + ((pp0 & mask) + cr) * p.vs2 + cc * 8;
+          const T* k1 = k0 + 8 * p.ks2;
+          const T* v1 = v0 + 8 * p.vs2;
+          if (p.bs_log2 == 3) {
+            k1 = static_cast<const T*>(p.k) + blk1 * p.ks0 + h * p.ks1 + cr * p.ks2 + cc * 8;
+            v1 = static_cast<const T*>(p.v) + blk1 * p.vs0 + h * p.vs1 + cr * p.vs2 + cc * 8;
           }
-          const uint32_t off = tile_chunk<D>(tok, c);
-          if (p.vec) {
-            cp_async16(smem_u32(kt) + off, ks, tp >= 0 ? 16 : 0);
-            cp_async16(smem_u32(vt) + off, vs, tp >= 0 ? 16 : 0);
-          } else {
-            const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-            *reinterpret_cast<uint4*>(kt + off) = tp >= 0 ? gather8(ks, p.ks3) : zero;
-            *reinterpret_cast<uint4*>(vt + off) = tp >= 0 ? gather8(vs, p.vs3) : zero;
+          const int64_t kstep = kStep * p.ks2, vstep = kStep * p.vs2;
+          const uint32_t dst = smem_u32(kt);
+#pragma unroll
+          for (int i = 0; i < kN; ++i) {
+            const uint32_t off = (copy_off + i * (kStep * D * 2)) ^ (((i * kStep) & 7) << 4);
+            cp_async16(dst + off, i < kN / 2 ? k0 : k1);
+            cp_async16(dst + kTileBytes + off, i < kN / 2 ? v0 : v1);
+            if (i < kN / 2) {
+              k0 += kstep;
+              v0 += vstep;
+            } else {
+              k1 += kstep;
+              v1 += vstep;
+            }
+          }
+        } else {
+          uint8_t* vt = kt + kTileBytes;
+#pragma unroll 1
+          for (int i = 0; i < kN; ++i) {
+            const int tok = cr + i * kStep;
+            const int tp = token_pos(tok, blk0, blk1, pp0, pp1);
+            const int64_t blkid = p.bs_log2 == 3 && tok >= 8 ? blk1 : blk0;
+            const T* ks = static_cast<const T*>(p.k);
+            const T* vs = static_cast<const T*>(p.v);
+            if (tp >= 0) {
+              ks += blkid * p.ks0 + h * p.ks1 + (tp & mask) * p.ks2 + cc * 8 * p.ks3;
+              vs += blkid * p.vs0 + h * p.vs1 + (tp & mask) * p.vs2 + cc * 8 * p.vs3;
+            }
+            const uint32_t off = tile_chunk<D>(tok, cc);
+            if (p.vec) {
+              cp_async16(smem_u32(kt) + off, ks, tp >= 0 ? 16 : 0);
+              cp_async16(smem_u32(vt) + off, vs, tp >= 0 ? 16 : 0);
+            } else {
+              const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(kt + off) = tp >= 0 ? gather8(ks, p.ks3) : zero;
+              *reinterpret_cast<uint4*>(vt + off) = tp >= 0 ? gather8(vs, p.vs3) : zero;
+            }
           }
         }
       }
@@ -162,14 +239,15 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
         x = p.qs2 == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0
                 ? *reinterpret_cast<const uint4*>(src)
                 : gather8(src, p.qs2);
+        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
       }
       *reinterpret_cast<uint4*>(qsm + tile_chunk<D>(r, c)) = x;
     }
     __syncthreads();
 
     float o[kM][D / 8][4];
-    float m[kM][2], l[kM][2];
-    int pos_r[kM][2];  // query position of this thread's rows
+    float m[kM][2], l[kM][2];  // m in score units: P = exp2((S - m) scale)
+    int pos_r[kM][2];          // query position of this thread's rows
 #pragma unroll
     for (int a = 0; a < kM; ++a) {
 #pragma unroll
@@ -192,10 +270,12 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) load_q(0, kk, qf[kk]);
     }
+    const float slack = 8.f / scale;
 
     for (int t = t0 + warp; t < t1; t += kWarps) {
       issue(t + (kStages - 1) * kWarps, blk[kStages - 1], pos[kStages - 1]);
-      const int cb = blk[0], cp = pos[0];  // this tile's own pages, for the masks
+      const int cb0 = __shfl_sync(0xffffffffu, blk[0], 0), cb1 = __shfl_sync(0xffffffffu, blk[0], 1);
+      const int cp0 = __shfl_sync(0xffffffffu, pos[0], 0), cp1 = __shfl_sync(0xffffffffu, pos[0], 1);
 #pragma unroll
       for (int i = 0; i < kStages - 1; ++i) {
         blk[i] = blk[i + 1];
@@ -206,8 +286,6 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       __syncwarp();
       uint8_t* kt = kring + ((t / kWarps) % kStages) * (2 * kTileBytes);
       uint8_t* vt = kt + kTileBytes;
-      const int cb0 = __shfl_sync(0xffffffffu, cb, 0), cb1 = __shfl_sync(0xffffffffu, cb, 1);
-      const int cp0 = __shfl_sync(0xffffffffu, cp, 0), cp1 = __shfl_sync(0xffffffffu, cp, 1);
 
       float sc[kM][2][4];
 #pragma unroll
@@ -219,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         uint32_t b0, b1, b2, b3;
-        ldsm_x4(smem_u32(kt) + tile_chunk<D>((mi >> 1) * 8 + r8, 2 * kk + (mi & 1)), b0, b1, b2, b3);
+        ldsm_x4(smem_u32(kt) + (k_off ^ (kk << 5)), b0, b1, b2, b3);
 #pragma unroll
         for (int a = 0; a < kM; ++a) {
           if constexpr (kM == 1) {
@@ -233,67 +311,100 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
           }
         }
       }
-      // ---- scale and masks ----
-      int kp[2][2];  // positions of this thread's four tokens, -1: seen by no row
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) kp[j][e] = token_pos(8 * j + 2 * t4 + e, cb0, cb1, cp0, cp1);
-      uint32_t vis = 0;  // bit (a, row half, j, e): the row sees the token
-#pragma unroll
-      for (int a = 0; a < kM; ++a)
+      // ---- masks, where some row misses some token ----
+      const bool edge = !whole(cb0, cb1, cp0, cp1, true);
+      uint32_t vis = 0xffffffffu;  // bit (a, j, e): the row sees the token
+      if (edge) {
+        int kp[2][2];  // positions of this thread's four tokens, -1: seen by no row
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = kp[j][e & 1];
-            const int pos = pos_r[a][e >> 1];
-            const bool on = key >= 0 && key <= pos && (key > pos - p.window || key < p.sinks);
-            sc[a][j][e] = on ? sc[a][j][e] * p.scale_log2 : -INFINITY;
-            vis |= (on ? 1u : 0u) << (a * 8 + j * 4 + e);
-          }
-      if (p.raw) {  // one query: row = head of the group, token position = key position
+          for (int e = 0; e < 2; ++e) kp[j][e] = token_pos(8 * j + 2 * t4 + e, cb0, cb1, cp0, cp1);
+        vis = 0;
 #pragma unroll
         for (int a = 0; a < kM; ++a)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int r = 16 * a + 8 * (e >> 1) + g8;
-              if (r < rows && kp[j][e & 1] >= 0)
-                p.raw[(static_cast<int64_t>(s.q0) * p.hq + h * p.group + row0 + r) * p.raw_tokens +
-                      kp[j][e & 1]] = sc[a][j][e];
+            for (int e = 0; e < 4; ++e) {
+              const int key = kp[j][e & 1];
+              const int at = pos_r[a][e >> 1];
+              const bool on = key >= 0 && key <= at && (key > at - p.window || key < p.sinks);
+              if (!on) sc[a][j][e] = -INFINITY;
+              vis |= (on ? 1u : 0u) << (a * 8 + j * 4 + e);
             }
       }
-      // ---- running max and sum, P in the type of V ----
+      if (p.scores) {  // one query: row = head of the group; list place = position
+        float* dst;
+        int64_t stride;
+        int n_tok;
+        if (p.cluster) {
+          dst = raw + (t - t0) * kTok;
+          stride = p.raw_tokens;
+          n_tok = kTok;
+        } else {
+          dst = p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens + t * kTok;
+          stride = p.raw_tokens;
+          n_tok = min(kTok, s.n - t * kTok);
+        }
+#pragma unroll
+        for (int a = 0; a < kM; ++a)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 16 * a + 8 * e + g8;
+            if (r < rows) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float* at = dst + r * stride + 8 * j + 2 * t4;
+                if (8 * j + 2 * t4 < n_tok) at[0] = sc[a][j][2 * e] * scale;
+                if (8 * j + 2 * t4 + 1 < n_tok) at[1] = sc[a][j][2 * e + 1] * scale;
+              }
+            }
+          }
+      }
+      // ---- follow the maximum when it is 2^8 behind ----
+      bool behind = false;
+#pragma unroll
+      for (int a = 0; a < kM; ++a)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          behind |= fmaxf(fmaxf(sc[a][0][2 * e], sc[a][0][2 * e + 1]),
+                          fmaxf(sc[a][1][2 * e], sc[a][1][2 * e + 1])) > m[a][e] + slack;
+      if (__any_sync(0xffffffffu, behind)) {
+#pragma unroll
+        for (int a = 0; a < kM; ++a)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(sc[a][0][2 * e], sc[a][0][2 * e + 1]),
+                             fmaxf(sc[a][1][2 * e], sc[a][1][2 * e + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m[a][e], mx);
+            const float alpha = mn == -INFINITY ? 1.f : ex2((m[a][e] - mn) * scale);
+            m[a][e] = mn;
+            l[a][e] *= alpha;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+              o[a][j][2 * e] *= alpha;
+              o[a][j][2 * e + 1] *= alpha;
+            }
+          }
+      }
+      // ---- weights, rounded to the type of V for the product ----
       uint32_t pf[kM][4];
 #pragma unroll
       for (int a = 0; a < kM; ++a) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(sc[a][0][2 * e], sc[a][0][2 * e + 1]),
-                           fmaxf(sc[a][1][2 * e], sc[a][1][2 * e + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float mn = fmaxf(m[a][e], mx);
-          const float base = mn == -INFINITY ? 0.f : mn;
-          const float alpha = exp2f(m[a][e] - base);
-          m[a][e] = mn;
-          float sum = 0.f;
+          const float base = m[a][e] == -INFINITY ? 0.f : m[a][e] * scale;
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               float& x = sc[a][j][2 * e + i];
-              x = exp2f(x - base);
-              sum += x;
+              x = ex2(fmaf(x, scale, -base));
+              l[a][e] += x;
             }
-          l[a][e] = l[a][e] * alpha + sum;
-#pragma unroll
-          for (int j = 0; j < D / 8; ++j) {
-            o[a][j][2 * e] *= alpha;
-            o[a][j][2 * e + 1] *= alpha;
-          }
         }
         pf[a][0] = pack2<T>(sc[a][0][0], sc[a][0][1]);
         pf[a][1] = pack2<T>(sc[a][0][2], sc[a][0][3]);
@@ -303,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       // A token that some rows of the block see and others do not: an
       // infinity or NaN in its V row must not reach the others (0 * inf), so
       // such elements leave the tile and are added row by row.
-      if (rg.pos0 != rg.pos1) {
+      if (edge && rg.pos0 != rg.pos1) {
         constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
         bool odd = false;
 #pragma unroll
@@ -354,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
 #pragma unroll
       for (int dp = 0; dp < D / 16; ++dp) {
         uint32_t b0, b1, b2, b3;
-        ldsm_x4_t(smem_u32(vt) + tile_chunk<D>((mi & 1) * 8 + r8, 2 * dp + (mi >> 1)), b0, b1, b2, b3);
+        ldsm_x4_t(smem_u32(vt) + (v_off ^ (dp << 5)), b0, b1, b2, b3);
 #pragma unroll
         for (int a = 0; a < kM; ++a) {
           mma_16816<T>(o[a][2 * dp], pf[a], b0, b1);
@@ -367,9 +478,9 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
     // ---- merge the warps: (max, sum, acc) per row through the ring ----
     cp_async_wait<0>();
     __syncthreads();
-    float* acc = reinterpret_cast<float*>(smem);        // [warp][row][D]
-    float* ml = acc + kWarps * kRows * D;               // [warp][row][2]
-    static_assert(sizeof(float) * kWarps * kRows * (D + 2) <= split_smem_bytes<D, kM>(), "merge buffer");
+    float* acc = reinterpret_cast<float*>(smem);  // [warp][row][D], then the CTA's in [0]
+    float* ml = acc + kWarps * kRows * D;         // [warp][row][2]
+    static_assert(sizeof(float) * kWarps * kRows * (D + 2) <= ring_bytes<D>(), "merge buffer");
 #pragma unroll
     for (int a = 0; a < kM; ++a)
 #pragma unroll
@@ -378,13 +489,14 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const int r = 16 * a + 8 * e + g8;
+        if (r >= rows) continue;
         float* dst = acc + (warp * kRows + r) * D;
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
           *reinterpret_cast<float2*>(dst + 8 * j + 2 * t4) =
               make_float2(o[a][j][2 * e], o[a][j][2 * e + 1]);
         if (t4 == 0) {
-          ml[(warp * kRows + r) * 2] = m[a][e];
+          ml[(warp * kRows + r) * 2] = m[a][e] * scale;
           ml[(warp * kRows + r) * 2 + 1] = sum;
         }
       }
@@ -398,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       float sum = 0.f, x = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(ml[(w * kRows + r) * 2] - base);
+        const float f = ex2(ml[(w * kRows + r) * 2] - base);
         sum += f * ml[(w * kRows + r) * 2 + 1];
         x += f * acc[(w * kRows + r) * D + d];
       }
@@ -406,71 +518,155 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       const int head = h * p.group + (row0 + r) - qt * p.group;
       const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
       if (p.splits == 1) {
-        const float y = sum == 0.f ? 0.f : x / sum;
-        static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] = from_f32<T>(y);
-        if (p.lse && d == 0) p.lse[row] = sum == 0.f ? INFINITY : base + log2f(sum);
+        static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] =
+            from_f32<T>(sum == 0.f ? 0.f : x / sum);
+      } else if (p.cluster) {
+        acc[e] = x;  // warp 0's place of the same element
       } else {
         p.part_acc[(row * p.splits + split) * D + d] = x;
-        if (d == 0) {
+      }
+      if (d == 0) {
+        if (p.cluster) {
+          cml[2 * r] = mx;
+          cml[2 * r + 1] = sum;
+        } else if (p.part_ml) {
           p.part_ml[(row * p.splits + split) * 2] = mx;
           p.part_ml[(row * p.splits + split) * 2 + 1] = sum;
         }
       }
     }
+    if (p.cluster) {
+      // ---- merge the cluster's splits: every CTA its share of the elements ----
+      cluster_arrive();
+      cluster_wait();
+      for (int r = tid; r < rows; r += kThreads) {
+        float pm[kMaxCluster], pl[kMaxCluster], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kMaxCluster; ++i) {
+          pm[i] = -INFINITY;
+          pl[i] = 0.f;
+          if (i < p.splits) {
+            const uint32_t at = map_to_rank(smem_u32(&cml[2 * r]), i);
+            pm[i] = ld_cluster(at);
+            pl[i] = ld_cluster(at + 4);
+          }
+          mx = fmaxf(mx, pm[i]);
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMaxCluster; ++i) sum += ex2(pm[i] - base) * pl[i];
+#pragma unroll
+        for (int i = 0; i < kMaxCluster; ++i)
+          weight[i * kRows + r] = sum == 0.f ? 0.f : ex2(pm[i] - base) / sum;
+        lse[r] = sum == 0.f ? INFINITY : base + log2f(sum);
+      }
+      __syncthreads();
+      for (int e = split * kThreads + tid; e < rows * D; e += p.splits * kThreads) {
+        const int r = e / D, d = e - r * D;
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMaxCluster; ++i)
+          if (i < p.splits) x += weight[i * kRows + r] * ld_cluster(map_to_rank(smem_u32(acc + e), i));
+        const int qt = (row0 + r) / p.group;
+        const int head = h * p.group + (row0 + r) - qt * p.group;
+        static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] = from_f32<T>(x);
+      }
+      if (p.scores) {
+        for (int i = tid; i < (t1 - t0) * kTok; i += kThreads) {
+          const int tok = t0 * kTok + i;
+          if (tok >= s.n) break;
+          const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(tok >> p.bs_log2) * p.bts1);
+          if (id < 0 || id >= p.num_blocks) continue;
+          float* dst = p.scores + id * p.scs0 + h * p.scs1 + (tok & mask) * p.scs2;
+          const float old = tok == s.n - 1 ? 0.f : *dst;
+          float w = 0.f;
+          for (int r = 0; r < rows; ++r) w += ex2(raw[r * p.raw_tokens + i] - lse[r]);
+          *dst = old + w;
+        }
+      }
+      cluster_arrive();  // the others have read this CTA's partials
+      cluster_wait();
+    }
     __syncthreads();
   }
 }
 
-// Merge of the splits' partials: one warp per row of q.
+// What remains after the split kernel: rows whose splits are partials are
+// merged (one row a CTA at a time, thread = dim), and with scores every
+// token gets the sum over the group of exp2(raw - lse).
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_constant__ StreamParams p) {
-  const int lane = threadIdx.x & 31;
-  const int b = blockIdx.y;
-  pdl_wait();
-  pdl_launch_dependents();
-  const StreamSeq s = sequence_of(p, b);
-  for (int64_t r = blockIdx.x * kWarps + (threadIdx.x >> 5); r < static_cast<int64_t>(s.qlen) * p.hq;
-       r += static_cast<int64_t>(gridDim.x) * kWarps) {
-    const int64_t row = static_cast<int64_t>(s.q0) * p.hq + r;
-    const float* ml = p.part_ml + row * p.splits * 2;
-    const float* acc = p.part_acc + row * p.splits * D;
-    float mx = -INFINITY;
-    for (int i = 0; i < p.splits; ++i) mx = fmaxf(mx, ml[2 * i]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, x[D / 32];
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) x[j] = 0.f;
-    for (int i = 0; i < p.splits; ++i) {
-      const float f = exp2f(ml[2 * i] - base);
-      sum += f * ml[2 * i + 1];
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) x[j] += f * acc[static_cast<int64_t>(i) * D + lane + 32 * j];
-    }
-    const int64_t qt = s.q0 + r / p.hq, head = r % p.hq;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j)
-      static_cast<T*>(p.out)[qt * p.os0 + head * p.os1 + (lane + 32 * j) * p.os2] =
-          from_f32<T>(sum == 0.f ? 0.f : x[j] / sum);
-    if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? INFINITY : base + log2f(sum);
-  }
-}
-
-// scores[token] += sum over the group of exp2(raw - lse): one thread per token.
-__global__ void __launch_bounds__(256) stream_scores_kernel(const __grid_constant__ StreamParams p) {
+__global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_constant__ StreamParams p) {
+  extern __shared__ float lse[];  // [group], with scores
+  __shared__ float weight[kMaxSplits];
+  __shared__ float stat[2];
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
   const int h = blockIdx.y;
   const int b = blockIdx.z;
   pdl_wait();
   pdl_launch_dependents();
   const StreamSeq s = sequence_of(p, b);
-  for (int t = blockIdx.x * 256 + threadIdx.x; t < s.n; t += gridDim.x * 256) {
+  const int rows_all = s.qlen * p.group;
+  // max and sum over the splits of a row, by one warp
+  auto row_stats = [&](const float* ml, float& base, float& sum) {
+    float mx = -INFINITY;
+    for (int i = lane; i < p.splits; i += 32) mx = fmaxf(mx, ml[2 * i]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    base = mx == -INFINITY ? 0.f : mx;
+    sum = 0.f;
+    for (int i = lane; i < p.splits; i += 32) sum += ex2(ml[2 * i] - base) * ml[2 * i + 1];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  };
+  if (p.splits > 1) {
+    for (int r = blockIdx.x; r < rows_all; r += gridDim.x) {
+      const int qt = r / p.group;
+      const int head = h * p.group + r - qt * p.group;
+      const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
+      const float* ml = p.part_ml + row * p.splits * 2;
+      if (warp == 0) {
+        float base, sum;
+        row_stats(ml, base, sum);
+        for (int i = lane; i < p.splits; i += 32)
+          weight[i] = ml[2 * i] == -INFINITY && ml[2 * i + 1] == 0.f ? 0.f : ex2(ml[2 * i] - base);
+        if (lane == 0) stat[0] = sum;
+      }
+      __syncthreads();
+      if (tid < D) {
+        const float* acc = p.part_acc + row * p.splits * D + tid;
+        float x = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < p.splits; ++i) {
+          const float w = weight[i];  // 0: the split wrote no partial
+          if (w != 0.f) x += w * acc[static_cast<int64_t>(i) * D];
+        }
+        const float sum = stat[0];
+        static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + tid * p.os2] =
+            from_f32<T>(sum == 0.f ? 0.f : x / sum);
+      }
+      __syncthreads();
+    }
+  }
+  if (!p.scores) return;
+  for (int g = warp; g < p.group; g += kWarps) {
+    float base, sum;
+    row_stats(p.part_ml + (static_cast<int64_t>(b) * p.hq + h * p.group + g) * p.splits * 2, base, sum);
+    if (lane == 0) lse[g] = sum == 0.f ? INFINITY : base + log2f(sum);
+  }
+  __syncthreads();
+  const float* raw = p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group) * p.raw_tokens;
+  for (int t = blockIdx.x * kThreads + tid; t < s.n; t += gridDim.x * kThreads) {
     const int64_t id =
         load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(t >> p.bs_log2) * p.bts1);
     if (id < 0 || id >= p.num_blocks) continue;
-    const int64_t row = static_cast<int64_t>(b) * p.hq + h * p.group;
-    float w = 0.f;
-    for (int g = 0; g < p.group; ++g) w += exp2f(p.raw[(row + g) * p.raw_tokens + t] - p.lse[row + g]);
     float* dst = p.scores + id * p.scs0 + h * p.scs1 + (t & ((1 << p.bs_log2) - 1)) * p.scs2;
-    *dst = t == s.n - 1 ? w : *dst + w;
+    const float old = t == s.n - 1 ? 0.f : *dst;
+    float w = 0.f;
+    for (int g = 0; g < p.group; ++g) w += ex2(raw[g * p.raw_tokens + t] - lse[g]);
+    *dst = old + w;
   }
 }
 
@@ -478,11 +674,14 @@ struct StreamPlan {
   int m16;         // 16-row tiles per CTA: 1 or 2
   int row_blocks;  // grid extent
   int splits;
+  int min_tiles;   // tiles a split holds at least
+  bool cluster;    // the splits are a cluster
   bool prompt;     // many rows: prompt_attention, where it takes the layout
   int64_t max_query;
   int64_t raw_tokens;
-  size_t acc_bytes, ml_bytes, raw_bytes, lse_bytes;
-  size_t bytes() const { return acc_bytes + ml_bytes + raw_bytes + lse_bytes; }
+  size_t raw_smem;
+  size_t acc_bytes, ml_bytes, raw_bytes;
+  size_t bytes() const { return acc_bytes + ml_bytes + raw_bytes; }
 };
 
 int check(const fd_stream_attention_args* a, bool scored) {
@@ -538,42 +737,73 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   }
   const int64_t tiles = (seen + kTok - 1) / kTok;
   const int64_t units = static_cast<int64_t>(a->num_seqs) * a->num_kv_heads * pl.row_blocks;
-  // two CTAs fit an SM; a split holds two tiles per warp at least
-  int64_t splits = units > 0 ? 2 * sms / units : 1;
-  splits = std::min<int64_t>(std::min<int64_t>(splits, tiles / (2 * kWarps)), kMaxSplits);
-  pl.splits = static_cast<int>(std::max<int64_t>(splits, 1));
+  // Few units: one wave of CTAs, two to an SM.  Many: splits of 1024 tokens at
+  // most, so that the long sequences of a ragged batch do not finish alone; a
+  // short one then has fewer splits (of 512 tokens), and the rest of its CTAs
+  // end at once.
+  const int64_t wave = units > 0 ? std::max<int64_t>(2 * sms / units, 1) : 1;
+  const int64_t even = (tiles + 63) / 64;
+  int64_t splits = std::min<int64_t>(std::min<int64_t>(std::max(wave, even), tiles / (2 * kWarps)), kMaxSplits);
+  splits = std::max<int64_t>(splits, 1);
+  pl.min_tiles = splits > wave ? 32 : 2 * kWarps;
   const size_t q_rows = static_cast<size_t>(tokens) * a->num_q_heads;
-  if (pl.splits > 1) {
-    pl.acc_bytes = q_rows * pl.splits * a->head_dim * sizeof(float);
-    pl.ml_bytes = q_rows * pl.splits * 2 * sizeof(float);
+  // One wave of short splits merges inside clusters: no second launch.
+  const int64_t in_cluster = std::min<int64_t>(splits, kMaxCluster);
+  pl.raw_tokens = cap;
+  if (splits > 1 && splits <= wave) {
+    const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, pl.min_tiles) * kTok;
+    const size_t raw = scored ? static_cast<size_t>(run) * std::min<int64_t>(rows, per) * sizeof(float) : 0;
+    if (run <= 512 && raw <= kRawBytes) {
+      pl.cluster = true;
+      pl.raw_smem = raw;
+      pl.raw_tokens = run;
+      splits = in_cluster;
+    }
   }
-  if (scored) {
-    pl.raw_tokens = cap;
-    pl.raw_bytes = q_rows * static_cast<size_t>(cap) * sizeof(float);
-    pl.lse_bytes = q_rows * sizeof(float);
-  }
+  pl.splits = static_cast<int>(splits);
+  if (pl.cluster) return pl;
+  if (pl.splits > 1) pl.acc_bytes = q_rows * pl.splits * a->head_dim * sizeof(float);
+  if (pl.splits > 1 || scored) pl.ml_bytes = q_rows * pl.splits * 2 * sizeof(float);
+  if (scored) pl.raw_bytes = q_rows * static_cast<size_t>(cap) * sizeof(float);
   return pl;
 }
 
 template <typename T, int D, int kM>
-int launch_split(const StreamParams& p, dim3 grid, cudaStream_t stream) {
+int launch_split(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
   auto kern = stream_split_kernel<T, D, kM>;
-  constexpr size_t smem = split_smem_bytes<D, kM>();
+  const size_t smem = split_smem_bytes<D, kM>() + pl.raw_smem;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
-  if (e == cudaSuccess) e = launch_pdl(kern, grid, dim3(kThreads), smem, stream, p);
-  return cuda_status(e);
+                                       static_cast<int>(split_smem_bytes<D, kM>() + kRawBytes));
+  if (e != cudaSuccess) return cuda_status(e);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.splits, p.hkv * pl.row_blocks, p.num_seqs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = pl.splits;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pl.cluster ? 2 : 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
 template <typename T, int D>
 int launch_typed(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
-  const dim3 grid(pl.splits, p.hkv * pl.row_blocks, p.num_seqs);
-  int rc = pl.m16 == 1 ? launch_split<T, D, 1>(p, grid, stream) : launch_split<T, D, 2>(p, grid, stream);
-  if (rc != FD_OK || pl.splits == 1) return rc;
-  const int64_t rows = static_cast<int64_t>(pl.row_blocks) * 16 * pl.m16 * p.hkv;
-  const int blocks = static_cast<int>(std::min<int64_t>((rows + kWarps - 1) / kWarps, 65535));
-  return cuda_status(launch_pdl(stream_merge_kernel<T, D>, dim3(blocks, p.num_seqs), dim3(kThreads), 0,
-                                stream, p));
+  const int rc = pl.m16 == 1 ? launch_split<T, D, 1>(p, pl, stream) : launch_split<T, D, 2>(p, pl, stream);
+  if (rc != FD_OK || pl.cluster || (pl.splits == 1 && !p.scores)) return rc;
+  // rows to merge, or four CTA widths of tokens a block
+  const int64_t rows = static_cast<int64_t>(pl.row_blocks) * 16 * pl.m16;
+  const int64_t tokens = p.scores ? (pl.raw_tokens + 4 * kThreads - 1) / (4 * kThreads) : 0;
+  const int64_t most = std::max<int64_t>(1, (1 << 20) / (static_cast<int64_t>(p.hkv) * p.num_seqs));
+  const int blocks = static_cast<int>(std::min(std::max(pl.splits > 1 ? std::min<int64_t>(rows, pl.max_query * p.group) : 1, tokens), most));
+  const size_t smem = p.scores ? static_cast<size_t>(p.group) * sizeof(float) : 0;
+  return cuda_status(launch_pdl(stream_finish_kernel<T, D>, dim3(blocks, p.hkv, p.num_seqs), dim3(kThreads),
+                                smem, stream, p));
 }
 
 int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
@@ -628,6 +858,8 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   }
   p.row_blocks = pl.row_blocks;
   p.splits = pl.splits;
+  p.min_tiles = pl.min_tiles;
+  p.cluster = pl.cluster;
   auto aligned = [](const void* base, const int64_t* st) {
     return reinterpret_cast<uintptr_t>(base) % 16 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 &&
            st[2] % 8 == 0 && st[3] == 1;
@@ -635,25 +867,17 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   p.vec = aligned(a->k_cache, a->k_stride) && aligned(a->v_cache, a->v_stride);
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   char* at = static_cast<char*>(a->scratch);
-  p.part_acc = reinterpret_cast<float*>(at);
-  p.part_ml = reinterpret_cast<float*>(at + pl.acc_bytes);
-  if (scored) {
-    p.raw = reinterpret_cast<float*>(at + pl.acc_bytes + pl.ml_bytes);
-    p.lse = reinterpret_cast<float*>(at + pl.acc_bytes + pl.ml_bytes + pl.raw_bytes);
-  }
+  if (pl.acc_bytes) p.part_acc = reinterpret_cast<float*>(at);
+  if (pl.ml_bytes) p.part_ml = reinterpret_cast<float*>(at + pl.acc_bytes);
+  if (pl.raw_bytes) p.raw = reinterpret_cast<float*>(at + pl.acc_bytes + pl.ml_bytes);
   p.raw_tokens = pl.raw_tokens;
   p.status = status;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   const bool bf16 = a->dtype == FD_DTYPE_BF16;
   if (pl.prompt && prompt_attention(p, bf16, a->head_dim, pl.max_query, stream, &rc)) return rc;
-  if (a->head_dim == 128) {
-    rc = bf16 ? launch_typed<__nv_bfloat16, 128>(p, pl, stream) : launch_typed<__half, 128>(p, pl, stream);
-  } else {
-    rc = bf16 ? launch_typed<__nv_bfloat16, 64>(p, pl, stream) : launch_typed<__half, 64>(p, pl, stream);
-  }
-  if (rc != FD_OK || !scored) return rc;
-  const int chunks = static_cast<int>(std::min<int64_t>((pl.raw_tokens + 255) / 256, 1024));
-  return cuda_status(launch_pdl(stream_scores_kernel, dim3(chunks, p.hkv, p.num_seqs), dim3(256), 0, stream, p));
+  if (a->head_dim == 128)
+    return bf16 ? launch_typed<__nv_bfloat16, 128>(p, pl, stream) : launch_typed<__half, 128>(p, pl, stream);
+  return bf16 ? launch_typed<__nv_bfloat16, 64>(p, pl, stream) : launch_typed<__half, 64>(p, pl, stream);
 }
 
 int workspace(const fd_stream_attention_args* a, bool scored, size_t* bytes) {
