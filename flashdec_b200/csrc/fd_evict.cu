@@ -59,7 +59,7 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 512;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
 constexpr int kSelectWords = 3 * kBins;  // histograms of the three digits
@@ -75,14 +75,15 @@ __device__ __forceinline__ int block_exclusive(int x, int* warp_sums, int& total
   }
   if (lane == 31) warp_sums[warp] = y;
   __syncthreads();
-  int w = warp_sums[lane];
+  constexpr int kW = kSelectThreads / 32;
+  int w = lane < kW ? warp_sums[lane] : 0;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
+  for (int d = 1; d < kW; d <<= 1) {
     const int z = __shfl_up_sync(0xffffffffu, w, d);
     if (lane >= d) w += z;
   }
-  total = __shfl_sync(0xffffffffu, w, 31);
-  const int before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+  total = __shfl_sync(0xffffffffu, w, kW - 1);
+  const int before = __shfl_sync(0xffffffffu, w, (warp + kW - 1) % kW);
   __syncthreads();  // warp_sums may be written again
   return (warp > 0 ? before : 0) + y - x;
 }
@@ -95,7 +96,7 @@ __device__ __forceinline__ int block_exclusive(int x, int* warp_sums, int& total
 // (sinks and recent), the keys above the threshold and the first of the keys
 // equal to it.  The counts are whole numbers: no order of the atomics changes
 // the result.
-__global__ void __launch_bounds__(kSelectThreads)
+__global__ void __launch_bounds__(kSelectThreads, 3)
     evict_select_kernel(const __grid_constant__ EvictParams p, int key_cap) {
   extern __shared__ __align__(16) int dyn[];
   int* hist = dyn;                                                // [3][kBins]
@@ -192,22 +193,27 @@ __global__ void __launch_bounds__(kSelectThreads)
       }
       cluster_arrive();
       cluster_wait();
-      // bins from the top: thread i has bins 2047 - 2 i and 2046 - 2 i
-      const int hi = kBins - 1 - 2 * tid;
-      int c_hi = 0, c_lo = 0;
+      // bins from the top: thread i has bins top, top - 1, top - 2 and top - 3
+      const int top = kBins - 1 - 4 * tid;
+      static_assert(4 * kSelectThreads == kBins, "four bins a thread");
+      int c[4] = {0, 0, 0, 0};
       for (int r = 0; r < ranks; ++r) {
-        uint32_t at = map_to_rank(smem_u32(mine + hi - 1), r);
-        int x, y;
-        asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(at) : "memory");
-        c_lo += x;
-        c_hi += y;
+        const uint32_t at = map_to_rank(smem_u32(mine + top - 3), r);
+        int x[4];
+        asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(x[3]), "=r"(x[2]), "=r"(x[1]), "=r"(x[0]) : "r"(at) : "memory");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] += x[i];
       }
       int total;
-      const int before = block_exclusive(c_hi + c_lo, warp_sums, total);
-      if (before < need && need <= before + c_hi + c_lo) {  // exactly one thread
-        const bool up = need <= before + c_hi;
-        pick[0] = up ? hi : hi - 1;
-        pick[1] = need - before - (up ? 0 : c_hi);
+      int before = block_exclusive(c[0] + c[1] + c[2] + c[3], warp_sums, total);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // one bin of one thread holds the key
+        if (before < need && need <= before + c[i]) {
+          pick[0] = top - i;
+          pick[1] = need - before;
+        }
+        before += c[i];
       }
       __syncthreads();
       prefix |= static_cast<uint32_t>(pick[0]) << shift;
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(kSelectThreads)
   for (int c = t0; c < t1; c += 4 * kSelectThreads) {
     uint32_t sure, tie;
     flags(c + 4 * tid, sure, tie);
-    int total;  // both counts in one sum: at most 4096 of each
+    int total;  // both counts in one sum: at most 2048 of each
     const int before = block_exclusive(__popc(sure) | (__popc(tie) << 16), warp_sums, total);
     int s = base + (before & 0xffff), w = ties + (before >> 16);
 #pragma unroll
@@ -276,33 +282,47 @@ constexpr int kCopyThreads = 256;
 constexpr int kCopyRows = 8;  // rows a warp has in flight
 
 // A warp copies K, V and score of 8 kept tokens at a time: lane i < 8 looks up
-// row i's pages, then all rows' loads go out before the first store.
+// row i's pages, all rows' loads go out before the first store, and the next
+// eight are looked up meanwhile.  A few CTAs an SM that loop: with one batch a
+// warp and a CTA for every 64 rows the SMs stood at 23 % of their warps, waiting
+// for new CTAs (131 us for 537 MB).
 template <int D>
 __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_constant__ EvictParams p) {
   const int lane = threadIdx.x & 31;
-  const int h = blockIdx.y;
+  const int h = blockIdx.x;  // the heads of a page run together
   const int b = blockIdx.z;
   const int mask = (1 << p.bs_log2) - 1;
   pdl_wait();
   pdl_launch_dependents();
   const int m = kept_of(p, length_of(p, b));
   const int* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
-  const int step = gridDim.x * (kCopyThreads / 32) * kCopyRows;
-  for (int i0 = (blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5)) * kCopyRows; i0 < m; i0 += step) {
-    int64_t src = -1, dst = -1;
-    int t = 0;
+  const int step = gridDim.y * (kCopyThreads / 32) * kCopyRows;
+  struct Rows {  // lane i < 8: row i0 + i
+    int64_t src, dst;
+    int t;
+    float score;
+  };
+  auto look = [&](int i0) -> Rows {
+    Rows r = {-1, -1, 0, 0.f};
     const int i = i0 + lane;
     if (lane < kCopyRows && i < m) {
-      t = kept[i];
-      src = page_of(p, p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(t >> p.bs_log2) * p.bts1);
-      dst = page_of(p, p.nbt, p.nbt64, b * p.nbts0 + static_cast<int64_t>(i >> p.bs_log2) * p.nbts1);
-      if (src < 0 || dst < 0) {
-        src = dst = -1;
+      r.dst = page_of(p, p.nbt, p.nbt64, b * p.nbts0 + static_cast<int64_t>(i >> p.bs_log2) * p.nbts1);
+      r.t = kept[i];
+      r.src = page_of(p, p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(r.t >> p.bs_log2) * p.bts1);
+      if (r.src < 0 || r.dst < 0) {
+        r.src = r.dst = -1;
       } else {
-        p.scores[dst * p.scs0 + h * p.scs1 + (i & mask) * p.scs2] =
-            p.scores[src * p.scs0 + h * p.scs1 + (t & mask) * p.scs2];
+        r.score = p.scores[r.src * p.scs0 + h * p.scs1 + (r.t & mask) * p.scs2];
       }
     }
+    return r;
+  };
+  int i0 = (blockIdx.y * (kCopyThreads / 32) + (threadIdx.x >> 5)) * kCopyRows;
+  Rows next = look(i0);
+  for (; i0 < m; i0 += step) {
+    const Rows cur = next;
+    const int64_t src = cur.src, dst = cur.dst;
+    const int t = cur.t;
     if (p.vec) {
       constexpr int kChunks = D / 8;      // 16-byte chunks of a row
       constexpr int kSide = 16 / kChunks; // rows a half warp moves at once: lanes 0-15 K, 16-31 V
@@ -319,6 +339,7 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_c
         const int tok = __shfl_sync(0xffffffffu, t, r);
         if (from >= 0) x[j] = __ldcs(reinterpret_cast<const uint4*>(base + from * s0 + h * s1 + (tok & mask) * s2 + c * 16));
       }
+      next = look(i0 + step);
 #pragma unroll
       for (int j = 0; j < kCopyRows / kSide; ++j) {
         const int r = j * kSide + sub;
@@ -326,6 +347,7 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_c
         if (to >= 0) *reinterpret_cast<uint4*>(base + to * s0 + h * s1 + ((i0 + r) & mask) * s2 + c * 16) = x[j];
       }
     } else {
+      next = look(i0 + step);
       for (int r = 0; r < kCopyRows; ++r) {
         const int64_t from = __shfl_sync(0xffffffffu, src, r), to = __shfl_sync(0xffffffffu, dst, r);
         const int tok = __shfl_sync(0xffffffffu, t, r);
@@ -340,6 +362,7 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_c
         }
       }
     }
+    if (dst >= 0) p.scores[dst * p.scs0 + h * p.scs1 + ((i0 + lane) & mask) * p.scs2] = cur.score;
   }
 }
 
@@ -442,8 +465,9 @@ extern "C" int fd_evict_tokens(const fd_evict_tokens_args* a, void* cuda_stream)
       std::min<int64_t>(p.budget, static_cast<int64_t>(p.max_new_blocks) << p.bs_log2),
       static_cast<int64_t>(p.max_blocks) << p.bs_log2);
   const int per = kCopyThreads / 32 * kCopyRows;
-  const int blocks = static_cast<int>(std::min<int64_t>((most + per - 1) / per, 1 << 20));
-  const dim3 grid(std::max(blocks, 1), p.hkv, a->num_seqs);
+  const int64_t fill = (4 * dev->num_sms + p.hkv * a->num_seqs - 1) / (p.hkv * a->num_seqs);  // four CTAs an SM
+  const int blocks = static_cast<int>(std::min((most + per - 1) / per, fill));
+  const dim3 grid(p.hkv, std::max(blocks, 1), a->num_seqs);
   return cuda_status(a->head_dim == 128
                          ? launch_pdl(evict_copy_kernel<128>, grid, dim3(kCopyThreads), 0, stream, p)
                          : launch_pdl(evict_copy_kernel<64>, grid, dim3(kCopyThreads), 0, stream, p));

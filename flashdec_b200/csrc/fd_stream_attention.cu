@@ -335,30 +335,18 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
             }
       }
       if (p.scores) {  // one query: row = head of the group; list place = position
-        float* dst;
-        int64_t stride;
-        int n_tok;
-        if (p.cluster) {
-          dst = raw + (t - t0) * kTok;
-          stride = p.raw_tokens;
-          n_tok = kTok;
-        } else {
-          dst = p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens + t * kTok;
-          stride = p.raw_tokens;
-          n_tok = min(kTok, s.n - t * kTok);
-        }
+        float* dst = p.cluster ? raw + (t - t0) * kTok
+                               : p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens + t * kTok;
 #pragma unroll
         for (int a = 0; a < kM; ++a)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = 16 * a + 8 * e + g8;
-            if (r < rows) {
+            if (r < rows) {  // rows are padded to whole tiles
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float* at = dst + r * stride + 8 * j + 2 * t4;
-                if (8 * j + 2 * t4 < n_tok) at[0] = sc[a][j][2 * e] * scale;
-                if (8 * j + 2 * t4 + 1 < n_tok) at[1] = sc[a][j][2 * e + 1] * scale;
-              }
+              for (int j = 0; j < 2; ++j)
+                *reinterpret_cast<float2*>(dst + r * p.raw_tokens + 8 * j + 2 * t4) =
+                    make_float2(sc[a][j][2 * e] * scale, sc[a][j][2 * e + 1] * scale);
             }
           }
       }
@@ -593,13 +581,13 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
 }
 
 // What remains after the split kernel: rows whose splits are partials are
-// merged (one row a CTA at a time, thread = dim), and with scores every
+// merged (one row a CTA at a time), and with scores every
 // token gets the sum over the group of exp2(raw - lse).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_constant__ StreamParams p) {
   extern __shared__ float lse[];  // [group], with scores
-  __shared__ float weight[kMaxSplits];
-  __shared__ float stat[2];
+  __shared__ float part[kWarps][D];
+  constexpr int kPer = D / 32;
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -627,30 +615,38 @@ __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_co
       const int head = h * p.group + r - qt * p.group;
       const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
       const float* ml = p.part_ml + row * p.splits * 2;
-      if (warp == 0) {
-        float base, sum;
-        row_stats(ml, base, sum);
-        for (int i = lane; i < p.splits; i += 32)
-          weight[i] = ml[2 * i] == -INFINITY && ml[2 * i + 1] == 0.f ? 0.f : ex2(ml[2 * i] - base);
-        if (lane == 0) stat[0] = sum;
+      float base, sum;
+      row_stats(ml, base, sum);
+      // warp w takes splits w, w + 4, ...; lane: D / 32 neighbouring dims
+      float x[kPer];
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) x[j] = 0.f;
+#pragma unroll 8
+      for (int i = warp; i < p.splits; i += kWarps) {
+        const float mx = ml[2 * i];
+        if (mx == -INFINITY && ml[2 * i + 1] == 0.f) continue;  // no partial there
+        const float w = ex2(mx - base);
+        float y[kPer];
+        if constexpr (kPer == 4) {
+          *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(p.part_acc + (row * p.splits + i) * D + lane * 4);
+        } else {
+          *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(p.part_acc + (row * p.splits + i) * D + lane * 2);
+        }
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[j] += w * y[j];
       }
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) part[warp][lane * kPer + j] = x[j];
       __syncthreads();
       if (tid < D) {
-        const float* acc = p.part_acc + row * p.splits * D + tid;
-        float x = 0.f;
-#pragma unroll 8
-        for (int i = 0; i < p.splits; ++i) {
-          const float w = weight[i];  // 0: the split wrote no partial
-          if (w != 0.f) x += w * acc[static_cast<int64_t>(i) * D];
-        }
-        const float sum = stat[0];
+        const float y = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
         static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + tid * p.os2] =
-            from_f32<T>(sum == 0.f ? 0.f : x / sum);
+            from_f32<T>(sum == 0.f ? 0.f : y / sum);
       }
       __syncthreads();
     }
   }
-  if (!p.scores) return;
+  if (!p.scores || static_cast<int>(blockIdx.x) * kThreads >= s.n) return;
   for (int g = warp; g < p.group; g += kWarps) {
     float base, sum;
     row_stats(p.part_ml + (static_cast<int64_t>(b) * p.hq + h * p.group + g) * p.splits * 2, base, sum);
@@ -745,11 +741,13 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   const int64_t even = (tiles + 63) / 64;
   int64_t splits = std::min<int64_t>(std::min<int64_t>(std::max(wave, even), tiles / (2 * kWarps)), kMaxSplits);
   splits = std::max<int64_t>(splits, 1);
+  if (splits > wave && units * splits < 16 * sms)  // a few waves: whole ones
+    splits = std::max<int64_t>(units * splits / (2 * sms) * (2 * sms) / units, 1);
   pl.min_tiles = splits > wave ? 32 : 2 * kWarps;
   const size_t q_rows = static_cast<size_t>(tokens) * a->num_q_heads;
   // One wave of short splits merges inside clusters: no second launch.
   const int64_t in_cluster = std::min<int64_t>(splits, kMaxCluster);
-  pl.raw_tokens = cap;
+  pl.raw_tokens = (cap + kTok - 1) / kTok * kTok;
   if (splits > 1 && splits <= wave) {
     const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, pl.min_tiles) * kTok;
     const size_t raw = scored ? static_cast<size_t>(run) * std::min<int64_t>(rows, per) * sizeof(float) : 0;
@@ -763,8 +761,8 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   pl.splits = static_cast<int>(splits);
   if (pl.cluster) return pl;
   if (pl.splits > 1) pl.acc_bytes = q_rows * pl.splits * a->head_dim * sizeof(float);
-  if (pl.splits > 1 || scored) pl.ml_bytes = q_rows * pl.splits * 2 * sizeof(float);
-  if (scored) pl.raw_bytes = q_rows * static_cast<size_t>(cap) * sizeof(float);
+  if (pl.splits > 1 || scored) pl.ml_bytes = (q_rows * pl.splits * 2 * sizeof(float) + 15) & ~size_t(15);
+  if (scored) pl.raw_bytes = q_rows * static_cast<size_t>(pl.raw_tokens) * sizeof(float);
   return pl;
 }
 
