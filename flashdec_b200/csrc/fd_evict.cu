@@ -60,9 +60,13 @@ __device__ __forceinline__ uint32_t score_key(float x) {
 }
 
 constexpr int kSelectThreads = 512;
-constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
-constexpr int kSelectWords = 3 * kBins;  // histograms of the three digits
+// Four digits: sign and exponent, then 8, 8 and 7 bits.  Wider ones (11, 11,
+// 10) need a pass less but cost more: every CTA reads the counts of its whole
+// cluster, and 48 clusters of 8 took 51 us on that traffic.
+constexpr int kDigits = 4;
+constexpr int kSelectWords = 512 + 256 + 256 + 128;  // their histograms
+constexpr int kShort = 2048;  // keys of the second digit's bin that are listed for the last two
 
 // Exclusive sum over the threads of a CTA (in thread order) and the total.
 __device__ __forceinline__ int block_exclusive(int x, int* warp_sums, int& total) {
@@ -90,7 +94,7 @@ __device__ __forceinline__ int block_exclusive(int x, int* warp_sums, int& total
 
 // One cluster per (KV head, sequence), each CTA a run of its tokens, whose keys
 // it keeps in shared memory when they fit (`key_cap`).  The threshold key is
-// found digit by digit (11, 11 and 10 bits): each CTA counts its keys, the
+// found digit by digit: each CTA counts its keys, the
 // cluster's counts are added through distributed shared memory, and every CTA
 // finds the same digit.  Then one pass in order keeps the protected tokens
 // (sinks and recent), the keys above the threshold and the first of the keys
@@ -99,17 +103,21 @@ __device__ __forceinline__ int block_exclusive(int x, int* warp_sums, int& total
 __global__ void __launch_bounds__(kSelectThreads, 3)
     evict_select_kernel(const __grid_constant__ EvictParams p, int key_cap) {
   extern __shared__ __align__(16) int dyn[];
-  int* hist = dyn;                                                // [3][kBins]
-  uint32_t* keys = reinterpret_cast<uint32_t*>(dyn + kSelectWords);  // [key_cap]
+  int* hist = dyn;                                                   // by digit
+  uint32_t* list = reinterpret_cast<uint32_t*>(dyn + kSelectWords);  // [kShort]
+  uint32_t* keys = list + kShort;                                    // [key_cap]
   __shared__ int warp_sums[32];
   __shared__ int pick[2];    // digit, keys still to take among that digit's
   __shared__ int counts[2];  // this CTA's sure keeps and threshold keys
+  __shared__ int listed;     // keys that matched the first two digits
   const int tid = threadIdx.x;
   const int ranks = gridDim.x;  // the cluster
   const int rank = blockIdx.x;
   const int h = blockIdx.y;
   const int b = blockIdx.z;
   for (int i = tid; i < kSelectWords; i += kSelectThreads) hist[i] = 0;
+  if (tid == 0) listed = 0;
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
   const int n = length_of(p, b);
@@ -165,61 +173,82 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
       load4(t, k);
     }
   };
-  if (cached) {
-    for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {
-      uint32_t k[4];
-      load4(t, k);
-      *reinterpret_cast<uint4*>(keys + (t - t0)) = make_uint4(k[0], k[1], k[2], k[3]);
-    }
-  }
-  __syncthreads();
   // ---- the (m - sinks - recent)-th greatest key of [mid0, mid1) ----
   int need = m - sinks - recent;
   const bool any_mid = need > 0;
   uint32_t prefix = 0;
-  if (any_mid) {
-#pragma unroll 1
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 21 : (digit == 1 ? 10 : 0);
-      const int above = digit == 0 ? 32 : (digit == 1 ? 21 : 10);  // bits found so far lie above
-      int* mine = hist + digit * kBins;
-      for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {
-        uint32_t k[4];
-        four(t, k);
+#pragma unroll 2
+  for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {  // keys, and the first digit's counts
+    uint32_t k[4];
+    load4(t, k);
+    if (cached) *reinterpret_cast<uint4*>(keys + (t - t0)) = make_uint4(k[0], k[1], k[2], k[3]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (t + i >= mid0 && t + i < mid1 && (above == 32 || (k[i] >> above) == (prefix >> above)))
-            atomicAdd(&mine[(k[i] >> shift) & (above - shift == 11 ? 2047 : 1023)], 1);
+    for (int i = 0; i < 4; ++i)
+      if (t + i >= mid0 && t + i < mid1) atomicAdd(&hist[k[i] >> 23], 1);
+  }
+  int above = 0;  // of this CTA's keys, those that a thread's bins put above the threshold
+  if (any_mid) {
+    int* mine = hist;
+#pragma unroll 1
+    for (int digit = 0; digit < kDigits; ++digit) {
+      const int shift = digit == 0 ? 23 : (digit == 1 ? 15 : (digit == 2 ? 7 : 0));
+      const int width = digit == 0 ? 9 : (digit == 3 ? 7 : 8);
+      const int bins = 1 << width;
+      const uint32_t found = prefix >> shift >> width;  // the bits above this digit
+      if (digit == 1 || (digit > 1 && listed > kShort)) {
+        for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {
+          uint32_t k[4];
+          four(t, k);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t x = k[i] >> shift;
+            if ((x >> width) == found && t + i >= mid0 && t + i < mid1) {
+              atomicAdd(&mine[x & (bins - 1)], 1);
+              if (digit == 1) {
+                const int at = atomicAdd(&listed, 1);
+                if (at < kShort) list[at] = k[i];
+              }
+            }
+          }
+        }
+      } else if (digit > 1) {
+        for (int i = tid; i < listed; i += kSelectThreads) {
+          const uint32_t x = list[i] >> shift;
+          if ((x >> width) == found) atomicAdd(&mine[x & (bins - 1)], 1);
+        }
       }
       cluster_arrive();
       cluster_wait();
-      // bins from the top: thread i has bins top, top - 1, top - 2 and top - 3
-      const int top = kBins - 1 - 4 * tid;
-      static_assert(4 * kSelectThreads == kBins, "four bins a thread");
-      int c[4] = {0, 0, 0, 0};
-      for (int r = 0; r < ranks; ++r) {
-        const uint32_t at = map_to_rank(smem_u32(mine + top - 3), r);
-        int x[4];
-        asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(x[3]), "=r"(x[2]), "=r"(x[1]), "=r"(x[0]) : "r"(at) : "memory");
+      // thread i: bin bins - 1 - i, counted over the cluster
+      int c = 0;
+      if (tid < bins) {
+        int x[kMaxCluster];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] += x[i];
-      }
-      int total;
-      int before = block_exclusive(c[0] + c[1] + c[2] + c[3], warp_sums, total);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {  // one bin of one thread holds the key
-        if (before < need && need <= before + c[i]) {
-          pick[0] = top - i;
-          pick[1] = need - before;
+        for (int r = 0; r < kMaxCluster; ++r) {
+          x[r] = 0;
+          if (r < ranks)
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x[r]) : "r"(map_to_rank(smem_u32(mine + bins - 1 - tid), r)) : "memory");
         }
-        before += c[i];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) c += x[r];
+      }
+      static_assert(kSelectThreads == 512, "a bin a thread");
+      int total;
+      const int before = block_exclusive(c, warp_sums, total);
+      if (before < need && need <= before + c) {  // one thread
+        pick[0] = bins - 1 - tid;
+        pick[1] = need - before;
       }
       __syncthreads();
+      if (tid < bins - 1 - pick[0]) above += mine[bins - 1 - tid];
       prefix |= static_cast<uint32_t>(pick[0]) << shift;
       need = pick[1];
+      if (digit == kDigits - 1 && tid == 0) counts[1] = mine[pick[0]];  // keys equal to the threshold
+      mine += bins;
       __syncthreads();
     }
+  } else if (tid == 0) {
+    counts[1] = 0;
   }
   // ---- keep `need` of the keys equal to `prefix` and all greater ones ----
   auto flags = [&](int t, uint32_t& sure, uint32_t& tie) {
@@ -234,20 +263,10 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
       tie |= (in && mid && any_mid && k[i] == prefix ? 1u : 0u) << i;
     }
   };
-  int sure_n = 0, tie_n = 0;
-  for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {
-    uint32_t sure, tie;
-    flags(t, sure, tie);
-    sure_n += __popc(sure);
-    tie_n += __popc(tie);
-  }
-  int total_sure, total_tie;
-  block_exclusive(sure_n, warp_sums, total_sure);
-  block_exclusive(tie_n, warp_sums, total_tie);
-  if (tid == 0) {
-    counts[0] = total_sure;
-    counts[1] = total_tie;
-  }
+  int total_above;
+  block_exclusive(above, warp_sums, total_above);
+  if (tid == 0)  // with the protected tokens of the run
+    counts[0] = total_above + max(min(t1, mid0) - t0, 0) + max(t1 - max(t0, mid1), 0);
   cluster_arrive();
   cluster_wait();
   int base = 0, ties = 0;  // sure keeps and threshold keys before this CTA's run
@@ -278,27 +297,40 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
   cluster_wait();
 }
 
-constexpr int kCopyThreads = 256;
-constexpr int kCopyRows = 8;  // rows a warp has in flight
+constexpr int kCopyWarps = 4;
+constexpr int kCopyThreads = kCopyWarps * 32;
+constexpr int kCopyRows = 8;    // rows of a batch
+constexpr int kCopyStages = 3;  // batches a warp has in flight
+
+template <int D>
+constexpr size_t copy_smem_bytes() {
+  return static_cast<size_t>(kCopyWarps) * kCopyStages * kCopyRows * 2 * D * 2;
+}
 
 // A warp copies K, V and score of 8 kept tokens at a time: lane i < 8 looks up
-// row i's pages, all rows' loads go out before the first store, and the next
-// eight are looked up meanwhile.  A few CTAs an SM that loop: with one batch a
-// warp and a CTA for every 64 rows the SMs stood at 23 % of their warps, waiting
-// for new CTAs (131 us for 537 MB).
+// row i's pages, cp.async brings the rows to the warp's ring in shared memory
+// and they go out from there two batches later.  Reads and writes both random
+// 256-byte rows: what bounds it is the bytes in flight.  Rows held in registers
+// instead (20 warps an SM, 4 KB each, and nothing in flight while they store)
+// took 119 us for 537 MB.
 template <int D>
 __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ __align__(16) uint8_t ring_all[];
+  constexpr int kBatch = kCopyRows * 2 * D * 2;  // bytes: per row K then V
   const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int h = blockIdx.x;  // the heads of a page run together
   const int b = blockIdx.z;
   const int mask = (1 << p.bs_log2) - 1;
+  uint8_t* ring = ring_all + warp * (kCopyStages * kBatch);
   pdl_wait();
   pdl_launch_dependents();
   const int m = kept_of(p, length_of(p, b));
   const int* kept = p.kept + (static_cast<int64_t>(b) * p.hkv + h) * p.budget;
-  const int step = gridDim.y * (kCopyThreads / 32) * kCopyRows;
-  struct Rows {  // lane i < 8: row i0 + i
-    int64_t src, dst;
+  const int step = gridDim.y * kCopyWarps * kCopyRows;
+  // lane i < 8: row i0 + i; offsets of its slot (bytes from the caches), -1: no row
+  struct Rows {
+    int64_t src, dst;  // pages
     int t;
     float score;
   };
@@ -317,40 +349,58 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_c
     }
     return r;
   };
-  int i0 = (blockIdx.y * (kCopyThreads / 32) + (threadIdx.x >> 5)) * kCopyRows;
-  Rows next = look(i0);
-  for (; i0 < m; i0 += step) {
-    const Rows cur = next;
-    const int64_t src = cur.src, dst = cur.dst;
-    const int t = cur.t;
+  constexpr int kChunks = D / 8;        // 16-byte chunks of a row
+  constexpr int kSide = 16 / kChunks;   // rows a half warp moves at once: lanes 0-15 K, 16-31 V
+  const bool is_v = lane >= 16;
+  const int c = lane & (kChunks - 1);
+  const int sub = (lane & 15) / kChunks;
+  uint8_t* const base = (is_v ? p.v + h * p.vs1 : p.k + h * p.ks1) + c * 16;
+  const int64_t s0 = is_v ? p.vs0 : p.ks0, s2 = is_v ? p.vs2 : p.ks2;
+  uint8_t* const mine = ring + (is_v ? D * 2 : 0) + sub * (4 * D) + c * 16;  // + stage, + row
+  auto load = [&](const Rows& r, int stage) {
     if (p.vec) {
-      constexpr int kChunks = D / 8;      // 16-byte chunks of a row
-      constexpr int kSide = 16 / kChunks; // rows a half warp moves at once: lanes 0-15 K, 16-31 V
-      const bool is_v = lane >= 16;
-      const int c = lane & (kChunks - 1);
-      const int sub = (lane & 15) / kChunks;
-      uint8_t* base = is_v ? p.v : p.k;
-      const int64_t s0 = is_v ? p.vs0 : p.ks0, s1 = is_v ? p.vs1 : p.ks1, s2 = is_v ? p.vs2 : p.ks2;
-      uint4 x[kCopyRows / kSide];
 #pragma unroll
       for (int j = 0; j < kCopyRows / kSide; ++j) {
-        const int r = j * kSide + sub;
-        const int64_t from = __shfl_sync(0xffffffffu, src, r);
-        const int tok = __shfl_sync(0xffffffffu, t, r);
-        if (from >= 0) x[j] = __ldcs(reinterpret_cast<const uint4*>(base + from * s0 + h * s1 + (tok & mask) * s2 + c * 16));
+        const int64_t from = __shfl_sync(0xffffffffu, r.src, j * kSide + sub);
+        const int tok = __shfl_sync(0xffffffffu, r.t, j * kSide + sub);
+        if (from >= 0)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                           smem_u32(mine + stage * kBatch + j * (kSide * 4 * D))),
+                       "l"(base + from * s0 + (tok & mask) * s2)
+                       : "memory");
       }
-      next = look(i0 + step);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const int first = (blockIdx.y * kCopyWarps + warp) * kCopyRows;
+  Rows rows[kCopyStages];  // batches in flight, and the next one's look-up
+#pragma unroll
+  for (int i = 0; i < kCopyStages; ++i) rows[i] = look(first + i * step);
+#pragma unroll
+  for (int i = 0; i < kCopyStages - 1; ++i) load(rows[i], i);
+  int stage = 0;
+  for (int i0 = first; i0 < m; i0 += step) {
+    const Rows cur = rows[0];
+    int ahead = stage + kCopyStages - 1;
+    load(rows[kCopyStages - 1], ahead >= kCopyStages ? ahead - kCopyStages : ahead);
+#pragma unroll
+    for (int i = 0; i + 1 < kCopyStages; ++i) rows[i] = rows[i + 1];
+    rows[kCopyStages - 1] = look(i0 + kCopyStages * step);
+    if (p.vec) {
+      // each lane reads back what it copied itself
+      asm volatile("cp.async.wait_group %0;" ::"n"(kCopyStages - 1) : "memory");
 #pragma unroll
       for (int j = 0; j < kCopyRows / kSide; ++j) {
         const int r = j * kSide + sub;
-        const int64_t to = __shfl_sync(0xffffffffu, dst, r);
-        if (to >= 0) *reinterpret_cast<uint4*>(base + to * s0 + h * s1 + ((i0 + r) & mask) * s2 + c * 16) = x[j];
+        const int64_t to = __shfl_sync(0xffffffffu, cur.dst, r);
+        if (to >= 0)
+          *reinterpret_cast<uint4*>(base + to * s0 + ((i0 + r) & mask) * s2) =
+              *reinterpret_cast<const uint4*>(mine + stage * kBatch + j * (kSide * 4 * D));
       }
     } else {
-      next = look(i0 + step);
       for (int r = 0; r < kCopyRows; ++r) {
-        const int64_t from = __shfl_sync(0xffffffffu, src, r), to = __shfl_sync(0xffffffffu, dst, r);
-        const int tok = __shfl_sync(0xffffffffu, t, r);
+        const int64_t from = __shfl_sync(0xffffffffu, cur.src, r), to = __shfl_sync(0xffffffffu, cur.dst, r);
+        const int tok = __shfl_sync(0xffffffffu, cur.t, r);
         if (to < 0) continue;
         const uint8_t* k0 = p.k + from * p.ks0 + h * p.ks1 + (tok & mask) * p.ks2;
         uint8_t* k1 = p.k + to * p.ks0 + h * p.ks1 + ((i0 + r) & mask) * p.ks2;
@@ -362,8 +412,27 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_c
         }
       }
     }
-    if (dst >= 0) p.scores[dst * p.scs0 + h * p.scs1 + ((i0 + lane) & mask) * p.scs2] = cur.score;
+    if (cur.dst >= 0) p.scores[cur.dst * p.scs0 + h * p.scs1 + ((i0 + lane) & mask) * p.scs2] = cur.score;
+    if (++stage == kCopyStages) stage = 0;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+template <int D>
+int copy(const EvictParams& p, int num_seqs, int sms, cudaStream_t stream) {
+  constexpr size_t smem = copy_smem_bytes<D>();
+  constexpr int kPerSm = D == 128 ? 4 : 8;  // rings that fill an SM's shared memory
+  cudaError_t e = cudaFuncSetAttribute(evict_copy_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(smem));
+  if (e != cudaSuccess) return cuda_status(e);
+  const int64_t most = std::min<int64_t>(
+      std::min<int64_t>(p.budget, static_cast<int64_t>(p.max_new_blocks) << p.bs_log2),
+      static_cast<int64_t>(p.max_blocks) << p.bs_log2);
+  const int per = kCopyWarps * kCopyRows;
+  const int64_t units = static_cast<int64_t>(p.hkv) * num_seqs;
+  const int64_t blocks = std::min((most + per - 1) / per, std::max<int64_t>(kPerSm * sms / units, 1));
+  return cuda_status(launch_pdl(evict_copy_kernel<D>, dim3(p.hkv, static_cast<unsigned>(blocks), num_seqs),
+                                dim3(kCopyThreads), smem, stream, p));
 }
 
 // Tokens a CTA of the selection holds: about 4096, and no more than a cluster
@@ -375,7 +444,7 @@ int select(const EvictParams& p, int num_seqs, cudaStream_t stream) {
   const int64_t run = ((cap + ranks - 1) / ranks + 7) & ~int64_t(7);
   // past this the keys are read again for every digit
   const int key_cap = run <= 48 * 1024 ? static_cast<int>(run) : 0;
-  const size_t smem = sizeof(int) * (kSelectWords + static_cast<size_t>(key_cap));
+  const size_t smem = sizeof(int) * (kSelectWords + kShort + static_cast<size_t>(key_cap));
   cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(smem));
   if (e != cudaSuccess) return cuda_status(e);
@@ -461,14 +530,6 @@ extern "C" int fd_evict_tokens(const fd_evict_tokens_args* a, void* cuda_stream)
                 a->scores_stride[1] % 4 == 0 && a->scores_stride[2] == 1;
   int rc = select(p, a->num_seqs, stream);
   if (rc != FD_OK) return rc;
-  const int64_t most = std::min<int64_t>(
-      std::min<int64_t>(p.budget, static_cast<int64_t>(p.max_new_blocks) << p.bs_log2),
-      static_cast<int64_t>(p.max_blocks) << p.bs_log2);
-  const int per = kCopyThreads / 32 * kCopyRows;
-  const int64_t fill = (4 * dev->num_sms + p.hkv * a->num_seqs - 1) / (p.hkv * a->num_seqs);  // four CTAs an SM
-  const int blocks = static_cast<int>(std::min((most + per - 1) / per, fill));
-  const dim3 grid(p.hkv, std::max(blocks, 1), a->num_seqs);
-  return cuda_status(a->head_dim == 128
-                         ? launch_pdl(evict_copy_kernel<128>, grid, dim3(kCopyThreads), 0, stream, p)
-                         : launch_pdl(evict_copy_kernel<64>, grid, dim3(kCopyThreads), 0, stream, p));
+  return a->head_dim == 128 ? copy<128>(p, a->num_seqs, dev->num_sms, stream)
+                            : copy<64>(p, a->num_seqs, dev->num_sms, stream);
 }
