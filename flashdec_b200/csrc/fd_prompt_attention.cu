@@ -293,6 +293,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // ======== tcgen05.mma, one thread ========
     if (lane == 0) {
       constexpr uint32_t kIdO = umma_idesc_f16(kBf16, true, 128, D);
+      // Operand descriptors by addition: one built for each product (a dozen
+      // dependent instructions) kept the tensor pipe waiting for this thread.
+      const uint64_t q_desc = umma_smem_desc(smem_u32(smem), 16, 1024, 2);
+      const uint64_t k_desc = umma_smem_desc(smem_u32(smem + SM::kRing), 16, 1024, 2);
+      const uint64_t v_desc = umma_smem_desc(smem_u32(smem + SM::kRing), SM::kHalf, 1024, 2);
       uint32_t n = 0, it = 0;  // slots taken, tiles done (per group)
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -308,13 +313,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         };
         auto issue_s = [&](int g, int t, uint32_t slot) {
           const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, 16 * keys16(t));
-          const uint32_t qa = smem_u32(smem + g * SM::kOperand);
-          const uint32_t ka = smem_u32(smem + SM::kRing + slot * SM::kOperand);
+          const uint64_t qa = q_desc + g * (SM::kOperand >> 4);
+          const uint64_t ka = k_desc + slot * (SM::kOperand >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (k >> 2) * SM::kHalf + (k & 3) * 32u;
-            umma_f16(tmem + 128 * g, umma_smem_desc(qa + off, 16, 1024, 2),
-                     umma_smem_desc(ka + off, 16, 1024, 2), idesc, k > 0);
+            umma_f16(tmem + 128 * g, qa + (off >> 4), ka + (off >> 4), idesc, k > 0);
           }
           umma_commit(smem_u32(&s_full[g]));
         };
@@ -329,14 +333,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const uint32_t vs = n % kSlots, ks = (n + 1) % kSlots;
           if (!wait(&v_ready[vs], (n / kSlots) & 1)) break;
           if (t + 1 < tiles && !wait(&full[ks], ((n + 1) / kSlots) & 1)) break;
-          const uint32_t va = smem_u32(smem + SM::kRing + vs * SM::kOperand);
+          const uint64_t va = v_desc + vs * (SM::kOperand >> 4);
           for (int g = 0; ok && g < groups; ++g) {
             if (!wait(&p_ready[g], it & 1)) break;
             tc_fence_after();
             const int steps = keys16(t);
-            for (int k = 0; k < steps; ++k)
-              umma_f16_ts(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k,
-                          umma_smem_desc(va + k * 2048, SM::kHalf, 1024, 2), kIdO, t > 0 || k > 0);
+            umma_f16_ts(tmem + 256 + 128 * g, tmem + 128 * g, va, kIdO, t > 0);
+#pragma unroll
+            for (int k = 1; k < kKeys / 16; ++k)
+              if (k < steps) umma_f16_ts(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k, va + k * 128, kIdO, 1);
             umma_commit(smem_u32(&pv_done[g]));
             // The tensor pipe takes this thread's products in order: S of the
             // next tile lands on P only after the product above has read it.
