@@ -15,12 +15,14 @@ namespace fd {
 namespace {
 
 // One CTA: 256 query rows (row = query x head of the group) of a (sequence, KV
-// head) as two groups of 128, against the list of cache pages they see in
-// tiles of 128 keys.  Per group: S = Q K^T (M 128, N 128) into TMEM, one
-// thread per row takes it from there, writes P = exp2(S - m) back over S in the
-// cache's type, and O += P V accumulates in TMEM with P as the TMEM operand.
-// The two groups alternate, so the tensor pipe works on one while the other
-// does its softmax.
+// head) as two groups of 128, against the list of cache pages they see, loaded
+// in tiles of 128 keys and worked on in steps of 64.  Per group and step:
+// S = Q K^T (M 128, N 64) into one of two TMEM buffers, one thread per row
+// takes it from there, writes P = exp2(S - m) back over it in the cache's type,
+// and O += P V accumulates in TMEM with P as the TMEM operand.  S of the next
+// step is there before the softmax of this one ends, so a group never waits
+// for its own products; with one S buffer of 128 keys (the other half of TMEM
+// holds O) it waited half of the time: 395 us on an 8k prompt.
 //
 //   warp 0      TMA producer: K and V tiles alternate through a ring of slots
 //   warp 1      issues the tcgen05.mma (one thread)
@@ -30,10 +32,14 @@ namespace {
 //   warps 4-7   softmax and epilogue of rows 0-127
 //   warps 8-11  the same of rows 128-255
 //
-// TMEM columns: S/P of group g at 128 g, O of group g at 256 + 128 g.
+// TMEM columns: S/P buffer i of group g at 128 g + 64 i, O of group g at 256 +
+// 128 g.
 constexpr int kPromptThreads = 384;
 constexpr int kRows = 256;
-constexpr int kKeys = 128;
+constexpr int kKeys = 128;  // of a tile (one load)
+constexpr int kStep = 128;  // of a softmax step
+constexpr int kBufs = 128 / kStep;
+constexpr int kPerTile = kKeys / kStep;
 
 template <int D>
 struct PromptSmem {
@@ -51,27 +57,40 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 128 consecutive fp32 columns of this thread's TMEM lane.
-__device__ __forceinline__ void tmem_ld128(uint32_t taddr, float (&v)[128]) {
+// 64 consecutive fp32 columns of this thread's TMEM lane.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
 #define R4(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3])
 #define R16(i) R4(i), R4(i + 4), R4(i + 8), R4(i + 12)
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
       "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
       "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-      "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-      "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-      "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-      "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n"
       "tcgen05.wait::ld.sync.aligned;\n"
-      : R16(0), R16(16), R16(32), R16(48), R16(64), R16(80), R16(96), R16(112)
+      : R16(0), R16(16), R16(32), R16(48)
       : "r"(taddr)
       : "memory");
 #undef R16
 #undef R4
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)),
+        "l"(reinterpret_cast<uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
 }
 
 // 32 columns of this thread's TMEM lane <- registers.
@@ -89,14 +108,38 @@ __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// D[tmem] (+)= A[tmem] x B[smem desc]; issued by one thread.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
-                                            uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0));
+// The products are issued by a whole warp of which one elected lane acts: the
+// operands stay in uniform registers (from one lane of a divergent branch
+// each product first moved its descriptors there, about 80 cycles a product).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on;
 }
+// D[tmem] (+)= A[smem desc] x B[smem desc], by the lane with `on`.
+__device__ __forceinline__ void umma_ss(uint32_t on, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], %2, %3, %4, p;\n\t}\n" ::"r"(on),
+      "r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// D[tmem] (+)= A[tmem] x B[smem desc], by the lane with `on`.
+__device__ __forceinline__ void umma_ts(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %0, 0;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], %3, %4, p;\n\t}\n" ::"r"(on),
+      "r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void umma_done(uint32_t on, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}\n" ::"r"(on),
+      "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // The first x bits, clamped to [0, 32].
 __device__ __forceinline__ uint32_t low_bits(int x) {
@@ -111,8 +154,8 @@ __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
   }
 }
 
-// What a row sees, in list coordinates (entry i of tile t is key list place
-// 128 t + i): [0, sink_end) and [w0, w1].
+// What a row sees, in list coordinates (key i of step j is list place 64 j +
+// i): [0, sink_end) and [w0, w1].
 struct RowView {
   int sink_end, w0, w1;
 };
@@ -187,10 +230,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* empty = full + kSlots;      // [slot] the products that read it are done
   uint64_t* v_ready = empty + kSlots;   // [slot] V checked
   uint64_t* q_ready = v_ready + kSlots; // [group]
-  uint64_t* s_full = q_ready + 2;       // [group] S in TMEM
-  uint64_t* p_ready = s_full + 2;       // [group] P in TMEM (and O rescaled)
-  uint64_t* pv_done = p_ready + 2;      // [group] O holds the tile
-  uint64_t* drained = pv_done + 2;
+  uint64_t* s_full = q_ready + 2;       // [group][buffer] S in TMEM
+  uint64_t* p_ready = s_full + 4;       // [group][buffer] P in TMEM (and O rescaled)
+  uint64_t* pv_done = p_ready + 4;      // [group][buffer] O holds the step
+  uint64_t* drained = pv_done + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* careful = abort_flag + 1;  // [2], by parity of the row block
@@ -208,9 +251,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&q_ready[g]), 128);
-      mbar_init(smem_u32(&s_full[g]), 1);
-      mbar_init(smem_u32(&p_ready[g]), 128);
-      mbar_init(smem_u32(&pv_done[g]), 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_u32(&s_full[2 * g + i]), 1);
+        mbar_init(smem_u32(&p_ready[2 * g + i]), 128);
+        mbar_init(smem_u32(&pv_done[2 * g + i]), 1);
+      }
     }
     mbar_init(smem_u32(drained), 1);
     fence_mbar_init();
@@ -236,11 +281,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   auto range_of = [&](int rb) {
     return StreamRange(s, rb * kRows, min(rb * kRows + kRows, rows_all), p.group, p.window, p.sinks, p.bs_log2);
   };
-  // every row of the block sees every key of tile t
-  auto interior = [&](const StreamRange& rg, int t) {
+  // every row of the block sees list places [at, at + n)
+  auto interior = [&](const StreamRange& rg, int at, int n) {
     const RowView first = view_of(p, rg, rg.pos0), last = view_of(p, rg, rg.pos1);
-    return rg.pos0 >= 0 && ((t + 1) * kKeys <= first.sink_end ||
-                            (t * kKeys >= last.w0 && (t + 1) * kKeys - 1 <= first.w1));
+    return rg.pos0 >= 0 && (at + n <= first.sink_end || (at >= last.w0 && at + n - 1 <= first.w1));
   };
 
   if (warp == 0) {
@@ -290,71 +334,86 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         drain_wait(smem_u32(&full[i % kSlots]), (i / kSlots) & 1);
     }
   } else if (warp == 1) {
-    // ======== tcgen05.mma, one thread ========
-    if (lane == 0) {
+    // ======== tcgen05.mma, issued by one elected lane ========
+    {
+      const uint32_t on = elect_one();
+      const uint32_t tm = uniform(tmem);
       constexpr uint32_t kIdO = umma_idesc_f16(kBf16, true, 128, D);
+      const uint32_t base = uniform(smem_u32(smem));
       // Operand descriptors by addition: one built for each product (a dozen
       // dependent instructions) kept the tensor pipe waiting for this thread.
-      const uint64_t q_desc = umma_smem_desc(smem_u32(smem), 16, 1024, 2);
-      const uint64_t k_desc = umma_smem_desc(smem_u32(smem + SM::kRing), 16, 1024, 2);
-      const uint64_t v_desc = umma_smem_desc(smem_u32(smem + SM::kRing), SM::kHalf, 1024, 2);
-      uint32_t n = 0, it = 0;  // slots taken, tiles done (per group)
+      const uint64_t q_desc = umma_smem_desc(base, 16, 1024, 2);
+      const uint64_t k_desc = umma_smem_desc(base + SM::kRing, 16, 1024, 2);
+      const uint64_t v_desc = umma_smem_desc(base + SM::kRing, SM::kHalf, 1024, 2);
+      uint32_t n = 0, it = 0;  // slots before this row block's, steps before it (per group)
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        ok = ok && mbar_wait(smem_u32(bar), parity, p.status, abort_flag);
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, p.status, abort_flag));
         return ok;
       };
       for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
         const StreamRange rg = range_of(rb);
-        const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
-        const int groups = rows_all - rb * kRows > 128 ? 2 : 1;
-        auto keys16 = [&](int t) {  // 16-key steps of tile t
-          return (min(kKeys, (rg.pages << p.bs_log2) - t * kKeys) + 15) >> 4;
-        };
-        auto issue_s = [&](int g, int t, uint32_t slot) {
-          const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, 16 * keys16(t));
+        const int keys = uniform(rg.pages << p.bs_log2);
+        const int steps = (keys + kStep - 1) / kStep;
+        const int groups = uniform(rows_all - rb * kRows > 128 ? 2 : 1);
+        if (steps == 0) continue;
+        auto keys16 = [&](int j) { return (min(kStep, keys - j * kStep) + 15) >> 4; };  // of step j
+        // S of step j (its K tile has landed) into its buffer
+        auto issue_s = [&](int g, int j) {
+          const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, 16 * keys16(j));
+          const uint32_t slot = (n + 2 * (j / kPerTile)) % kSlots, buf = (it + j) % kBufs;
           const uint64_t qa = q_desc + g * (SM::kOperand >> 4);
-          const uint64_t ka = k_desc + slot * (SM::kOperand >> 4);
+          const uint64_t ka = k_desc + slot * (SM::kOperand >> 4) + (j % kPerTile) * (kStep * 128 >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (k >> 2) * SM::kHalf + (k & 3) * 32u;
-            umma_f16(tmem + 128 * g, qa + (off >> 4), ka + (off >> 4), idesc, k > 0);
+            umma_ss(on, tm + 128 * g + kStep * buf, qa + (off >> 4), ka + (off >> 4), idesc, k > 0);
           }
-          umma_commit(smem_u32(&s_full[g]));
+          umma_done(on, smem_u32(&s_full[2 * g + buf]));
         };
-        if (tiles == 0) continue;
+        auto k_full = [&](int j) {  // at the first step of a tile
+          const uint32_t i = n + 2 * (j / kPerTile);
+          return j % kPerTile != 0 || wait(&full[i % kSlots], (i / kSlots) & 1);
+        };
+        // after S of step j for all groups: the K tile is free after its last step
+        auto k_done = [&](int j) {
+          if (j % kPerTile == kPerTile - 1 || j + 1 == steps) umma_done(on, smem_u32(&empty[(n + 2 * (j / kPerTile)) % kSlots]));
+        };
         for (int g = 0; ok && g < groups; ++g) wait(&q_ready[g], round & 1);
-        if (!wait(&full[n % kSlots], (n / kSlots) & 1)) break;
-        tc_fence_after();
-        for (int g = 0; g < groups; ++g) issue_s(g, 0, n % kSlots);
-        umma_commit(smem_u32(&empty[n % kSlots]));
-        ++n;
-        for (int t = 0; t < tiles; ++t, ++it) {
-          const uint32_t vs = n % kSlots, ks = (n + 1) % kSlots;
-          if (!wait(&v_ready[vs], (n / kSlots) & 1)) break;
-          if (t + 1 < tiles && !wait(&full[ks], ((n + 1) / kSlots) & 1)) break;
-          const uint64_t va = v_desc + vs * (SM::kOperand >> 4);
-          for (int g = 0; ok && g < groups; ++g) {
-            if (!wait(&p_ready[g], it & 1)) break;
+        for (int j = 0; j < kBufs && j < steps; ++j) {
+          if (!k_full(j)) break;
+          tc_fence_after();
+          for (int g = 0; g < groups; ++g) issue_s(g, j);
+          k_done(j);
+        }
+        for (int j = 0; ok && j < steps; ++j) {
+          const uint32_t vi = n + 2 * (j / kPerTile) + 1, vs = vi % kSlots, buf = (it + j) % kBufs;
+          if (j % kPerTile == 0 && !wait(&v_ready[vs], (vi / kSlots) & 1)) break;
+          if (j + kBufs < steps && !k_full(j + kBufs)) break;
+          const uint64_t va = v_desc + vs * (SM::kOperand >> 4) + (j % kPerTile) * (kStep * 128 >> 4);
+          const int k16 = keys16(j);
+          for (int g = 0; g < groups; ++g) {
+            if (!wait(&p_ready[2 * g + buf], ((it + j) / kBufs) & 1)) break;
             tc_fence_after();
-            const int steps = keys16(t);
-            umma_f16_ts(tmem + 256 + 128 * g, tmem + 128 * g, va, kIdO, t > 0);
+            const uint32_t pa = tm + 128 * g + kStep * buf, oa = tm + 256 + 128 * g;
+            umma_ts(on, oa, pa, va, kIdO, j > 0);
 #pragma unroll
-            for (int k = 1; k < kKeys / 16; ++k)
-              if (k < steps) umma_f16_ts(tmem + 256 + 128 * g, tmem + 128 * g + 8 * k, va + k * 128, kIdO, 1);
-            umma_commit(smem_u32(&pv_done[g]));
-            // The tensor pipe takes this thread's products in order: S of the
-            // next tile lands on P only after the product above has read it.
-            if (t + 1 < tiles) issue_s(g, t + 1, ks);
+            for (int k = 1; k < kStep / 16; ++k)
+              if (k < k16) umma_ts(on, oa, pa + 8 * k, va + k * 128, kIdO, 1);
+            umma_done(on, smem_u32(&pv_done[2 * g + buf]));
+            // The tensor pipe takes this thread's products in order: S of step
+            // j + 2 lands on P only after the product above has read it.
+            if (j + kBufs < steps) issue_s(g, j + kBufs);
           }
           if (!ok) break;
-          umma_commit(smem_u32(&empty[vs]));
-          if (t + 1 < tiles) umma_commit(smem_u32(&empty[ks]));
-          n += t + 1 < tiles ? 2 : 1;
+          if (j % kPerTile == kPerTile - 1 || j + 1 == steps) umma_done(on, smem_u32(&empty[vs]));
+          if (j + kBufs < steps) k_done(j + kBufs);
         }
+        n += 2 * ((steps + kPerTile - 1) / kPerTile);
+        it += steps;
       }
       if (*abort_flag) {  // products in flight still read shared memory and write TMEM
-        umma_commit(smem_u32(drained));
+        umma_done(on, smem_u32(drained));
         drain_wait(smem_u32(drained), 0);
       }
     }
@@ -373,7 +432,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int slot = n % kSlots;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), (n / kSlots) & 1, p.status, abort_flag));
         if (!ok) break;
-        if (!interior(rg, t)) {
+        if (!interior(rg, t * kKeys, kKeys)) {
           uint8_t* v = smem + SM::kRing + slot * SM::kOperand;
           const int end = min(kKeys, (((rg.pages << p.bs_log2) - t * kKeys) + 15) & ~15);
           bool odd = false;
@@ -416,7 +475,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     bool ok = true;
     for (int rb = blockIdx.x, round = 0; ok && rb * kRows + 128 * g < rows_all; rb += gridDim.x, ++round) {
       const StreamRange rg = range_of(rb);
-      const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
       const int grow0 = rb * kRows + 128 * g;
       // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane ----
       constexpr int kChunks = D / 8;
@@ -443,41 +501,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int row = grow0 + gt;
       const int qt = min(row, rows_all - 1) / p.group;
       const RowView view = view_of(p, rg, s.n - s.qlen + qt);
-      float m = -INFINITY, l = 0.f;  // m in score units: P = exp2((S - m) scale)
-      for (int t = 0; t < tiles; ++t, ++it) {
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[g]), it & 1, p.status, abort_flag));
+      const int steps = ((rg.pages << p.bs_log2) + kStep - 1) / kStep;
+      // The products of all steps before `step`.  One barrier for every other
+      // step: the last two may both be pending or both be done, and a parity
+      // tells a phase from the next one only.
+      auto pv_wait = [&](uint32_t step) {
+        const uint32_t last = step - 1;
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[2 * g + last % kBufs]), (last / kBufs) & 1, p.status,
+                                                 abort_flag)) != 0;
+      };
+      float m = -INFINITY;  // in score units: P = exp2((S - m) scale)
+      float2 l2 = make_float2(0.f, 0.f);
+      for (int j = 0; j < steps; ++j, ++it) {
+        const uint32_t buf = it % kBufs;
+        const uint32_t sb = s_addr + kStep * buf;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[2 * g + buf]), (it / kBufs) & 1, p.status, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        float v[128];
-        tmem_ld128(s_addr, v);
-        if (!interior(rg, t)) {
+        float v[kStep];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int at = t * kKeys + 32 * c;
+        for (int c = 0; c < kStep / 64; ++c) tmem_ld64(sb + 64 * c, *reinterpret_cast<float(*)[64]>(v + 64 * c));
+        if (!interior(rg, j * kStep, kStep)) {
+#pragma unroll
+          for (int c = 0; c < kStep / 32; ++c) {
+            const int at = j * kStep + 32 * c;
             const uint32_t on = low_bits(view.sink_end - at) |
                                 (low_bits(view.w1 + 1 - at) & ~low_bits(view.w0 - at));
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[32 * c + j] = (on >> j) & 1u ? v[32 * c + j] : -INFINITY;
+            for (int i = 0; i < 32; ++i) v[32 * c + i] = (on >> i) & 1u ? v[32 * c + i] : -INFINITY;
           }
         }
         float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
+        for (int i = 4; i + 8 <= kStep; i += 8)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(fmaxf(mx[c], v[i + c]), v[i + 4 + c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], v[kStep - 4 + c]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // The reference maximum follows the running one only when it is 2^8
         // behind: P stays below 2^8, and O is rescaled rarely.
         const bool first = m == -INFINITY;
         const bool behind = !first && (top - m) * scale > 8.f;
-        float alpha = 1.f;
         if (first) m = top;
-        if (behind) {
-          alpha = ex2((m - top) * scale);
-          m = top;
-          l *= alpha;
-        }
         if (__any_sync(0xffffffffu, behind)) {
-          // PV of the tile before has to be in O first
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[g]), (it - 1) & 1, p.status, abort_flag));
+          float alpha = 1.f;
+          if (behind) {
+            alpha = ex2((m - top) * scale);
+            m = top;
+          }
+          l2 = make_float2(l2.x * alpha, l2.y * alpha);
+          ok = pv_wait(it);  // the steps before have to be in O first
           if (!ok) break;
           tc_fence_after();
           for (int c = 0; c < D / 32; ++c) {
@@ -485,33 +559,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             tmem_ld32(o_addr + 32 * c, o);
             uint32_t w[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(o[j] * alpha);
+            for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(o[i] * alpha);
             tmem_st32(o_addr + 32 * c, w);
           }
           tmem_wait_st();
         }
         const float base = m == -INFINITY ? 0.f : m * scale;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kStep / 64; ++c) {
           uint32_t w[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float a = ex2(fmaf(v[64 * c + 2 * j], scale, -base));
-            const float e = ex2(fmaf(v[64 * c + 2 * j + 1], scale, -base));
-            sum[(2 * j) & 3] += a;
-            sum[(2 * j + 1) & 3] += e;
-            w[j] = pack2<T>(a, e);
+          for (int i = 0; i < 32; ++i) {
+            float2 x = fma2(make_float2(v[64 * c + 2 * i], v[64 * c + 2 * i + 1]), scale2, base2);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sum[i & 1] = add2(sum[i & 1], x);
+            w[i] = pack2<T>(x.x, x.y);
           }
-          tmem_st32(s_addr + 32 * c, w);
+          tmem_st32(sb + 32 * c, w);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l2 = add2(l2, add2(sum[0], sum[1]));
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(smem_u32(&p_ready[g]));
+        mbar_arrive(smem_u32(&p_ready[2 * g + buf]));
       }
-      if (ok && tiles > 0)
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[g]), (it - 1) & 1, p.status, abort_flag));
+      const float l = l2.x + l2.y;
+      if (ok && steps > 0) ok = pv_wait(it);
       if (!ok) break;
       tc_fence_after();
       if (careful[round & 1] == round + 1) {
@@ -525,7 +600,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const bool wide = p.os2 == 1 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0;
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
-        if (tiles > 0) {
+        if (steps > 0) {
           tmem_ld32(o_addr + 32 * c, o);
         } else {
 #pragma unroll
