@@ -26,7 +26,7 @@ namespace {
 //
 //   warp 0      TMA producer: K and V tiles alternate through a ring of slots
 //   warp 1      issues the tcgen05.mma (one thread)
-//   warp 2      V tiles with keys that some row does not see: rows that no row
+//   warps 2, 3  V tiles with keys that some row does not see: rows that no row
 //               sees are zeroed, and an infinity or NaN in another raises the
 //               CTA's `careful` flag
 //   warps 4-7   softmax and epilogue of rows 0-127
@@ -141,6 +141,19 @@ __device__ __forceinline__ void umma_done(uint32_t on, uint32_t bar) {
 }
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 
+// The greater magnitude of each 16-bit half; NaN wins.
+template <typename T>
+__device__ __forceinline__ uint32_t max_abs(uint32_t a, uint32_t b) {
+  uint32_t d;
+  b &= 0x7fff7fffu;
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  } else {
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  }
+  return d;
+}
+
 // The first x bits, clamped to [0, 32].
 __device__ __forceinline__ uint32_t low_bits(int x) {
   return x <= 0 ? 0u : (x >= 32 ? 0xffffffffu : (1u << x) - 1u);
@@ -247,7 +260,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
       mbar_init(smem_u32(&empty[i]), 1);
-      mbar_init(smem_u32(&v_ready[i]), 1);
+      mbar_init(smem_u32(&v_ready[i]), 2);
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&q_ready[g]), 128);
@@ -287,6 +300,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     return rg.pos0 >= 0 && (at + n <= first.sink_end || (at >= last.w0 && at + n - 1 <= first.w1));
   };
 
+  // 128 x 88 + 256 x 208 registers: the launch's 384 x 168
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ======== producer: lane = (page of the tile, 64-dim half) ========
     const uint64_t policy = l2_policy_evict_first();
@@ -418,8 +433,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 2) {
-    // ======== V tiles on the edge of what the rows see ========
+  } else if (warp < 4) {
+    // ======== V tiles on the edge of what the rows see, two warps ========
     constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
     uint32_t n = 0;
     bool ok = true;
@@ -427,34 +442,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const StreamRange rg = range_of(rb);
       const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
       const int shift = (rg.sink_pages - rg.win_page) << p.bs_log2;
+      const int list = rg.pages << p.bs_log2;
+      // list places that some row of the block sees: [0, s1) and [w0, w1)
+      const int s1 = min(rg.sink_end, list), w0 = rg.lo + shift, w1 = min(rg.pos1 + shift + 1, list);
       for (int t = 0; ok && t < tiles; ++t) {
         ++n;  // K
         const int slot = n % kSlots;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), (n / kSlots) & 1, p.status, abort_flag));
         if (!ok) break;
         if (!interior(rg, t * kKeys, kKeys)) {
-          uint8_t* v = smem + SM::kRing + slot * SM::kOperand;
-          const int end = min(kKeys, (((rg.pages << p.bs_log2) - t * kKeys) + 15) & ~15);
-          bool odd = false;
-          for (int k0 = 0; k0 < end; k0 += 4) {
-            const int key = k0 + (lane >> 3);  // 8 lanes per 128-byte row
-            const int place = t * kKeys + key;
-            // seen by some row of the block
-            const bool seen = place < (rg.pages << p.bs_log2) &&
-                              (place < rg.sink_end || (place >= rg.lo + shift && place <= rg.pos1 + shift));
+          uint8_t* v = smem + SM::kRing + slot * SM::kOperand + (lane >> 3) * 128 + (lane & 7) * 16;
+          const int end = min(kKeys, (list - t * kKeys + 15) & ~15);
+          uint32_t top = 0;  // the largest magnitudes so far, NaN above all
+          // 16 keys of a 64-dim half at a time: lane = (key % 4, 16-byte chunk)
+#pragma unroll 2
+          for (int u = warp - 2; u < kHalves * (end >> 4); u += 2) {
+            const int hf = kHalves == 2 ? u & 1 : 0;
+            const int k0 = (kHalves == 2 ? u >> 1 : u) * 16;
+            const int at = t * kKeys + k0;
+            uint4* x = reinterpret_cast<uint4*>(v + hf * SM::kHalf + k0 * 128);
+            if (at + 16 <= s1 || (at >= w0 && at + 16 <= w1)) {
 #pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf) {
-              uint4* x = reinterpret_cast<uint4*>(v + hf * SM::kHalf + key * 128 + (lane & 7) * 16);
-              if (!seen) {
-                *x = make_uint4(0u, 0u, 0u, 0u);
-              } else {
-                const uint4 y = *x;
-                odd |= nonfinite16(y.x, kExp) | nonfinite16(y.y, kExp) | nonfinite16(y.z, kExp) |
-                       nonfinite16(y.w, kExp);
+              for (int i = 0; i < 4; ++i) {
+                const uint4 y = x[32 * i];
+                top = max_abs<T>(max_abs<T>(max_abs<T>(max_abs<T>(top, y.x), y.y), y.z), y.w);
+              }
+            } else {
+#pragma unroll 1
+              for (int i = 0; i < 4; ++i) {
+                const int place = at + 4 * i + (lane >> 3);
+                if (place < s1 || (place >= w0 && place < w1)) {
+                  const uint4 y = x[32 * i];
+                  top = max_abs<T>(max_abs<T>(max_abs<T>(max_abs<T>(top, y.x), y.y), y.z), y.w);
+                } else {
+                  x[32 * i] = make_uint4(0u, 0u, 0u, 0u);
+                }
               }
             }
           }
-          if (__any_sync(0xffffffffu, odd) && lane == 0) careful[round & 1] = round + 1;
+          if (__any_sync(0xffffffffu, nonfinite16(top, kExp)) && lane == 0) careful[round & 1] = round + 1;
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -462,8 +488,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ++n;  // V
       }
     }
-  } else if (warp >= 4) {
+  } else {
     // ======== softmax: thread = row = TMEM lane ========
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int g = (warp - 4) >> 2;
     const int gt = tid - 128 - 128 * g;  // row of the group
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -476,24 +503,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int rb = blockIdx.x, round = 0; ok && rb * kRows + 128 * g < rows_all; rb += gridDim.x, ++round) {
       const StreamRange rg = range_of(rb);
       const int grow0 = rb * kRows + 128 * g;
-      // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane ----
-      constexpr int kChunks = D / 8;
+      // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane;
+      // the loads of eight rows go out before the first store ----
+      constexpr int kChunks = D / 8, kRowStep = 128 / kChunks;
+      const int c = gt % kChunks, r0 = gt / kChunks;
+      const int qt0 = grow0 / p.group, rem0 = grow0 - qt0 * p.group;
+      // element offset of row r of the group (a small dividend: one multiplication)
+      auto row_at = [&](int r, int64_t s0, int64_t s1) -> int64_t {
+        const int add = p.group == 1 ? r : __umulhi(static_cast<uint32_t>(rem0 + r), p.group_magic);
+        return (s.q0 + qt0 + add) * s0 + (h * p.group + rem0 + r - add * p.group) * s1;
+      };
+      uint8_t* const area = smem + g * SM::kOperand + (c >> 3) * SM::kHalf;
+      if (p.q_vec) {
+        const T* const src = static_cast<const T*>(p.q) + c * 8;
+#pragma unroll 1
+        for (int i0 = 0; i0 < kChunks; i0 += 8) {
+          uint4 x[8];
 #pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const int e = gt + 128 * i;
-        const int r = e / kChunks, c = e % kChunks;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (grow0 + r < rows_all) {
-          const int qt = (grow0 + r) / p.group;
-          const int head = h * p.group + (grow0 + r) - qt * p.group;
-          const T* src = static_cast<const T*>(p.q) + (s.q0 + qt) * p.qs0 + head * p.qs1 + c * 8 * p.qs2;
-          x = p.qs2 == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0
-                  ? *reinterpret_cast<const uint4*>(src)
-                  : gather8(src, p.qs2);
-          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+          for (int i = 0; i < 8; ++i) {
+            const int r = r0 + (i0 + i) * kRowStep;
+            x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (grow0 + r < rows_all) x[i] = *reinterpret_cast<const uint4*>(src + row_at(r, p.qs0, p.qs1));
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = r0 + (i0 + i) * kRowStep;
+            x[i].x ^= flip; x[i].y ^= flip; x[i].z ^= flip; x[i].w ^= flip;
+            *reinterpret_cast<uint4*>(area + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
+          }
         }
-        *reinterpret_cast<uint4*>(smem + g * SM::kOperand + (c >> 3) * SM::kHalf + r * 128 +
-                                  (((c & 7) ^ (r & 7)) << 4)) = x;
+      } else {
+#pragma unroll 1
+        for (int r = r0; r < 128; r += kRowStep) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (grow0 + r < rows_all)
+            x = gather8(static_cast<const T*>(p.q) + row_at(r, p.qs0, p.qs1) + c * 8 * p.qs2, p.qs2);
+          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+          *reinterpret_cast<uint4*>(area + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&q_ready[g]));
@@ -594,33 +641,43 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         careful_rows<T, D>(p, s, b, h, w0, max(0, min(32, rows_all - w0)), lane);
         continue;
       }
+      // ---- O / l through the group's q area (its products are done), so that
+      // 16 (or 8) lanes write a row: stored from TMEM rows directly, a lane
+      // each, the epilogue took 11k cycles of a 100k-cycle row block ----
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int head = h * p.group + row - qt * p.group;
-      T* dst = static_cast<T*>(p.out) + (s.q0 + qt) * p.os0 + head * p.os1;
-      const bool wide = p.os2 == 1 && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0;
-      for (int c = 0; c < D / 32; ++c) {
+      uint8_t* const rows_out = smem + g * SM::kOperand;
+#pragma unroll 1
+      for (int q4 = 0; q4 < D / 32; ++q4) {
         float o[32];
         if (steps > 0) {
-          tmem_ld32(o_addr + 32 * c, o);
+          tmem_ld32(o_addr + 32 * q4, o);
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = 0.f;
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = l == 0.f ? 0.f : o[j] * inv;
-        if (row < rows_all) {
-          if (wide) {
+        for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<uint4*>(dst + 32 * c + 8 * j) =
-                  make_uint4(pack2<T>(o[8 * j], o[8 * j + 1]), pack2<T>(o[8 * j + 2], o[8 * j + 3]),
-                             pack2<T>(o[8 * j + 4], o[8 * j + 5]), pack2<T>(o[8 * j + 6], o[8 * j + 7]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) dst[(32 * c + j) * p.os2] = from_f32<T>(o[j]);
-          }
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(rows_out + gt * (D * 2) + (((4 * q4 + i) ^ (gt & 7)) << 4)) =
+              make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
+                         pack2<T>(o[8 * i + 4], o[8 * i + 5]), pack2<T>(o[8 * i + 6], o[8 * i + 7]));
+      }
+      named_barrier(1 + g, 128);
+      T* const out = static_cast<T*>(p.out);
+#pragma unroll 4
+      for (int r = r0; r < min(128, rows_all - grow0); r += kRowStep) {
+        const uint4 x = *reinterpret_cast<const uint4*>(rows_out + r * (D * 2) + ((c ^ (r & 7)) << 4));
+        if (p.out_vec) {
+          *reinterpret_cast<uint4*>(out + row_at(r, p.os0, p.os1) + c * 8) = x;
+        } else {
+          T* dst = out + row_at(r, p.os0, p.os1);
+          const T* y = reinterpret_cast<const T*>(rows_out + r * (D * 2) + ((c ^ (r & 7)) << 4));
+#pragma unroll 1
+          for (int k = 0; k < 8; ++k) dst[(c * 8 + k) * p.os2] = y[k];
         }
       }
+      named_barrier(1 + g, 128);  // the q area is free
       tc_fence_before();
     }
   }

@@ -27,11 +27,13 @@ struct StreamParams {
   int64_t scs0, scs1, scs2;
   int bt64, sl64, qs64;
   int num_seqs, num_tokens, hq, hkv, group;
+  uint32_t group_magic;  // ceil(2^32 / group): x / group = mulhi(x, magic) while x * group < 2^32 (not for group 1)
   int bs_log2, num_blocks, max_blocks;
   int window, sinks;
   int row_blocks;  // grid extent of the row-block axis
   int splits;      // CTAs per (sequence, KV head, row block)
   int vec;         // rows of K and V are 16-byte aligned and contiguous
+  int q_vec, out_vec;  // the same of q and of out
   float scale_log2;
   int cluster;      // the splits of a unit form a cluster
   int min_tiles;    // tiles a split holds at least

@@ -689,7 +689,7 @@ int check(const fd_stream_attention_args* a, bool scored) {
   if (a->num_seqs < 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->num_blocks <= 0 ||
       a->max_blocks_per_seq <= 0 || a->num_q_heads % a->num_kv_heads != 0)
     return FD_ERR_INVALID_ARGUMENT;
-  if (a->num_seqs > 65535 || a->num_kv_heads > 65535 ||
+  if (a->num_seqs > 65535 || a->num_kv_heads > 65535 || a->num_q_heads / a->num_kv_heads > 16384 ||
       static_cast<int64_t>(a->max_blocks_per_seq) * a->block_size > 0x3fffffff)
     return FD_ERR_UNSUPPORTED;
   if (!scored) {
@@ -839,6 +839,7 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   p.hq = a->num_q_heads;
   p.hkv = a->num_kv_heads;
   p.group = a->num_q_heads / a->num_kv_heads;
+  p.group_magic = static_cast<uint32_t>(((uint64_t(1) << 32) + p.group - 1) / p.group);
   p.bs_log2 = a->block_size == 8 ? 3 : (a->block_size == 16 ? 4 : 5);
   p.num_blocks = a->num_blocks;
   p.max_blocks = a->max_blocks_per_seq;
@@ -863,6 +864,11 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
            st[2] % 8 == 0 && st[3] == 1;
   };
   p.vec = aligned(a->k_cache, a->k_stride) && aligned(a->v_cache, a->v_stride);
+  auto aligned3 = [](const void* base, const int64_t* st) {
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] == 1;
+  };
+  p.q_vec = aligned3(a->q, a->q_stride);
+  p.out_vec = aligned3(a->out, a->out_stride);
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   char* at = static_cast<char*>(a->scratch);
   if (pl.acc_bytes) p.part_acc = reinterpret_cast<float*>(at);
