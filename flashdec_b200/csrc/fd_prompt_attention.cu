@@ -15,14 +15,15 @@ namespace fd {
 namespace {
 
 // One CTA: 256 query rows (row = query x head of the group) of a (sequence, KV
-// head) as two groups of 128, against the list of cache pages they see, loaded
-// in tiles of 128 keys and worked on in steps of 64.  Per group and step:
-// S = Q K^T (M 128, N 64) into one of two TMEM buffers, one thread per row
-// takes it from there, writes P = exp2(S - m) back over it in the cache's type,
-// and O += P V accumulates in TMEM with P as the TMEM operand.  S of the next
-// step is there before the softmax of this one ends, so a group never waits
-// for its own products; with one S buffer of 128 keys (the other half of TMEM
-// holds O) it waited half of the time: 395 us on an 8k prompt.
+// head) as two groups of 128, against the list of cache pages they see in
+// tiles of 128 keys.  Per group: S = Q K^T (M 128, N 128) into TMEM, one thread
+// per row takes it from there and writes P = exp2(S - m) back over it in the
+// cache's type, in two halves, and O += P V accumulates in TMEM with P as the
+// TMEM operand, the first half while the second is being computed.  The two
+// groups alternate, so the tensor pipe works on one while the other does its
+// softmax.  With two S buffers of 64 keys a group never waits for its own
+// products, but a product of N 64 takes nearly as long as one of N 128 (it
+// reads the same Q operand): 428 us on an 8k prompt against 378 at that point.
 //
 //   warp 0      TMA producer: K and V tiles alternate through a ring of slots
 //   warp 1      issues the tcgen05.mma (one thread)
@@ -32,14 +33,10 @@ namespace {
 //   warps 4-7   softmax and epilogue of rows 0-127
 //   warps 8-11  the same of rows 128-255
 //
-// TMEM columns: S/P buffer i of group g at 128 g + 64 i, O of group g at 256 +
-// 128 g.
+// TMEM columns: S/P of group g at 128 g, O of group g at 256 + 128 g.
 constexpr int kPromptThreads = 384;
 constexpr int kRows = 256;
-constexpr int kKeys = 128;  // of a tile (one load)
-constexpr int kStep = 128;  // of a softmax step
-constexpr int kBufs = 128 / kStep;
-constexpr int kPerTile = kKeys / kStep;
+constexpr int kKeys = 128;  // of a tile
 
 template <int D>
 struct PromptSmem {
@@ -50,12 +47,6 @@ struct PromptSmem {
   static constexpr uint32_t kBars = kRing + kSlots * kOperand;
   static constexpr size_t kBytes = kBars + 512 + 1024;     // barriers; alignment
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // 64 consecutive fp32 columns of this thread's TMEM lane.
 __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
@@ -243,10 +234,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* empty = full + kSlots;      // [slot] the products that read it are done
   uint64_t* v_ready = empty + kSlots;   // [slot] V checked
   uint64_t* q_ready = v_ready + kSlots; // [group]
-  uint64_t* s_full = q_ready + 2;       // [group][buffer] S in TMEM
-  uint64_t* p_ready = s_full + 4;       // [group][buffer] P in TMEM (and O rescaled)
-  uint64_t* pv_done = p_ready + 4;      // [group][buffer] O holds the step
-  uint64_t* drained = pv_done + 4;
+  uint64_t* s_full = q_ready + 2;       // [group] S in TMEM
+  uint64_t* p_ready = s_full + 2;       // [group] P in TMEM (and O rescaled)
+  uint64_t* pv_done = p_ready + 2;      // [group] O holds the tile
+  uint64_t* drained = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   volatile int* careful = abort_flag + 1;  // [2], by parity of the row block
@@ -264,11 +255,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&q_ready[g]), 128);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(smem_u32(&s_full[2 * g + i]), 1);
-        mbar_init(smem_u32(&p_ready[2 * g + i]), 128);
-        mbar_init(smem_u32(&pv_done[2 * g + i]), 1);
-      }
+      mbar_init(smem_u32(&s_full[g]), 1);
+      mbar_init(smem_u32(&p_ready[g]), 128);
+      mbar_init(smem_u32(&pv_done[g]), 1);
     }
     mbar_init(smem_u32(drained), 1);
     fence_mbar_init();
@@ -360,7 +349,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const uint64_t q_desc = umma_smem_desc(base, 16, 1024, 2);
       const uint64_t k_desc = umma_smem_desc(base + SM::kRing, 16, 1024, 2);
       const uint64_t v_desc = umma_smem_desc(base + SM::kRing, SM::kHalf, 1024, 2);
-      uint32_t n = 0, it = 0;  // slots before this row block's, steps before it (per group)
+      uint32_t n = 0, it = 0;  // next slot, tiles done (per group)
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, p.status, abort_flag));
@@ -369,63 +358,52 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
         const StreamRange rg = range_of(rb);
         const int keys = uniform(rg.pages << p.bs_log2);
-        const int steps = (keys + kStep - 1) / kStep;
+        const int tiles = (keys + kKeys - 1) / kKeys;
         const int groups = uniform(rows_all - rb * kRows > 128 ? 2 : 1);
-        if (steps == 0) continue;
-        auto keys16 = [&](int j) { return (min(kStep, keys - j * kStep) + 15) >> 4; };  // of step j
-        // S of step j (its K tile has landed) into its buffer
-        auto issue_s = [&](int g, int j) {
-          const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, 16 * keys16(j));
-          const uint32_t slot = (n + 2 * (j / kPerTile)) % kSlots, buf = (it + j) % kBufs;
+        if (tiles == 0) continue;
+        auto keys16 = [&](int t) { return (min(kKeys, keys - t * kKeys) + 15) >> 4; };  // of tile t
+        auto issue_s = [&](int g, int t, uint32_t slot) {
+          const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, 16 * keys16(t));
           const uint64_t qa = q_desc + g * (SM::kOperand >> 4);
-          const uint64_t ka = k_desc + slot * (SM::kOperand >> 4) + (j % kPerTile) * (kStep * 128 >> 4);
+          const uint64_t ka = k_desc + slot * (SM::kOperand >> 4);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (k >> 2) * SM::kHalf + (k & 3) * 32u;
-            umma_ss(on, tm + 128 * g + kStep * buf, qa + (off >> 4), ka + (off >> 4), idesc, k > 0);
+            umma_ss(on, tm + 128 * g, qa + (off >> 4), ka + (off >> 4), idesc, k > 0);
           }
-          umma_done(on, smem_u32(&s_full[2 * g + buf]));
-        };
-        auto k_full = [&](int j) {  // at the first step of a tile
-          const uint32_t i = n + 2 * (j / kPerTile);
-          return j % kPerTile != 0 || wait(&full[i % kSlots], (i / kSlots) & 1);
-        };
-        // after S of step j for all groups: the K tile is free after its last step
-        auto k_done = [&](int j) {
-          if (j % kPerTile == kPerTile - 1 || j + 1 == steps) umma_done(on, smem_u32(&empty[(n + 2 * (j / kPerTile)) % kSlots]));
+          umma_done(on, smem_u32(&s_full[g]));
         };
         for (int g = 0; ok && g < groups; ++g) wait(&q_ready[g], round & 1);
-        for (int j = 0; j < kBufs && j < steps; ++j) {
-          if (!k_full(j)) break;
-          tc_fence_after();
-          for (int g = 0; g < groups; ++g) issue_s(g, j);
-          k_done(j);
-        }
-        for (int j = 0; ok && j < steps; ++j) {
-          const uint32_t vi = n + 2 * (j / kPerTile) + 1, vs = vi % kSlots, buf = (it + j) % kBufs;
-          if (j % kPerTile == 0 && !wait(&v_ready[vs], (vi / kSlots) & 1)) break;
-          if (j + kBufs < steps && !k_full(j + kBufs)) break;
-          const uint64_t va = v_desc + vs * (SM::kOperand >> 4) + (j % kPerTile) * (kStep * 128 >> 4);
-          const int k16 = keys16(j);
+        if (!wait(&full[n % kSlots], (n / kSlots) & 1)) break;
+        tc_fence_after();
+        for (int g = 0; g < groups; ++g) issue_s(g, 0, n % kSlots);
+        umma_done(on, smem_u32(&empty[n % kSlots]));
+        ++n;
+        for (int t = 0; t < tiles; ++t, ++it, n += 2) {  // n: V of tile t
+          const uint32_t vs = n % kSlots, ks = (n + 1) % kSlots;
+          const bool more = t + 1 < tiles;
+          if (!wait(&v_ready[vs], (n / kSlots) & 1)) break;
+          if (more && !wait(&full[ks], ((n + 1) / kSlots) & 1)) break;
+          const uint64_t va = v_desc + vs * (SM::kOperand >> 4);
+          const int k16 = keys16(t);
           for (int g = 0; g < groups; ++g) {
-            if (!wait(&p_ready[2 * g + buf], ((it + j) / kBufs) & 1)) break;
+            const uint32_t pa = tm + 128 * g, oa = tm + 256 + 128 * g;
+            if (!wait(&p_ready[g], it & 1)) break;
             tc_fence_after();
-            const uint32_t pa = tm + 128 * g + kStep * buf, oa = tm + 256 + 128 * g;
-            umma_ts(on, oa, pa, va, kIdO, j > 0);
+            umma_ts(on, oa, pa, va, kIdO, t > 0);
 #pragma unroll
-            for (int k = 1; k < kStep / 16; ++k)
+            for (int k = 1; k < 8; ++k)
               if (k < k16) umma_ts(on, oa, pa + 8 * k, va + k * 128, kIdO, 1);
-            umma_done(on, smem_u32(&pv_done[2 * g + buf]));
-            // The tensor pipe takes this thread's products in order: S of step
-            // j + 2 lands on P only after the product above has read it.
-            if (j + kBufs < steps) issue_s(g, j + kBufs);
+            umma_done(on, smem_u32(&pv_done[g]));
+            // The tensor pipe takes this warp's products in order: S of the
+            // next tile lands on P only after the product above has read it.
+            if (more) issue_s(g, t + 1, ks);
           }
           if (!ok) break;
-          if (j % kPerTile == kPerTile - 1 || j + 1 == steps) umma_done(on, smem_u32(&empty[vs]));
-          if (j + kBufs < steps) k_done(j + kBufs);
+          umma_done(on, smem_u32(&empty[vs]));
+          if (more) umma_done(on, smem_u32(&empty[ks]));
         }
-        n += 2 * ((steps + kPerTile - 1) / kPerTile);
-        it += steps;
+        --n;  // no K after the last V
       }
       if (*abort_flag) {  // products in flight still read shared memory and write TMEM
         umma_done(on, smem_u32(drained));
@@ -503,8 +481,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int rb = blockIdx.x, round = 0; ok && rb * kRows + 128 * g < rows_all; rb += gridDim.x, ++round) {
       const StreamRange rg = range_of(rb);
       const int grow0 = rb * kRows + 128 * g;
-      // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane;
-      // the loads of eight rows go out before the first store ----
+      // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane.
+      // A rolled loop: this code runs once per row block, and unrolled sixteen
+      // times its instruction fetches took 14k cycles of a 90k-cycle block ----
       constexpr int kChunks = D / 8, kRowStep = 128 / kChunks;
       const int c = gt % kChunks, r0 = gt / kChunks;
       const int qt0 = grow0 / p.group, rem0 = grow0 - qt0 * p.group;
@@ -517,29 +496,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (p.q_vec) {
         const T* const src = static_cast<const T*>(p.q) + c * 8;
 #pragma unroll 1
-        for (int i0 = 0; i0 < kChunks; i0 += 8) {
-          uint4 x[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = r0 + (i0 + i) * kRowStep;
-            x[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (grow0 + r < rows_all) x[i] = *reinterpret_cast<const uint4*>(src + row_at(r, p.qs0, p.qs1));
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = r0 + (i0 + i) * kRowStep;
-            x[i].x ^= flip; x[i].y ^= flip; x[i].z ^= flip; x[i].w ^= flip;
-            *reinterpret_cast<uint4*>(area + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[i];
-          }
+        for (int r = r0; r < 128; r += kRowStep) {
+          const bool in = grow0 + r < rows_all;
+          cp_async16(smem_u32(area) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (in ? row_at(r, p.qs0, p.qs1) : 0),
+                     in ? 16 : 0);
         }
+        cp_async_commit();
+        cp_async_wait<0>();
       } else {
 #pragma unroll 1
         for (int r = r0; r < 128; r += kRowStep) {
           uint4 x = make_uint4(0u, 0u, 0u, 0u);
           if (grow0 + r < rows_all)
             x = gather8(static_cast<const T*>(p.q) + row_at(r, p.qs0, p.qs1) + c * 8 * p.qs2, p.qs2);
-          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
           *reinterpret_cast<uint4*>(area + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+        }
+      }
+      if (flip) {  // the chunks this thread brought itself
+#pragma unroll 1
+        for (int r = r0; r < 128; r += kRowStep) {
+          uint4* x = reinterpret_cast<uint4*>(area + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+          *x = make_uint4(x->x ^ flip, x->y ^ flip, x->z ^ flip, x->w ^ flip);
         }
       }
       fence_proxy_async_smem();
@@ -548,44 +525,44 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int row = grow0 + gt;
       const int qt = min(row, rows_all - 1) / p.group;
       const RowView view = view_of(p, rg, s.n - s.qlen + qt);
-      const int steps = ((rg.pages << p.bs_log2) + kStep - 1) / kStep;
-      // The products of all steps before `step`.  One barrier for every other
-      // step: the last two may both be pending or both be done, and a parity
-      // tells a phase from the next one only.
-      auto pv_wait = [&](uint32_t step) {
-        const uint32_t last = step - 1;
-        return __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[2 * g + last % kBufs]), (last / kBufs) & 1, p.status,
-                                                 abort_flag)) != 0;
+      const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      // list places that every row sees: [0, all_s) and [all_0, all_1)
+      const RowView row_0 = view_of(p, rg, rg.pos0), row_n = view_of(p, rg, rg.pos1);
+      const int all_s = rg.pos0 < 0 ? 0 : row_0.sink_end, all_0 = row_n.w0, all_1 = rg.pos0 < 0 ? 0 : row_0.w1 + 1;
+      // the products of all tiles before `it` (S of tile `it` was issued after
+      // that of tile it - 2, so the phase is the next one or the one before)
+      auto pv_wait = [&] {
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[g]), (it - 1) & 1, p.status, abort_flag)) != 0;
       };
       float m = -INFINITY;  // in score units: P = exp2((S - m) scale)
       float2 l2 = make_float2(0.f, 0.f);
-      for (int j = 0; j < steps; ++j, ++it) {
-        const uint32_t buf = it % kBufs;
-        const uint32_t sb = s_addr + kStep * buf;
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[2 * g + buf]), (it / kBufs) & 1, p.status, abort_flag));
+      for (int t = 0; t < tiles; ++t, ++it) {
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[g]), it & 1, p.status, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        float v[kStep];
+        float v[kKeys];
+        tmem_ld64(s_addr, *reinterpret_cast<float(*)[64]>(v));
+        tmem_ld64(s_addr + 64, *reinterpret_cast<float(*)[64]>(v + 64));
+        const int at = t * kKeys;
+        if (!(at + kKeys <= all_s || (at >= all_0 && at + kKeys <= all_1))) {
 #pragma unroll
-        for (int c = 0; c < kStep / 64; ++c) tmem_ld64(sb + 64 * c, *reinterpret_cast<float(*)[64]>(v + 64 * c));
-        if (!interior(rg, j * kStep, kStep)) {
-#pragma unroll
-          for (int c = 0; c < kStep / 32; ++c) {
-            const int at = j * kStep + 32 * c;
-            const uint32_t on = low_bits(view.sink_end - at) |
-                                (low_bits(view.w1 + 1 - at) & ~low_bits(view.w0 - at));
+          for (int c = 0; c < kKeys / 32; ++c) {
+            const int place = at + 32 * c;
+            const uint32_t on = low_bits(view.sink_end - place) |
+                                (low_bits(view.w1 + 1 - place) & ~low_bits(view.w0 - place));
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[32 * c + i] = (on >> i) & 1u ? v[32 * c + i] : -INFINITY;
           }
         }
-        float mx[4] = {v[0], v[1], v[2], v[3]};
+        float mx[8];
 #pragma unroll
-        for (int i = 4; i + 8 <= kStep; i += 8)
+        for (int c = 0; c < 8; ++c) mx[c] = fmaxf(v[c], v[c + 8]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(fmaxf(mx[c], v[i + c]), v[i + 4 + c]);
+        for (int i = 16; i < kKeys; i += 16)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], v[kStep - 4 + c]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          for (int c = 0; c < 8; ++c) mx[c] = fmaxf(fmaxf(mx[c], v[i + c]), v[i + 8 + c]);
+        const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
         // The reference maximum follows the running one only when it is 2^8
         // behind: P stays below 2^8, and O is rescaled rarely.
         const bool first = m == -INFINITY;
@@ -598,7 +575,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             m = top;
           }
           l2 = make_float2(l2.x * alpha, l2.y * alpha);
-          ok = pv_wait(it);  // the steps before have to be in O first
+          ok = pv_wait();  // the tiles before have to be in O first
           if (!ok) break;
           tc_fence_after();
           for (int c = 0; c < D / 32; ++c) {
@@ -615,7 +592,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const float2 scale2 = make_float2(scale, scale), base2 = make_float2(-base, -base);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int c = 0; c < kStep / 64; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t w[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -625,16 +602,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             sum[i & 1] = add2(sum[i & 1], x);
             w[i] = pack2<T>(x.x, x.y);
           }
-          tmem_st32(sb + 32 * c, w);
+          tmem_st32(s_addr + 32 * c, w);
         }
         l2 = add2(l2, add2(sum[0], sum[1]));
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(smem_u32(&p_ready[2 * g + buf]));
+        mbar_arrive(smem_u32(&p_ready[g]));
       }
-      const float l = l2.x + l2.y;
-      if (ok && steps > 0) ok = pv_wait(it);
+      if (ok && tiles > 0) ok = pv_wait();
       if (!ok) break;
+      const float l = l2.x + l2.y;
       tc_fence_after();
       if (careful[round & 1] == round + 1) {
         const int w0 = grow0 + (warp & 3) * 32;
@@ -649,7 +626,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll 1
       for (int q4 = 0; q4 < D / 32; ++q4) {
         float o[32];
-        if (steps > 0) {
+        if (tiles > 0) {
           tmem_ld32(o_addr + 32 * q4, o);
         } else {
 #pragma unroll

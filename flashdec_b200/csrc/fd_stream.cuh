@@ -33,6 +33,27 @@ __device__ __forceinline__ uint4 gather8(const T* src, int64_t stride) {
   return *reinterpret_cast<const uint4*>(el);
 }
 
+// 16 bytes to shared memory (of which `bytes` are read, the rest is zero).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Whether one of two packed 16-bit values is an infinity or NaN (all exponent
 // bits set).
 __device__ __forceinline__ bool nonfinite16(uint32_t w, uint32_t exp_mask) {
