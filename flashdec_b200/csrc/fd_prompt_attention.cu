@@ -150,6 +150,18 @@ __device__ __forceinline__ uint32_t low_bits(int x) {
   return x <= 0 ? 0u : (x >= 32 ? 0xffffffffu : (1u << x) - 1u);
 }
 
+// Whether the predicate holds for any of `threads` threads, which all wait here.
+__device__ __forceinline__ bool barrier_any(int id, int threads, bool x) {
+  uint32_t y;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(y)
+      : "r"(id), "r"(threads), "r"(x ? 1u : 0u)
+      : "memory");
+  return y != 0;
+}
+
 // Wait for a barrier's phase whatever the abort flag says: copies in flight
 // have to land before the CTA's shared memory is given up.
 __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
@@ -477,8 +489,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // the scale's sign goes to q
     uint32_t it = 0;
-    bool ok = true;
-    for (int rb = blockIdx.x, round = 0; ok && rb * kRows + 128 * g < rows_all; rb += gridDim.x, ++round) {
+    for (int rb = blockIdx.x, round = 0; rb * kRows + 128 * g < rows_all; rb += gridDim.x, ++round) {
+      bool ok = true;
       const StreamRange rg = range_of(rb);
       const int grow0 = rb * kRows + 128 * g;
       // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane.
@@ -562,7 +574,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
           for (int c = 0; c < 8; ++c) mx[c] = fmaxf(fmaxf(mx[c], v[i + c]), v[i + 8 + c]);
         const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+                            fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
         // The reference maximum follows the running one only when it is 2^8
         // behind: P stays below 2^8, and O is rescaled rarely.
         const bool first = m == -INFINITY;
@@ -610,7 +622,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         mbar_arrive(smem_u32(&p_ready[g]));
       }
       if (ok && tiles > 0) ok = pv_wait();
-      if (!ok) break;
+      // all warps of the group go on or none: the barriers below have no limit
+      if (barrier_any(1 + g, 128, !ok)) break;
       const float l = l2.x + l2.y;
       tc_fence_after();
       if (careful[round & 1] == round + 1) {
