@@ -30,13 +30,15 @@ struct StreamParams {
   uint32_t group_magic;  // ceil(2^32 / group): x / group = mulhi(x, magic) while x * group < 2^32 (not for group 1)
   int bs_log2, num_blocks, max_blocks;
   int window, sinks;
-  int row_blocks;  // grid extent of the row-block axis
-  int splits;      // CTAs per (sequence, KV head, row block)
+  int row_blocks;  // of the longest queries announced
+  int splits;      // most splits of a (sequence, KV head, row block)
   int vec;         // rows of K and V are 16-byte aligned and contiguous
   int q_vec, out_vec;  // the same of q and of out
   float scale_log2;
   int cluster;      // the splits of a unit form a cluster
-  int min_tiles;    // tiles a split holds at least
+  int chunk;        // tiles of a split (at least, in a cluster)
+  int rows_cta;     // rows of a row block
+  int score_vec;    // four scores of a page: one 16-byte access
   float* part_acc;  // [row = token * hq + head][split][D]
   float* part_ml;   // [row][split][2]: max (base 2), sum
   float* raw;       // [row][raw_tokens]: scaled scores (base 2)

@@ -18,8 +18,8 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTok = 16;    // tokens per warp tile
 constexpr int kStages = 3;  // tiles in flight per warp
-constexpr int kMaxSplits = 128;
 constexpr int kMaxCluster = 8;      // splits that merge inside a cluster
+constexpr int kMaxListed = 1024;    // sequences whose items a CTA counts
 constexpr int kRawBytes = 10 << 10; // scores a CTA may keep in shared memory
 
 template <int D>
@@ -39,6 +39,16 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   return x;
 }
 
+// Splits of a sequence's row blocks (of `rows` rows each): what the last block
+// sees, in runs of p.chunk tiles.
+__device__ __forceinline__ int splits_of(const StreamParams& p, const StreamSeq& s, int rows) {
+  const int all = s.qlen * p.group;
+  if (all == 0 || p.splits == 1) return 1;
+  const StreamRange rg(s, (all - 1) / rows * rows, all, p.group, p.window, p.sinks, p.bs_log2);
+  const int tiles = ((rg.pages << p.bs_log2) + kTok - 1) / kTok;
+  return min(max((tiles + p.chunk - 1) / p.chunk, 1), p.splits);
+}
+
 // Byte offset of 16-byte chunk `c` of row `r` in a [rows][D] 16-bit tile: the
 // chunk index is XORed with r % 8, so the 8 rows of an ldmatrix start on
 // different banks.
@@ -48,13 +58,20 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 }
 
 // ---------------------------------------------------------------------------
-// One CTA: rows [16 kM rb, +16 kM) of a (sequence, KV head), split `blockIdx.x`
+// One item: rows [16 kM rb, +16 kM) of a (sequence, KV head) against one split
 // of the pages they see.  Row r is head r % group of query r / group, so K and
 // V are read once for the whole group.  Tile i of 16 tokens goes to warp i % 4;
 // each warp keeps three tiles in flight with cp.async and its own maximum and
 // sum (base 2, the maximum followed only when a score passes it by 2^8), and
-// the four merge at the end.  The splits merge through distributed shared
-// memory when they form a cluster (p.cluster), else through fp32 partials and
+// the four merge at the end.
+//
+// p.cluster: the CTAs of a cluster have one item each, the splits of a (rows,
+// KV head), and merge through distributed shared memory.  Else a CTA takes
+// every gridDim.x-th item of the batch: a sequence has as many splits as its
+// length asks for, which the CTA counts from the lengths, so a ragged batch
+// launches no idle CTA (as a grid over the longest sequence's splits, 24
+// sequences of 512 to 32768 tokens took 147 us, a third of it for CTAs that
+// found nothing to do).  Splits then leave fp32 partials to
 // stream_finish_kernel.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int kM>
@@ -75,18 +92,14 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   const int t4 = lane & 3;
   const int mi = lane >> 3;
   const int r8 = lane & 7;
-  const int split = blockIdx.x;
-  const int h = blockIdx.y / p.row_blocks;
-  const int b = blockIdx.z;
   const int mask = (1 << p.bs_log2) - 1;
+  int* const upto = reinterpret_cast<int*>(raw);  // [num_seqs + 1] items before a sequence's
   // a scale of 0 (uniform weights) stays above it: -inf * 0 is NaN; its sign goes to q
   const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
 
   pdl_wait();
   pdl_launch_dependents();
-  const StreamSeq s = sequence_of(p, b);
-  const int rows_all = s.qlen * p.group;
   uint8_t* const kring = smem + warp * (kStages * 2 * kTileBytes);
   // this lane's part of a tile copy: chunk `cc` of rows cr, cr + kStep, ...
   constexpr int kStep = 32 / kChunks;
@@ -95,475 +108,535 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   const uint32_t k_off = tile_chunk<D>((mi >> 1) * 8 + r8, mi & 1);
   const uint32_t v_off = tile_chunk<D>((mi & 1) * 8 + r8, mi >> 1);
 
-  for (int rb = blockIdx.y - h * p.row_blocks; rb * kRows < rows_all; rb += p.row_blocks) {
-    const int row0 = rb * kRows;
-    const int rows = min(kRows, rows_all - row0);
-    const StreamRange rg(s, row0, row0 + rows, p.group, p.window, p.sinks, p.bs_log2);
-    const int tiles = ((rg.pages << p.bs_log2) + kTok - 1) / kTok;
-    const int per = max((tiles + p.splits - 1) / p.splits, p.min_tiles);
-    const int t0 = min(split * per, tiles);
-    const int t1 = min(t0 + per, tiles);
-
-    if (!p.cluster && p.splits > 1 && t0 >= t1 && split > 0) {  // nothing left for this split
-      if (tid < rows) {
-        const int qt = (row0 + tid) / p.group;
-        const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + h * p.group + (row0 + tid) - qt * p.group;
-        p.part_ml[(row * p.splits + split) * 2] = -INFINITY;
-        p.part_ml[(row * p.splits + split) * 2 + 1] = 0.f;
-      }
-      continue;
-    }
-
-    // lanes 0 and 1 hold the (at most two) pages of a tile: {block, position of its first token}
-    auto fetch = [&](int t, int& blk, int& pos) {
-      blk = -1;
-      pos = 0;
-      const int i = p.bs_log2 >= 4 ? (t * kTok) >> p.bs_log2 : 2 * t + lane;
-      if (lane < 2 && t < t1 && i < rg.pages) {
-        const int page = rg.page(i);
-        pos = p.bs_log2 >= 4 ? (page << p.bs_log2) + ((t * kTok) & mask) : page << p.bs_log2;
-        const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + page * p.bts1);
-        if (id >= 0 && id < p.num_blocks) {
-          blk = static_cast<int>(id);
-        } else if (pos <= rg.pos1 && (pos + (1 << min(p.bs_log2, 4)) > rg.lo || pos < rg.sink_end)) {
-          atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
-        }
-      }
-    };
-    // position of tile token `tok`, or -1 when no row sees it or its page is bad
-    auto token_pos = [&](int tok, int blk0, int blk1, int pos0, int pos1) -> int {
-      const bool second = p.bs_log2 == 3 && tok >= 8;
-      const int pos = second ? pos1 + tok - 8 : pos0 + tok;
-      const bool seen = pos <= rg.pos1 && (pos >= rg.lo || pos < rg.sink_end);
-      return (second ? blk1 : blk0) >= 0 && seen ? pos : -1;
-    };
-    // all 16 tokens seen by some row (`all`: by every row) and their pages good
-    auto whole = [&](int blk0, int blk1, int pos0, int pos1, bool all) -> bool {
-      const int hi = all ? rg.pos0 : rg.pos1;
-      const int lo = all ? max(rg.pos1 - p.window + 1, 0) : rg.lo;
-      const int se = all ? min(p.sinks, rg.pos0 + 1) : rg.sink_end;
-      auto run_ok = [&](int first, int n) { return first + n <= se || (first >= lo && first + n - 1 <= hi); };
-      if (p.bs_log2 == 3) return blk0 >= 0 && blk1 >= 0 && run_ok(pos0, 8) && run_ok(pos1, 8);
-      return blk0 >= 0 && run_ok(pos0, kTok);
-    };
-    auto issue = [&](int t, int blk, int pos) {
-      const int blk0 = __shfl_sync(0xffffffffu, blk, 0), blk1 = __shfl_sync(0xffffffffu, blk, 1);
-      const int pp0 = __shfl_sync(0xffffffffu, pos, 0), pp1 = __shfl_sync(0xffffffffu, pos, 1);
-      if (t < t1) {
-        uint8_t* kt = kring + ((t / kWarps) % kStages) * (2 * kTileBytes);
-        constexpr int kN = kTok / kStep;
-        if (p.vec && whole(blk0, blk1, pp0, pp1, false)) {
-          const T* k0 = static_cast<const T*>(p.k) + blk0 * p.ks0 + h * p.ks1 + ((pp0 & mask) + cr) * p.ks2 + cc * 8;
-          const T* v0 = static_cast<const T*>(p.v) + blk0 * p.vs0 + h * p.vs1 + ((pp0 & mask) + cr) * p.vs2 + cc * 8;
-          const T* k1 = k0 + 8 * p.ks2;
-          const T* v1 = v0 + 8 * p.vs2;
-          if (p.bs_log2 == 3) {
-            k1 = static_cast<const T*>(p.k) + blk1 * p.ks0 + h * p.ks1 + cr * p.ks2 + cc * 8;
-            v1 = static_cast<const T*>(p.v) + blk1 * p.vs0 + h * p.vs1 + cr * p.vs2 + cc * 8;
-          }
-          const int64_t kstep = kStep * p.ks2, vstep = kStep * p.vs2;
-          const uint32_t dst = smem_u32(kt);
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const uint32_t off = (copy_off + i * (kStep * D * 2)) ^ (((i * kStep) & 7) << 4);
-            cp_async16(dst + off, i < kN / 2 ? k0 : k1);
-            cp_async16(dst + kTileBytes + off, i < kN / 2 ? v0 : v1);
-            if (i < kN / 2) {
-              k0 += kstep;
-              v0 += vstep;
-            } else {
-              k1 += kstep;
-              v1 += vstep;
-            }
-          }
-        } else {
-          uint8_t* vt = kt + kTileBytes;
-#pragma unroll 1
-          for (int i = 0; i < kN; ++i) {
-            const int tok = cr + i * kStep;
-            const int tp = token_pos(tok, blk0, blk1, pp0, pp1);
-            const int64_t blkid = p.bs_log2 == 3 && tok >= 8 ? blk1 : blk0;
-            const T* ks = static_cast<const T*>(p.k);
-            const T* vs = static_cast<const T*>(p.v);
-            if (tp >= 0) {
-              ks += blkid * p.ks0 + h * p.ks1 + (tp & mask) * p.ks2 + cc * 8 * p.ks3;
-              vs += blkid * p.vs0 + h * p.vs1 + (tp & mask) * p.vs2 + cc * 8 * p.vs3;
-            }
-            const uint32_t off = tile_chunk<D>(tok, cc);
-            if (p.vec) {
-              cp_async16(smem_u32(kt) + off, ks, tp >= 0 ? 16 : 0);
-              cp_async16(smem_u32(vt) + off, vs, tp >= 0 ? 16 : 0);
-            } else {
-              const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(kt + off) = tp >= 0 ? gather8(ks, p.ks3) : zero;
-              *reinterpret_cast<uint4*>(vt + off) = tp >= 0 ? gather8(vs, p.vs3) : zero;
-            }
-          }
-        }
-      }
-      cp_async_commit();
-    };
-
-    // ---- first tiles on their way, then q ----
-    int blk[kStages], pos[kStages];  // pages of this warp's next tiles
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) fetch(t0 + warp + i * kWarps, blk[i], pos[i]);
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(t0 + warp + i * kWarps, blk[i], pos[i]);
-    for (int e = tid; e < kRows * kChunks; e += kThreads) {
-      const int r = e / kChunks, c = e % kChunks;
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) {
-        const int qt = (row0 + r) / p.group;
-        const int head = h * p.group + (row0 + r) - qt * p.group;
-        const T* src = static_cast<const T*>(p.q) + (s.q0 + qt) * p.qs0 + head * p.qs1 + c * 8 * p.qs2;
-        x = p.qs2 == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0
-                ? *reinterpret_cast<const uint4*>(src)
-                : gather8(src, p.qs2);
-        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-      }
-      *reinterpret_cast<uint4*>(qsm + tile_chunk<D>(r, c)) = x;
+  const bool listed = !p.cluster && p.num_seqs <= kMaxListed;
+  int items = p.cluster ? 1 : p.num_seqs * p.row_blocks * p.splits * p.hkv;
+  if (listed) {
+    // items of every sequence, then their running sum (warp 0)
+    for (int i = tid; i < p.num_seqs; i += kThreads) {
+      const StreamSeq s = sequence_of(p, i);
+      upto[i + 1] = ((s.qlen * p.group + kRows - 1) / kRows) * splits_of(p, s, kRows) * p.hkv;
     }
     __syncthreads();
-
-    float o[kM][D / 8][4];
-    float m[kM][2], l[kM][2];  // m in score units: P = exp2((S - m) scale)
-    int pos_r[kM][2];          // query position of this thread's rows
+    if (warp == 0) {
+      int sum = 0;
+      for (int i = 0; i < p.num_seqs; i += 32) {
+        int x = i + lane < p.num_seqs ? upto[i + lane + 1] : 0;
 #pragma unroll
-    for (int a = 0; a < kM; ++a) {
-#pragma unroll
-      for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[a][j][e] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        m[a][e] = -INFINITY;
-        l[a][e] = 0.f;
-        pos_r[a][e] = s.n - s.qlen + (row0 + 16 * a + 8 * e + g8) / p.group;
+        for (int d = 1; d < 32; d <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, d);
+          if (lane >= d) x += y;
+        }
+        if (i + lane < p.num_seqs) upto[i + lane + 1] = sum + x;
+        sum += __shfl_sync(0xffffffffu, x, 31);
       }
+      if (lane == 0) upto[0] = 0;
     }
-    uint32_t qf[D / 16][4];  // one row tile: its fragments stay in registers
-    auto load_q = [&](int a, int kk, uint32_t(&f)[4]) {
-      ldsm_x4(smem_u32(qsm) + tile_chunk<D>(16 * a + (mi & 1) * 8 + r8, 2 * kk + (mi >> 1)), f[0],
-              f[1], f[2], f[3]);
-    };
-    if constexpr (kM == 1) {
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) load_q(0, kk, qf[kk]);
-    }
-    const float slack = 8.f / scale;
-
-    for (int t = t0 + warp; t < t1; t += kWarps) {
-      issue(t + (kStages - 1) * kWarps, blk[kStages - 1], pos[kStages - 1]);
-      const int cb0 = __shfl_sync(0xffffffffu, blk[0], 0), cb1 = __shfl_sync(0xffffffffu, blk[0], 1);
-      const int cp0 = __shfl_sync(0xffffffffu, pos[0], 0), cp1 = __shfl_sync(0xffffffffu, pos[0], 1);
-#pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) {
-        blk[i] = blk[i + 1];
-        pos[i] = pos[i + 1];
-      }
-      fetch(t + kStages * kWarps, blk[kStages - 1], pos[kStages - 1]);
-      cp_async_wait<kStages - 1>();
-      __syncwarp();
-      uint8_t* kt = kring + ((t / kWarps) % kStages) * (2 * kTileBytes);
-      uint8_t* vt = kt + kTileBytes;
-
-      float sc[kM][2][4];
-#pragma unroll
-      for (int a = 0; a < kM; ++a)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[a][j][e] = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4(smem_u32(kt) + (k_off ^ (kk << 5)), b0, b1, b2, b3);
-#pragma unroll
-        for (int a = 0; a < kM; ++a) {
-          if constexpr (kM == 1) {
-            mma_16816<T>(sc[a][0], qf[kk], b0, b1);
-            mma_16816<T>(sc[a][1], qf[kk], b2, b3);
+    __syncthreads();
+    items = upto[p.num_seqs];
+  }
+  for (int item = p.cluster ? 0 : blockIdx.x; item < items; item += gridDim.x) {
+    // ---- the item: heads of a split are neighbours, then splits, row blocks, sequences ----
+    int b, h, split, rb0, splits = p.splits;
+    StreamSeq s;
+    if (p.cluster) {
+      b = blockIdx.z;
+      h = blockIdx.y % p.hkv;
+      split = blockIdx.x;
+      rb0 = blockIdx.y / p.hkv;
+      s = sequence_of(p, b);
+    } else {
+      int x = item, of;
+      if (listed) {
+        int lo = 0, hi = p.num_seqs;  // upto[lo] <= item < upto[hi]
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (upto[mid] <= item) {
+            lo = mid;
           } else {
-            uint32_t f[4];
-            load_q(a, kk, f);
-            mma_16816<T>(sc[a][0], f, b0, b1);
-            mma_16816<T>(sc[a][1], f, b2, b3);
+            hi = mid;
           }
         }
+        b = lo;
+        x -= upto[lo];
+        s = sequence_of(p, b);
+        of = splits = splits_of(p, s, kRows);
+      } else {
+        const int per_seq = p.row_blocks * p.splits * p.hkv;
+        b = x / per_seq;
+        x -= b * per_seq;
+        s = sequence_of(p, b);
+        splits = splits_of(p, s, kRows);
+        of = p.splits;
       }
-      // ---- masks, where some row misses some token ----
-      const bool edge = !whole(cb0, cb1, cp0, cp1, true);
-      uint32_t vis = 0xffffffffu;  // bit (a, j, e): the row sees the token
-      if (edge) {
-        int kp[2][2];  // positions of this thread's four tokens, -1: seen by no row
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) kp[j][e] = token_pos(8 * j + 2 * t4 + e, cb0, cb1, cp0, cp1);
-        vis = 0;
-#pragma unroll
-        for (int a = 0; a < kM; ++a)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = kp[j][e & 1];
-              const int at = pos_r[a][e >> 1];
-              const bool on = key >= 0 && key <= at && (key > at - p.window || key < p.sinks);
-              if (!on) sc[a][j][e] = -INFINITY;
-              vis |= (on ? 1u : 0u) << (a * 8 + j * 4 + e);
+      h = x % p.hkv;
+      x /= p.hkv;
+      split = x % of;
+      rb0 = x / of;
+    }
+    const int rows_all = s.qlen * p.group;
+    if (split >= splits) continue;
+    // more than one row block where the grid or the list of items is sized by
+    // the longest queries announced, and they are longer
+    for (int rb = rb0; rb * kRows < rows_all; rb += listed ? rows_all : p.row_blocks) {
+      const int row0 = rb * kRows;
+      const int rows = min(kRows, rows_all - row0);
+      const StreamRange rg(s, row0, row0 + rows, p.group, p.window, p.sinks, p.bs_log2);
+      const int tiles = ((rg.pages << p.bs_log2) + kTok - 1) / kTok;
+      const int per = max((tiles + splits - 1) / splits, p.cluster ? p.chunk : 1);
+      const int t0 = min(split * per, tiles);
+      const int t1 = min(t0 + per, tiles);
+
+      // lanes 0 and 1 hold the (at most two) pages of a tile: {block, position of its first token}
+      auto fetch = [&](int t, int& blk, int& pos) {
+        blk = -1;
+        pos = 0;
+        const int i = p.bs_log2 >= 4 ? (t * kTok) >> p.bs_log2 : 2 * t + lane;
+        if (lane < 2 && t < t1 && i < rg.pages) {
+          const int page = rg.page(i);
+          pos = p.bs_log2 >= 4 ? (page << p.bs_log2) + ((t * kTok) & mask) : page << p.bs_log2;
+          const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + page * p.bts1);
+          if (id >= 0 && id < p.num_blocks) {
+            blk = static_cast<int>(id);
+          } else if (pos <= rg.pos1 && (pos + (1 << min(p.bs_log2, 4)) > rg.lo || pos < rg.sink_end)) {
+            atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
+          }
+        }
+      };
+      // position of tile token `tok`, or -1 when no row sees it or its page is bad
+      auto token_pos = [&](int tok, int blk0, int blk1, int pos0, int pos1) -> int {
+        const bool second = p.bs_log2 == 3 && tok >= 8;
+        const int pos = second ? pos1 + tok - 8 : pos0 + tok;
+        const bool seen = pos <= rg.pos1 && (pos >= rg.lo || pos < rg.sink_end);
+        return (second ? blk1 : blk0) >= 0 && seen ? pos : -1;
+      };
+      // all 16 tokens seen by some row (`all`: by every row) and their pages good
+      auto whole = [&](int blk0, int blk1, int pos0, int pos1, bool all) -> bool {
+        const int hi = all ? rg.pos0 : rg.pos1;
+        const int lo = all ? max(rg.pos1 - p.window + 1, 0) : rg.lo;
+        const int se = all ? min(p.sinks, rg.pos0 + 1) : rg.sink_end;
+        auto run_ok = [&](int first, int n) { return first + n <= se || (first >= lo && first + n - 1 <= hi); };
+        if (p.bs_log2 == 3) return blk0 >= 0 && blk1 >= 0 && run_ok(pos0, 8) && run_ok(pos1, 8);
+        return blk0 >= 0 && run_ok(pos0, kTok);
+      };
+      auto issue = [&](int t, int blk, int pos) {
+        const int blk0 = __shfl_sync(0xffffffffu, blk, 0), blk1 = __shfl_sync(0xffffffffu, blk, 1);
+        const int pp0 = __shfl_sync(0xffffffffu, pos, 0), pp1 = __shfl_sync(0xffffffffu, pos, 1);
+        if (t < t1) {
+          uint8_t* kt = kring + ((t / kWarps) % kStages) * (2 * kTileBytes);
+          constexpr int kN = kTok / kStep;
+          if (p.vec && whole(blk0, blk1, pp0, pp1, false)) {
+            const T* k0 = static_cast<const T*>(p.k) + blk0 * p.ks0 + h * p.ks1 + ((pp0 & mask) + cr) * p.ks2 + cc * 8;
+            const T* v0 = static_cast<const T*>(p.v) + blk0 * p.vs0 + h * p.vs1 + ((pp0 & mask) + cr) * p.vs2 + cc * 8;
+            const T* k1 = k0 + 8 * p.ks2;
+            const T* v1 = v0 + 8 * p.vs2;
+            if (p.bs_log2 == 3) {
+              k1 = static_cast<const T*>(p.k) + blk1 * p.ks0 + h * p.ks1 + cr * p.ks2 + cc * 8;
+              v1 = static_cast<const T*>(p.v) + blk1 * p.vs0 + h * p.vs1 + cr * p.vs2 + cc * 8;
             }
-      }
-      if (p.scores) {  // one query: row = head of the group; list place = position
-        float* dst = p.cluster ? raw + (t - t0) * kTok
-                               : p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens + t * kTok;
+            const int64_t kstep = kStep * p.ks2, vstep = kStep * p.vs2;
+            const uint32_t dst = smem_u32(kt);
 #pragma unroll
-        for (int a = 0; a < kM; ++a)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = 16 * a + 8 * e + g8;
-            if (r < rows) {  // rows are padded to whole tiles
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                *reinterpret_cast<float2*>(dst + r * p.raw_tokens + 8 * j + 2 * t4) =
-                    make_float2(sc[a][j][2 * e] * scale, sc[a][j][2 * e + 1] * scale);
+            for (int i = 0; i < kN; ++i) {
+              const uint32_t off = (copy_off + i * (kStep * D * 2)) ^ (((i * kStep) & 7) << 4);
+              cp_async16(dst + off, i < kN / 2 ? k0 : k1);
+              cp_async16(dst + kTileBytes + off, i < kN / 2 ? v0 : v1);
+              if (i < kN / 2) {
+                k0 += kstep;
+                v0 += vstep;
+              } else {
+                k1 += kstep;
+                v1 += vstep;
+              }
+            }
+          } else {
+            uint8_t* vt = kt + kTileBytes;
+#pragma unroll 1
+            for (int i = 0; i < kN; ++i) {
+              const int tok = cr + i * kStep;
+              const int tp = token_pos(tok, blk0, blk1, pp0, pp1);
+              const int64_t blkid = p.bs_log2 == 3 && tok >= 8 ? blk1 : blk0;
+              const T* ks = static_cast<const T*>(p.k);
+              const T* vs = static_cast<const T*>(p.v);
+              if (tp >= 0) {
+                ks += blkid * p.ks0 + h * p.ks1 + (tp & mask) * p.ks2 + cc * 8 * p.ks3;
+                vs += blkid * p.vs0 + h * p.vs1 + (tp & mask) * p.vs2 + cc * 8 * p.vs3;
+              }
+              const uint32_t off = tile_chunk<D>(tok, cc);
+              if (p.vec) {
+                cp_async16(smem_u32(kt) + off, ks, tp >= 0 ? 16 : 0);
+                cp_async16(smem_u32(vt) + off, vs, tp >= 0 ? 16 : 0);
+              } else {
+                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(kt + off) = tp >= 0 ? gather8(ks, p.ks3) : zero;
+                *reinterpret_cast<uint4*>(vt + off) = tp >= 0 ? gather8(vs, p.vs3) : zero;
+              }
             }
           }
+        }
+        cp_async_commit();
+      };
+
+      // ---- first tiles on their way, then q ----
+      int blk[kStages], pos[kStages];  // pages of this warp's next tiles
+#pragma unroll
+      for (int i = 0; i < kStages; ++i) fetch(t0 + warp + i * kWarps, blk[i], pos[i]);
+#pragma unroll
+      for (int i = 0; i < kStages - 1; ++i) issue(t0 + warp + i * kWarps, blk[i], pos[i]);
+      for (int e = tid; e < kRows * kChunks; e += kThreads) {
+        const int r = e / kChunks, c = e % kChunks;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) {
+          const int qt = (row0 + r) / p.group;
+          const int head = h * p.group + (row0 + r) - qt * p.group;
+          const T* src = static_cast<const T*>(p.q) + (s.q0 + qt) * p.qs0 + head * p.qs1 + c * 8 * p.qs2;
+          x = p.qs2 == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0
+                  ? *reinterpret_cast<const uint4*>(src)
+                  : gather8(src, p.qs2);
+          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+        }
+        *reinterpret_cast<uint4*>(qsm + tile_chunk<D>(r, c)) = x;
       }
-      // ---- follow the maximum when it is 2^8 behind ----
-      bool behind = false;
-#pragma unroll
-      for (int a = 0; a < kM; ++a)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          behind |= fmaxf(fmaxf(sc[a][0][2 * e], sc[a][0][2 * e + 1]),
-                          fmaxf(sc[a][1][2 * e], sc[a][1][2 * e + 1])) > m[a][e] + slack;
-      if (__any_sync(0xffffffffu, behind)) {
-#pragma unroll
-        for (int a = 0; a < kM; ++a)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(fmaxf(sc[a][0][2 * e], sc[a][0][2 * e + 1]),
-                             fmaxf(sc[a][1][2 * e], sc[a][1][2 * e + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[a][e], mx);
-            const float alpha = mn == -INFINITY ? 1.f : ex2((m[a][e] - mn) * scale);
-            m[a][e] = mn;
-            l[a][e] *= alpha;
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j) {
-              o[a][j][2 * e] *= alpha;
-              o[a][j][2 * e + 1] *= alpha;
-            }
-          }
-      }
-      // ---- weights, rounded to the type of V for the product ----
-      uint32_t pf[kM][4];
+      __syncthreads();
+
+      float o[kM][D / 8][4];
+      float m[kM][2], l[kM][2];  // m in score units: P = exp2((S - m) scale)
+      int pos_r[kM][2];          // query position of this thread's rows
 #pragma unroll
       for (int a = 0; a < kM; ++a) {
 #pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[a][j][e] = 0.f;
+#pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float base = m[a][e] == -INFINITY ? 0.f : m[a][e] * scale;
+          m[a][e] = -INFINITY;
+          l[a][e] = 0.f;
+          pos_r[a][e] = s.n - s.qlen + (row0 + 16 * a + 8 * e + g8) / p.group;
+        }
+      }
+      uint32_t qf[D / 16][4];  // one row tile: its fragments stay in registers
+      auto load_q = [&](int a, int kk, uint32_t(&f)[4]) {
+        ldsm_x4(smem_u32(qsm) + tile_chunk<D>(16 * a + (mi & 1) * 8 + r8, 2 * kk + (mi >> 1)), f[0],
+                f[1], f[2], f[3]);
+      };
+      if constexpr (kM == 1) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) load_q(0, kk, qf[kk]);
+      }
+      const float slack = 8.f / scale;
+
+      for (int t = t0 + warp; t < t1; t += kWarps) {
+        issue(t + (kStages - 1) * kWarps, blk[kStages - 1], pos[kStages - 1]);
+        const int cb0 = __shfl_sync(0xffffffffu, blk[0], 0), cb1 = __shfl_sync(0xffffffffu, blk[0], 1);
+        const int cp0 = __shfl_sync(0xffffffffu, pos[0], 0), cp1 = __shfl_sync(0xffffffffu, pos[0], 1);
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) {
+          blk[i] = blk[i + 1];
+          pos[i] = pos[i + 1];
+        }
+        fetch(t + kStages * kWarps, blk[kStages - 1], pos[kStages - 1]);
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        uint8_t* kt = kring + ((t / kWarps) % kStages) * (2 * kTileBytes);
+        uint8_t* vt = kt + kTileBytes;
+
+        float sc[kM][2][4];
+#pragma unroll
+        for (int a = 0; a < kM; ++a)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& x = sc[a][j][2 * e + i];
-              x = ex2(fmaf(x, scale, -base));
-              l[a][e] += x;
+            for (int e = 0; e < 4; ++e) sc[a][j][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t b0, b1, b2, b3;
+          ldsm_x4(smem_u32(kt) + (k_off ^ (kk << 5)), b0, b1, b2, b3);
+#pragma unroll
+          for (int a = 0; a < kM; ++a) {
+            if constexpr (kM == 1) {
+              mma_16816<T>(sc[a][0], qf[kk], b0, b1);
+              mma_16816<T>(sc[a][1], qf[kk], b2, b3);
+            } else {
+              uint32_t f[4];
+              load_q(a, kk, f);
+              mma_16816<T>(sc[a][0], f, b0, b1);
+              mma_16816<T>(sc[a][1], f, b2, b3);
             }
+          }
         }
-        pf[a][0] = pack2<T>(sc[a][0][0], sc[a][0][1]);
-        pf[a][1] = pack2<T>(sc[a][0][2], sc[a][0][3]);
-        pf[a][2] = pack2<T>(sc[a][1][0], sc[a][1][1]);
-        pf[a][3] = pack2<T>(sc[a][1][2], sc[a][1][3]);
-      }
-      // A token that some rows of the block see and others do not: an
-      // infinity or NaN in its V row must not reach the others (0 * inf), so
-      // such elements leave the tile and are added row by row.
-      if (edge && rg.pos0 != rg.pos1) {
-        constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-        bool odd = false;
+        // ---- masks, where some row misses some token ----
+        const bool edge = !whole(cb0, cb1, cp0, cp1, true);
+        uint32_t vis = 0xffffffffu;  // bit (a, j, e): the row sees the token
+        if (edge) {
+          int kp[2][2];  // positions of this thread's four tokens, -1: seen by no row
 #pragma unroll
-        for (int i = 0; i < kTok * kChunks / 32; ++i) {
-          const uint4 x = *reinterpret_cast<const uint4*>(vt + (lane + 32 * i) * 16);
-          odd |= nonfinite16(x.x, kExp) | nonfinite16(x.y, kExp) | nonfinite16(x.z, kExp) |
-                 nonfinite16(x.w, kExp);
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) kp[j][e] = token_pos(8 * j + 2 * t4 + e, cb0, cb1, cp0, cp1);
+          vis = 0;
+#pragma unroll
+          for (int a = 0; a < kM; ++a)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = kp[j][e & 1];
+                const int at = pos_r[a][e >> 1];
+                const bool on = key >= 0 && key <= at && (key > at - p.window || key < p.sinks);
+                if (!on) sc[a][j][e] = -INFINITY;
+                vis |= (on ? 1u : 0u) << (a * 8 + j * 4 + e);
+              }
         }
-        if (__any_sync(0xffffffffu, odd)) {
-          for (int tok = 0; tok < kTok; ++tok) {
-            const int src = (lane & ~3) | ((tok & 7) >> 1);  // same rows, the lane with this token
+        if (p.scores) {  // one query: row = head of the group; list place = position
+          float* dst = p.cluster ? raw + (t - t0) * kTok
+                                 : p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens + t * kTok;
 #pragma unroll
-            for (int a = 0; a < kM; ++a)
+          for (int a = 0; a < kM; ++a)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float pv = 0.f;
-                bool on = false;
+            for (int e = 0; e < 2; ++e) {
+              const int r = 16 * a + 8 * e + g8;
+              if (r < rows) {  // rows are padded to whole tiles
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
-#pragma unroll
-                  for (int i = 0; i < 2; ++i) {
-                    const float x = __shfl_sync(0xffffffffu, sc[a][j][2 * e + i], src);
-                    const uint32_t w = __shfl_sync(0xffffffffu, vis, src);
-                    if (j == (tok >> 3) && i == (tok & 1)) {
-                      pv = x;
-                      on = (w >> (a * 8 + j * 4 + 2 * e + i)) & 1u;
-                    }
-                  }
-                if (!on) continue;
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                  for (int i = 0; i < 2; ++i) {
-                    const float x = to_f32<T>(*reinterpret_cast<const T*>(
-                        vt + tile_chunk<D>(tok, j) + (2 * t4 + i) * 2));
-                    if (!isfinite(x)) o[a][j][2 * e + i] += pv * x;
-                  }
+                  *reinterpret_cast<float2*>(dst + r * p.raw_tokens + 8 * j + 2 * t4) =
+                      make_float2(sc[a][j][2 * e] * scale, sc[a][j][2 * e + 1] * scale);
               }
-            __syncwarp();
-          }
-          for (int i = lane; i < kTok * D; i += 32) {
-            T* x = reinterpret_cast<T*>(vt) + i;
-            if (!isfinite(to_f32<T>(*x))) *x = from_f32<T>(0.f);
-          }
-          __syncwarp();
+            }
         }
-      }
+        // ---- follow the maximum when it is 2^8 behind ----
+        bool behind = false;
 #pragma unroll
-      for (int dp = 0; dp < D / 16; ++dp) {
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4_t(smem_u32(vt) + (v_off ^ (dp << 5)), b0, b1, b2, b3);
+        for (int a = 0; a < kM; ++a)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            behind |= fmaxf(fmaxf(sc[a][0][2 * e], sc[a][0][2 * e + 1]),
+                            fmaxf(sc[a][1][2 * e], sc[a][1][2 * e + 1])) > m[a][e] + slack;
+        if (__any_sync(0xffffffffu, behind)) {
+#pragma unroll
+          for (int a = 0; a < kM; ++a)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(fmaxf(sc[a][0][2 * e], sc[a][0][2 * e + 1]),
+                               fmaxf(sc[a][1][2 * e], sc[a][1][2 * e + 1]));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+              const float mn = fmaxf(m[a][e], mx);
+              const float alpha = mn == -INFINITY ? 1.f : ex2((m[a][e] - mn) * scale);
+              m[a][e] = mn;
+              l[a][e] *= alpha;
+#pragma unroll
+              for (int j = 0; j < D / 8; ++j) {
+                o[a][j][2 * e] *= alpha;
+                o[a][j][2 * e + 1] *= alpha;
+              }
+            }
+        }
+        // ---- weights, rounded to the type of V for the product ----
+        uint32_t pf[kM][4];
 #pragma unroll
         for (int a = 0; a < kM; ++a) {
-          mma_16816<T>(o[a][2 * dp], pf[a], b0, b1);
-          mma_16816<T>(o[a][2 * dp + 1], pf[a], b2, b3);
-        }
-      }
-      __syncwarp();  // the stage is free
-    }
-
-    // ---- merge the warps: (max, sum, acc) per row through the ring ----
-    cp_async_wait<0>();
-    __syncthreads();
-    float* acc = reinterpret_cast<float*>(smem);  // [warp][row][D], then the CTA's in [0]
-    float* ml = acc + kWarps * kRows * D;         // [warp][row][2]
-    static_assert(sizeof(float) * kWarps * kRows * (D + 2) <= ring_bytes<D>(), "merge buffer");
 #pragma unroll
-    for (int a = 0; a < kM; ++a)
+          for (int e = 0; e < 2; ++e) {
+            const float base = m[a][e] == -INFINITY ? 0.f : m[a][e] * scale;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[a][e];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const int r = 16 * a + 8 * e + g8;
-        if (r >= rows) continue;
-        float* dst = acc + (warp * kRows + r) * D;
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j)
-          *reinterpret_cast<float2*>(dst + 8 * j + 2 * t4) =
-              make_float2(o[a][j][2 * e], o[a][j][2 * e + 1]);
-        if (t4 == 0) {
-          ml[(warp * kRows + r) * 2] = m[a][e] * scale;
-          ml[(warp * kRows + r) * 2 + 1] = sum;
-        }
-      }
-    __syncthreads();
-    for (int e = tid; e < rows * D; e += kThreads) {
-      const int r = e / D, d = e - r * D;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[(w * kRows + r) * 2]);
-      const float base = mx == -INFINITY ? 0.f : mx;
-      float sum = 0.f, x = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = ex2(ml[(w * kRows + r) * 2] - base);
-        sum += f * ml[(w * kRows + r) * 2 + 1];
-        x += f * acc[(w * kRows + r) * D + d];
-      }
-      const int qt = (row0 + r) / p.group;
-      const int head = h * p.group + (row0 + r) - qt * p.group;
-      const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
-      if (p.splits == 1) {
-        static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] =
-            from_f32<T>(sum == 0.f ? 0.f : x / sum);
-      } else if (p.cluster) {
-        acc[e] = x;  // warp 0's place of the same element
-      } else {
-        p.part_acc[(row * p.splits + split) * D + d] = x;
-      }
-      if (d == 0) {
-        if (p.cluster) {
-          cml[2 * r] = mx;
-          cml[2 * r + 1] = sum;
-        } else if (p.part_ml) {
-          p.part_ml[(row * p.splits + split) * 2] = mx;
-          p.part_ml[(row * p.splits + split) * 2 + 1] = sum;
-        }
-      }
-    }
-    if (p.cluster) {
-      // ---- merge the cluster's splits: every CTA its share of the elements ----
-      cluster_arrive();
-      cluster_wait();
-      for (int r = tid; r < rows; r += kThreads) {
-        float pm[kMaxCluster], pl[kMaxCluster], mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kMaxCluster; ++i) {
-          pm[i] = -INFINITY;
-          pl[i] = 0.f;
-          if (i < p.splits) {
-            const uint32_t at = map_to_rank(smem_u32(&cml[2 * r]), i);
-            pm[i] = ld_cluster(at);
-            pl[i] = ld_cluster(at + 4);
+              for (int i = 0; i < 2; ++i) {
+                float& x = sc[a][j][2 * e + i];
+                x = ex2(fmaf(x, scale, -base));
+                l[a][e] += x;
+              }
           }
-          mx = fmaxf(mx, pm[i]);
+          pf[a][0] = pack2<T>(sc[a][0][0], sc[a][0][1]);
+          pf[a][1] = pack2<T>(sc[a][0][2], sc[a][0][3]);
+          pf[a][2] = pack2<T>(sc[a][1][0], sc[a][1][1]);
+          pf[a][3] = pack2<T>(sc[a][1][2], sc[a][1][3]);
         }
-        const float base = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f;
+        // A token that some rows of the block see and others do not: an
+        // infinity or NaN in its V row must not reach the others (0 * inf), so
+        // such elements leave the tile and are added row by row.
+        if (edge && rg.pos0 != rg.pos1) {
+          constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+          bool odd = false;
 #pragma unroll
-        for (int i = 0; i < kMaxCluster; ++i) sum += ex2(pm[i] - base) * pl[i];
+          for (int i = 0; i < kTok * kChunks / 32; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vt + (lane + 32 * i) * 16);
+            odd |= nonfinite16(x.x, kExp) | nonfinite16(x.y, kExp) | nonfinite16(x.z, kExp) |
+                   nonfinite16(x.w, kExp);
+          }
+          if (__any_sync(0xffffffffu, odd)) {
+            for (int tok = 0; tok < kTok; ++tok) {
+              const int src = (lane & ~3) | ((tok & 7) >> 1);  // same rows, the lane with this token
 #pragma unroll
-        for (int i = 0; i < kMaxCluster; ++i)
-          weight[i * kRows + r] = sum == 0.f ? 0.f : ex2(pm[i] - base) / sum;
-        lse[r] = sum == 0.f ? INFINITY : base + log2f(sum);
+              for (int a = 0; a < kM; ++a)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  float pv = 0.f;
+                  bool on = false;
+#pragma unroll
+                  for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                      const float x = __shfl_sync(0xffffffffu, sc[a][j][2 * e + i], src);
+                      const uint32_t w = __shfl_sync(0xffffffffu, vis, src);
+                      if (j == (tok >> 3) && i == (tok & 1)) {
+                        pv = x;
+                        on = (w >> (a * 8 + j * 4 + 2 * e + i)) & 1u;
+                      }
+                    }
+                  if (!on) continue;
+#pragma unroll
+                  for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                      const float x = to_f32<T>(*reinterpret_cast<const T*>(
+                          vt + tile_chunk<D>(tok, j) + (2 * t4 + i) * 2));
+                      if (!isfinite(x)) o[a][j][2 * e + i] += pv * x;
+                    }
+                }
+              __syncwarp();
+            }
+            for (int i = lane; i < kTok * D; i += 32) {
+              T* x = reinterpret_cast<T*>(vt) + i;
+              if (!isfinite(to_f32<T>(*x))) *x = from_f32<T>(0.f);
+            }
+            __syncwarp();
+          }
+        }
+#pragma unroll
+        for (int dp = 0; dp < D / 16; ++dp) {
+          uint32_t b0, b1, b2, b3;
+          ldsm_x4_t(smem_u32(vt) + (v_off ^ (dp << 5)), b0, b1, b2, b3);
+#pragma unroll
+          for (int a = 0; a < kM; ++a) {
+            mma_16816<T>(o[a][2 * dp], pf[a], b0, b1);
+            mma_16816<T>(o[a][2 * dp + 1], pf[a], b2, b3);
+          }
+        }
+        __syncwarp();  // the stage is free
       }
+
+      // ---- merge the warps: (max, sum, acc) per row through the ring ----
+      cp_async_wait<0>();
       __syncthreads();
-      for (int e = split * kThreads + tid; e < rows * D; e += p.splits * kThreads) {
-        const int r = e / D, d = e - r * D;
-        float x = 0.f;
+      float* acc = reinterpret_cast<float*>(smem);  // [warp][row][D], then the CTA's in [0]
+      float* ml = acc + kWarps * kRows * D;         // [warp][row][2]
+      static_assert(sizeof(float) * kWarps * kRows * (D + 2) <= ring_bytes<D>(), "merge buffer");
 #pragma unroll
-        for (int i = 0; i < kMaxCluster; ++i)
-          if (i < p.splits) x += weight[i * kRows + r] * ld_cluster(map_to_rank(smem_u32(acc + e), i));
+      for (int a = 0; a < kM; ++a)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[a][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          const int r = 16 * a + 8 * e + g8;
+          if (r >= rows) continue;
+          float* dst = acc + (warp * kRows + r) * D;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j)
+            *reinterpret_cast<float2*>(dst + 8 * j + 2 * t4) =
+                make_float2(o[a][j][2 * e], o[a][j][2 * e + 1]);
+          if (t4 == 0) {
+            ml[(warp * kRows + r) * 2] = m[a][e] * scale;
+            ml[(warp * kRows + r) * 2 + 1] = sum;
+          }
+        }
+      __syncthreads();
+      for (int e = tid; e < rows * D; e += kThreads) {
+        const int r = e / D, d = e - r * D;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[(w * kRows + r) * 2]);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f, x = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = ex2(ml[(w * kRows + r) * 2] - base);
+          sum += f * ml[(w * kRows + r) * 2 + 1];
+          x += f * acc[(w * kRows + r) * D + d];
+        }
         const int qt = (row0 + r) / p.group;
         const int head = h * p.group + (row0 + r) - qt * p.group;
-        static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] = from_f32<T>(x);
-      }
-      if (p.scores) {
-        for (int i = tid; i < (t1 - t0) * kTok; i += kThreads) {
-          const int tok = t0 * kTok + i;
-          if (tok >= s.n) break;
-          const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(tok >> p.bs_log2) * p.bts1);
-          if (id < 0 || id >= p.num_blocks) continue;
-          float* dst = p.scores + id * p.scs0 + h * p.scs1 + (tok & mask) * p.scs2;
-          const float old = tok == s.n - 1 ? 0.f : *dst;
-          float w = 0.f;
-          for (int r = 0; r < rows; ++r) w += ex2(raw[r * p.raw_tokens + i] - lse[r]);
-          *dst = old + w;
+        const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
+        if (splits == 1) {
+          static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] =
+              from_f32<T>(sum == 0.f ? 0.f : x / sum);
+        } else if (p.cluster) {
+          acc[e] = x;  // warp 0's place of the same element
+        } else {
+          p.part_acc[(row * p.splits + split) * D + d] = x;
+        }
+        if (d == 0) {
+          if (p.cluster) {
+            cml[2 * r] = mx;
+            cml[2 * r + 1] = sum;
+          } else if (p.part_ml) {
+            p.part_ml[(row * p.splits + split) * 2] = mx;
+            p.part_ml[(row * p.splits + split) * 2 + 1] = sum;
+          }
         }
       }
-      cluster_arrive();  // the others have read this CTA's partials
-      cluster_wait();
+      if (p.cluster) {
+        // ---- merge the cluster's splits: every CTA its share of the elements ----
+        cluster_arrive();
+        cluster_wait();
+        for (int r = tid; r < rows; r += kThreads) {
+          float pm[kMaxCluster], pl[kMaxCluster], mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kMaxCluster; ++i) {
+            pm[i] = -INFINITY;
+            pl[i] = 0.f;
+            if (i < p.splits) {
+              const uint32_t at = map_to_rank(smem_u32(&cml[2 * r]), i);
+              pm[i] = ld_cluster(at);
+              pl[i] = ld_cluster(at + 4);
+            }
+            mx = fmaxf(mx, pm[i]);
+          }
+          const float base = mx == -INFINITY ? 0.f : mx;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < kMaxCluster; ++i) sum += ex2(pm[i] - base) * pl[i];
+#pragma unroll
+          for (int i = 0; i < kMaxCluster; ++i)
+            weight[i * kRows + r] = sum == 0.f ? 0.f : ex2(pm[i] - base) / sum;
+          lse[r] = sum == 0.f ? INFINITY : base + log2f(sum);
+        }
+        __syncthreads();
+        for (int e = split * kThreads + tid; e < rows * D; e += p.splits * kThreads) {
+          const int r = e / D, d = e - r * D;
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < kMaxCluster; ++i)
+            if (i < p.splits) x += weight[i * kRows + r] * ld_cluster(map_to_rank(smem_u32(acc + e), i));
+          const int qt = (row0 + r) / p.group;
+          const int head = h * p.group + (row0 + r) - qt * p.group;
+          static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] = from_f32<T>(x);
+        }
+        if (p.scores) {
+          for (int i = tid; i < (t1 - t0) * kTok; i += kThreads) {
+            const int tok = t0 * kTok + i;
+            if (tok >= s.n) break;
+            const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(tok >> p.bs_log2) * p.bts1);
+            if (id < 0 || id >= p.num_blocks) continue;
+            float* dst = p.scores + id * p.scs0 + h * p.scs1 + (tok & mask) * p.scs2;
+            const float old = tok == s.n - 1 ? 0.f : *dst;
+            float w = 0.f;
+            for (int r = 0; r < rows; ++r) w += ex2(raw[r * p.raw_tokens + i] - lse[r]);
+            *dst = old + w;
+          }
+        }
+        cluster_arrive();  // the others have read this CTA's partials
+        cluster_wait();
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
 // What remains after the split kernel: rows whose splits are partials are
-// merged (one row a CTA at a time), and with scores every
-// token gets the sum over the group of exp2(raw - lse).
+// merged (one row a CTA at a time), and with scores every token gets the sum
+// over the group of exp2(raw - lse), four neighbouring tokens a thread.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_constant__ StreamParams p) {
   extern __shared__ float lse[];  // [group], with scores
@@ -578,19 +651,40 @@ __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_co
   pdl_launch_dependents();
   const StreamSeq s = sequence_of(p, b);
   const int rows_all = s.qlen * p.group;
+  const int splits = splits_of(p, s, p.rows_cta);
+  const int t = 4 * (blockIdx.x * kThreads + tid);  // this thread's first tokens
+  const bool scores_here = p.scores && 4 * static_cast<int>(blockIdx.x) * kThreads < s.n;
+  if (!scores_here && (splits == 1 || static_cast<int>(blockIdx.x) >= rows_all)) return;
+  // the tokens' slot and old scores, on their way while the rows are merged
+  float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
+  float* slot = nullptr;
+  auto look = [&](int at) {  // four tokens: one page
+    slot = nullptr;
+    if (at >= s.n) return;
+    const int64_t id =
+        load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(at >> p.bs_log2) * p.bts1);
+    if (id < 0 || id >= p.num_blocks) return;
+    slot = p.scores + id * p.scs0 + h * p.scs1 + (at & ((1 << p.bs_log2) - 1)) * p.scs2;
+    if (p.score_vec) {
+      old = *reinterpret_cast<const float4*>(slot);
+    } else {
+      old = make_float4(slot[0], slot[p.scs2], slot[2 * p.scs2], slot[3 * p.scs2]);
+    }
+  };
+  if (scores_here) look(t);
   // max and sum over the splits of a row, by one warp
   auto row_stats = [&](const float* ml, float& base, float& sum) {
     float mx = -INFINITY;
-    for (int i = lane; i < p.splits; i += 32) mx = fmaxf(mx, ml[2 * i]);
+    for (int i = lane; i < splits; i += 32) mx = fmaxf(mx, ml[2 * i]);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
     base = mx == -INFINITY ? 0.f : mx;
     sum = 0.f;
-    for (int i = lane; i < p.splits; i += 32) sum += ex2(ml[2 * i] - base) * ml[2 * i + 1];
+    for (int i = lane; i < splits; i += 32) sum += ex2(ml[2 * i] - base) * ml[2 * i + 1];
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   };
-  if (p.splits > 1) {
+  if (splits > 1) {
     for (int r = blockIdx.x; r < rows_all; r += gridDim.x) {
       const int qt = r / p.group;
       const int head = h * p.group + r - qt * p.group;
@@ -603,10 +697,8 @@ __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_co
 #pragma unroll
       for (int j = 0; j < kPer; ++j) x[j] = 0.f;
 #pragma unroll 8
-      for (int i = warp; i < p.splits; i += kWarps) {
-        const float mx = ml[2 * i];
-        if (mx == -INFINITY && ml[2 * i + 1] == 0.f) continue;  // no partial there
-        const float w = ex2(mx - base);
+      for (int i = warp; i < splits; i += kWarps) {
+        const float w = ex2(ml[2 * i] - base);
         float y[kPer];
         if constexpr (kPer == 4) {
           *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(p.part_acc + (row * p.splits + i) * D + lane * 4);
@@ -627,7 +719,7 @@ __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_co
       __syncthreads();
     }
   }
-  if (!p.scores || static_cast<int>(blockIdx.x) * kThreads >= s.n) return;
+  if (!scores_here) return;
   for (int g = warp; g < p.group; g += kWarps) {
     float base, sum;
     row_stats(p.part_ml + (static_cast<int64_t>(b) * p.hq + h * p.group + g) * p.splits * 2, base, sum);
@@ -635,15 +727,27 @@ __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_co
   }
   __syncthreads();
   const float* raw = p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group) * p.raw_tokens;
-  for (int t = blockIdx.x * kThreads + tid; t < s.n; t += gridDim.x * kThreads) {
-    const int64_t id =
-        load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(t >> p.bs_log2) * p.bts1);
-    if (id < 0 || id >= p.num_blocks) continue;
-    float* dst = p.scores + id * p.scs0 + h * p.scs1 + (t & ((1 << p.bs_log2) - 1)) * p.scs2;
-    const float old = t == s.n - 1 ? 0.f : *dst;
-    float w = 0.f;
-    for (int g = 0; g < p.group; ++g) w += ex2(raw[g * p.raw_tokens + t] - lse[g]);
-    *dst = old + w;
+  for (int at = t; at < s.n; at += 4 * gridDim.x * kThreads) {
+    if (at != t) look(at);
+    if (!slot) continue;
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int g = 0; g < p.group; ++g) {
+      const float4 x = *reinterpret_cast<const float4*>(raw + g * p.raw_tokens + at);
+      const float y = lse[g];
+      w[0] += ex2(x.x - y);
+      w[1] += ex2(x.y - y);
+      w[2] += ex2(x.z - y);
+      w[3] += ex2(x.w - y);
+    }
+    const float before[4] = {old.x, old.y, old.z, old.w};
+    if (p.score_vec && at + 4 < s.n) {
+      *reinterpret_cast<float4*>(slot) = make_float4(old.x + w[0], old.y + w[1], old.z + w[2], old.w + w[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at + i < s.n) slot[i * p.scs2] = at + i == s.n - 1 ? w[i] : before[i] + w[i];
+    }
   }
 }
 
@@ -651,7 +755,8 @@ struct StreamPlan {
   int m16;         // 16-row tiles per CTA: 1 or 2
   int row_blocks;  // grid extent
   int splits;
-  int min_tiles;   // tiles a split holds at least
+  int chunk;       // tiles of a split (at least, in a cluster)
+  int ctas;        // grid, without clusters
   bool cluster;    // the splits are a cluster
   bool prompt;     // many rows: prompt_attention, where it takes the layout
   int64_t max_query;
@@ -677,9 +782,9 @@ int check(const fd_stream_attention_args* a, bool scored) {
     if (a->window < 1 || a->sinks < 0 || a->max_query_len < 1 || a->num_tokens < 0)
       return FD_ERR_INVALID_ARGUMENT;
     if (!a->query_start_loc && a->num_tokens != a->num_seqs) return FD_ERR_INVALID_ARGUMENT;
-    if (static_cast<int64_t>(a->num_tokens) * (a->num_q_heads / a->num_kv_heads) > 0x3fffffff)
-      return FD_ERR_UNSUPPORTED;
   }
+  const int64_t tokens = scored ? a->num_seqs : std::max(a->num_tokens, a->num_seqs);
+  if (tokens * a->num_q_heads > 0x3fffffff) return FD_ERR_UNSUPPORTED;
   return FD_OK;
 }
 
@@ -714,33 +819,37 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   }
   const int64_t tiles = (seen + kTok - 1) / kTok;
   const int64_t units = static_cast<int64_t>(a->num_seqs) * a->num_kv_heads * pl.row_blocks;
-  // Few units: one wave of CTAs, two to an SM.  Many: splits of 1024 tokens at
-  // most, so that the long sequences of a ragged batch do not finish alone; a
-  // short one then has fewer splits (of 512 tokens), and the rest of its CTAs
-  // end at once.
-  const int64_t wave = units > 0 ? std::max<int64_t>(2 * sms / units, 1) : 1;
-  const int64_t even = (tiles + 63) / 64;
-  int64_t splits = std::min<int64_t>(std::min<int64_t>(std::max(wave, even), tiles / (2 * kWarps)), kMaxSplits);
-  splits = std::max<int64_t>(splits, 1);
-  if (splits > wave && units * splits < 16 * sms)  // a few waves: whole ones
-    splits = std::max<int64_t>(units * splits / (2 * sms) * (2 * sms) / units, 1);
-  pl.min_tiles = splits > wave ? 32 : 2 * kWarps;
+  // Two CTAs fit an SM.  Splits of 1024 tokens or a few more, so that whole
+  // waves of them make up a uniform batch; fewer tokens when that is less than
+  // one wave, down to two tiles per warp.
+  const int64_t slots = 2 * sms, work = units * tiles;
+  const int64_t waves = std::max<int64_t>(work / (64 * slots), 1);
+  pl.chunk = static_cast<int>(std::max<int64_t>((work + waves * slots - 1) / (waves * slots), 2 * kWarps));
+  int64_t splits = std::max<int64_t>((tiles + pl.chunk - 1) / pl.chunk, 1);
+  // items are counted in 32 bits
+  const int64_t most = (tokens * group / per + a->num_seqs) * a->num_kv_heads + units;
+  if (most * splits > 0x7fffffff) {
+    splits = 1;
+    pl.chunk = static_cast<int>(tiles);
+  }
   const size_t q_rows = static_cast<size_t>(tokens) * a->num_q_heads;
-  // One wave of short splits merges inside clusters: no second launch.
-  const int64_t in_cluster = std::min<int64_t>(splits, kMaxCluster);
   pl.raw_tokens = (cap + kTok - 1) / kTok * kTok;
-  if (splits > 1 && splits <= wave) {
-    const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, pl.min_tiles) * kTok;
+  // One wave of short splits merges inside clusters: no second launch.
+  if (splits > 1 && waves == 1) {
+    const int64_t in_cluster = std::min<int64_t>(splits, kMaxCluster);
+    const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, 2 * kWarps) * kTok;
     const size_t raw = scored ? static_cast<size_t>(run) * std::min<int64_t>(rows, per) * sizeof(float) : 0;
     if (run <= 512 && raw <= kRawBytes) {
       pl.cluster = true;
       pl.raw_smem = raw;
       pl.raw_tokens = run;
-      splits = in_cluster;
+      pl.splits = static_cast<int>(in_cluster);
+      pl.chunk = 2 * kWarps;
+      return pl;
     }
   }
   pl.splits = static_cast<int>(splits);
-  if (pl.cluster) return pl;
+  pl.ctas = static_cast<int>(std::min<int64_t>(units * splits, slots));
   if (pl.splits > 1) pl.acc_bytes = q_rows * pl.splits * a->head_dim * sizeof(float);
   if (pl.splits > 1 || scored) pl.ml_bytes = (q_rows * pl.splits * 2 * sizeof(float) + 15) & ~size_t(15);
   if (scored) pl.raw_bytes = q_rows * static_cast<size_t>(pl.raw_tokens) * sizeof(float);
@@ -750,12 +859,13 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
 template <typename T, int D, int kM>
 int launch_split(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
   auto kern = stream_split_kernel<T, D, kM>;
-  const size_t smem = split_smem_bytes<D, kM>() + pl.raw_smem;
+  const size_t list = !pl.cluster && p.num_seqs <= kMaxListed ? (p.num_seqs + 1) * sizeof(int) : 0;
+  const size_t smem = split_smem_bytes<D, kM>() + pl.raw_smem + list;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(split_smem_bytes<D, kM>() + kRawBytes));
   if (e != cudaSuccess) return cuda_status(e);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(pl.splits, p.hkv * pl.row_blocks, p.num_seqs);
+  cfg.gridDim = pl.cluster ? dim3(pl.splits, p.hkv * pl.row_blocks, p.num_seqs) : dim3(std::max(pl.ctas, 1));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -775,7 +885,7 @@ template <typename T, int D>
 int launch_typed(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
   const int rc = pl.m16 == 1 ? launch_split<T, D, 1>(p, pl, stream) : launch_split<T, D, 2>(p, pl, stream);
   if (rc != FD_OK || pl.cluster || (pl.splits == 1 && !p.scores)) return rc;
-  // rows to merge, or four CTA widths of tokens a block
+  // rows to merge, or four tokens a thread
   const int64_t rows = static_cast<int64_t>(pl.row_blocks) * 16 * pl.m16;
   const int64_t tokens = p.scores ? (pl.raw_tokens + 4 * kThreads - 1) / (4 * kThreads) : 0;
   const int64_t most = std::max<int64_t>(1, (1 << 20) / (static_cast<int64_t>(p.hkv) * p.num_seqs));
@@ -838,7 +948,10 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   }
   p.row_blocks = pl.row_blocks;
   p.splits = pl.splits;
-  p.min_tiles = pl.min_tiles;
+  p.chunk = pl.chunk;
+  p.rows_cta = 16 * pl.m16;
+  p.score_vec = scored && reinterpret_cast<uintptr_t>(a->scores) % 16 == 0 && a->scores_stride[0] % 4 == 0 &&
+                a->scores_stride[1] % 4 == 0 && a->scores_stride[2] == 1;
   p.cluster = pl.cluster;
   auto aligned = [](const void* base, const int64_t* st) {
     return reinterpret_cast<uintptr_t>(base) % 16 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 &&
