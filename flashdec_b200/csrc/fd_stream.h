@@ -38,6 +38,7 @@ struct StreamParams {
   int cluster;      // the splits of a unit form a cluster
   int chunk;        // tiles of a split (at least, in a cluster)
   int rows_cta;     // rows of a row block
+  int rows_most;    // rows of a cluster's row block
   int score_vec;    // four scores of a page: one 16-byte access
   float* part_acc;  // [row = token * hq + head][split][D]
   float* part_ml;   // [row][split][2]: max (base 2), sum

@@ -21,22 +21,38 @@ constexpr int kStages = 3;  // tiles in flight per warp
 constexpr int kMaxCluster = 8;      // splits that merge inside a cluster
 constexpr int kMaxListed = 1024;    // sequences whose items a CTA counts
 constexpr int kRawBytes = 10 << 10; // scores a CTA may keep in shared memory
+constexpr int kClusterRun = 512;    // tokens of a split of a cluster, at most
+constexpr int kOldMost = kClusterRun / kThreads;
 
 template <int D>
 constexpr size_t ring_bytes() {
   return static_cast<size_t>(kWarps) * kStages * 2 * kTok * D * 2;
 }
-// ring (later the merge buffer: kWarps x rows x (D + 2) floats), q, the CTA's
-// (max, sum) and the cluster's weights per row
+// ring (later the merge buffer: kWarps x rows x (D + 2) floats) and q (one row
+// tile: in the ring, see below); per row the offset of its output, the warps'
+// and the cluster's weights, lse
 template <int D, int kM>
 constexpr size_t split_smem_bytes() {
-  return ring_bytes<D>() + static_cast<size_t>(kM) * 16 * (D * 2 + 2 * sizeof(float) + (kMaxCluster + 1) * sizeof(float));
+  return ring_bytes<D>() + static_cast<size_t>(kM) * 16 *
+                               ((kM > 1 ? D * 2 : 0) + sizeof(int64_t) + (kWarps + kMaxCluster + 2) * sizeof(float));
+}
+// what the other CTAs of a cluster send: (max, sum) per row and their part of
+// this CTA's share of the rows' elements
+constexpr size_t receive_bytes(int splits, int rows, int D) {
+  return sizeof(float) * (static_cast<size_t>(splits) * rows * 2 + static_cast<size_t>(rows) * D + 4 * splits);
 }
 
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float x;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
-  return x;
+// Elements d .. d + 3 of a row.
+template <typename T>
+__device__ __forceinline__ void store4(T* row, int d, int64_t stride, int vec, float4 x) {
+  if (vec) {
+    *reinterpret_cast<uint2*>(row + d) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+  } else {
+    row[d * stride] = from_f32<T>(x.x);
+    row[(d + 1) * stride] = from_f32<T>(x.y);
+    row[(d + 2) * stride] = from_f32<T>(x.z);
+    row[(d + 3) * stride] = from_f32<T>(x.w);
+  }
 }
 
 // Splits of a sequence's row blocks (of `rows` rows each): what the last block
@@ -80,11 +96,14 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   constexpr int kChunks = D / 8;
   constexpr uint32_t kTileBytes = kTok * D * 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* qsm = smem + ring_bytes<D>();
-  float* cml = reinterpret_cast<float*>(qsm + kRows * D * 2);  // [row][2] this CTA's max and sum
-  float* weight = cml + kRows * 2;                             // [split][row] of the cluster
-  float* lse = weight + kMaxCluster * kRows;                   // [row]
-  float* raw = reinterpret_cast<float*>(smem + split_smem_bytes<D, kM>());  // [row][raw_tokens]
+  int64_t* row_out = reinterpret_cast<int64_t*>(smem + ring_bytes<D>() + (kM > 1 ? kRows * D * 2 : 0));  // [row] element offset in out
+  float* warp_weight = reinterpret_cast<float*>(row_out + kRows);      // [warp][row]
+  float* weight = warp_weight + kWarps * kRows;                        // [split][row] of the cluster
+  float* lse = weight + kMaxCluster * kRows;                           // [row]
+  float* inv_sum = lse + kRows;                                        // [row], one split
+  float* got_ml = reinterpret_cast<float*>(smem + split_smem_bytes<D, kM>());  // [split][rows_most][2]
+  float* got = got_ml + 2 * p.splits * p.rows_most;                            // [split][share]
+  float* raw = p.cluster ? got_ml + receive_bytes(p.splits, p.rows_most, D) / sizeof(float) : got_ml;  // [row][raw_tokens]
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -282,6 +301,11 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       for (int i = 0; i < kStages; ++i) fetch(t0 + warp + i * kWarps, blk[i], pos[i]);
 #pragma unroll
       for (int i = 0; i < kStages - 1; ++i) issue(t0 + warp + i * kWarps, blk[i], pos[i]);
+      // One row tile of q goes to the stage of warp 0's third tile, which is not
+      // loaded before every warp has its fragments: two CTAs then fit an SM
+      // with what a cluster's CTA receives.
+      uint8_t* const qsm = kM > 1 ? smem + ring_bytes<D>()
+                                  : smem + ((t0 / kWarps + kStages - 1) % kStages) * (2 * kTileBytes);
       for (int e = tid; e < kRows * kChunks; e += kThreads) {
         const int r = e / kChunks, c = e % kChunks;
         uint4 x = make_uint4(0u, 0u, 0u, 0u);
@@ -322,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       if constexpr (kM == 1) {
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) load_q(0, kk, qf[kk]);
+        __syncthreads();
       }
       const float slack = 8.f / scale;
 
@@ -519,7 +544,25 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       // ---- merge the warps: (max, sum, acc) per row through the ring ----
       cp_async_wait<0>();
       __syncthreads();
-      float* acc = reinterpret_cast<float*>(smem);  // [warp][row][D], then the CTA's in [0]
+      // with scores: the slots and old values of this thread's tokens, on their way
+      float* slot[kOldMost];
+      float old[kOldMost];
+      if (p.cluster && p.scores) {
+#pragma unroll
+        for (int i = 0; i < kOldMost; ++i) {
+          const int tok = t0 * kTok + tid + i * kThreads;
+          slot[i] = nullptr;
+          old[i] = 0.f;
+          if (tok < min(t1 * kTok, s.n)) {
+            const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(tok >> p.bs_log2) * p.bts1);
+            if (id >= 0 && id < p.num_blocks) {
+              slot[i] = p.scores + id * p.scs0 + h * p.scs1 + (tok & mask) * p.scs2;
+              if (tok < s.n - 1) old[i] = *slot[i];
+            }
+          }
+        }
+      }
+      float* acc = reinterpret_cast<float*>(smem);  // [warp][row][D]
       float* ml = acc + kWarps * kRows * D;         // [warp][row][2]
       static_assert(sizeof(float) * kWarps * kRows * (D + 2) <= ring_bytes<D>(), "merge buffer");
 #pragma unroll
@@ -542,92 +585,116 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
           }
         }
       __syncthreads();
-      for (int e = tid; e < rows * D; e += kThreads) {
-        const int r = e / D, d = e - r * D;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[(w * kRows + r) * 2]);
-        const float base = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f, x = 0.f;
+      if (tid < rows) {  // the row's weights, and where it goes
+        const int r = tid;
+        float pm[kWarps], mx = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float f = ex2(ml[(w * kRows + r) * 2] - base);
+          pm[w] = ml[(w * kRows + r) * 2];
+          mx = fmaxf(mx, pm[w]);
+        }
+        const float base = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = ex2(pm[w] - base);
+          warp_weight[w * kRows + r] = f;
           sum += f * ml[(w * kRows + r) * 2 + 1];
-          x += f * acc[(w * kRows + r) * D + d];
         }
         const int qt = (row0 + r) / p.group;
         const int head = h * p.group + (row0 + r) - qt * p.group;
         const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
-        if (splits == 1) {
-          static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] =
-              from_f32<T>(sum == 0.f ? 0.f : x / sum);
-        } else if (p.cluster) {
-          acc[e] = x;  // warp 0's place of the same element
-        } else {
-          p.part_acc[(row * p.splits + split) * D + d] = x;
+        row_out[r] = p.cluster || splits == 1 ? (s.q0 + qt) * p.os0 + head * p.os1 : (row * p.splits + split) * D;
+        inv_sum[r] = sum == 0.f ? 0.f : 1.f / sum;
+        if (p.cluster) {
+          for (int i = 0; i < splits; ++i)
+            st_cluster_v2(map_to_rank(smem_u32(got_ml + (split * p.rows_most + r) * 2), i), mx, sum);
+        } else if (p.part_ml) {
+          *reinterpret_cast<float2*>(p.part_ml + (row * p.splits + split) * 2) = make_float2(mx, sum);
         }
-        if (d == 0) {
-          if (p.cluster) {
-            cml[2 * r] = mx;
-            cml[2 * r + 1] = sum;
-          } else if (p.part_ml) {
-            p.part_ml[(row * p.splits + split) * 2] = mx;
-            p.part_ml[(row * p.splits + split) * 2 + 1] = sum;
-          }
+      }
+      __syncthreads();
+      // elements 4 e4 .. + 3 of the rows' [rows][D]; rank i of a cluster gets [share i, + share)
+      const int share = p.cluster ? (rows * (D / 4) + splits - 1) / splits * 4 : 0;
+      T* const out = static_cast<T*>(p.out);
+      for (int e4 = tid; e4 < rows * (D / 4); e4 += kThreads) {
+        const int r = e4 / (D / 4), d = 4 * (e4 % (D / 4));
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = warp_weight[w * kRows + r];
+          const float4 y = *reinterpret_cast<const float4*>(acc + (w * kRows + r) * D + d);
+          x.x += f * y.x;
+          x.y += f * y.y;
+          x.z += f * y.z;
+          x.w += f * y.w;
+        }
+        if (p.cluster) {
+          const int to = 4 * e4 / share;
+          st_cluster_v4(map_to_rank(smem_u32(got + split * share + 4 * e4 - to * share), to), x.x, x.y, x.z, x.w);
+        } else if (splits == 1) {
+          const float f = inv_sum[r];
+          store4<T>(out + row_out[r], d, p.os2, p.out_vec, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
+        } else {
+          *reinterpret_cast<float4*>(p.part_acc + row_out[r] + d) = x;
         }
       }
       if (p.cluster) {
-        // ---- merge the cluster's splits: every CTA its share of the elements ----
+        // ---- merge the cluster's splits: everything needed has been sent here ----
         cluster_arrive();
         cluster_wait();
-        for (int r = tid; r < rows; r += kThreads) {
+        if (tid < rows) {
+          const int r = tid;
           float pm[kMaxCluster], pl[kMaxCluster], mx = -INFINITY;
 #pragma unroll
           for (int i = 0; i < kMaxCluster; ++i) {
-            pm[i] = -INFINITY;
-            pl[i] = 0.f;
-            if (i < p.splits) {
-              const uint32_t at = map_to_rank(smem_u32(&cml[2 * r]), i);
-              pm[i] = ld_cluster(at);
-              pl[i] = ld_cluster(at + 4);
-            }
+            pm[i] = i < splits ? got_ml[(i * p.rows_most + r) * 2] : -INFINITY;
+            pl[i] = i < splits ? got_ml[(i * p.rows_most + r) * 2 + 1] : 0.f;
             mx = fmaxf(mx, pm[i]);
           }
           const float base = mx == -INFINITY ? 0.f : mx;
           float sum = 0.f;
 #pragma unroll
-          for (int i = 0; i < kMaxCluster; ++i) sum += ex2(pm[i] - base) * pl[i];
+          for (int i = 0; i < kMaxCluster; ++i) {
+            pm[i] = ex2(pm[i] - base);
+            sum += pm[i] * pl[i];
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-          for (int i = 0; i < kMaxCluster; ++i)
-            weight[i * kRows + r] = sum == 0.f ? 0.f : ex2(pm[i] - base) / sum;
+          for (int i = 0; i < kMaxCluster; ++i) weight[i * kRows + r] = pm[i] * inv;
           lse[r] = sum == 0.f ? INFINITY : base + log2f(sum);
         }
         __syncthreads();
-        for (int e = split * kThreads + tid; e < rows * D; e += p.splits * kThreads) {
-          const int r = e / D, d = e - r * D;
-          float x = 0.f;
+        for (int e4 = tid; e4 < share / 4; e4 += kThreads) {
+          const int e = split * share + 4 * e4;
+          if (e >= rows * D) break;
+          const int r = e / D, d = e % D;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int i = 0; i < kMaxCluster; ++i)
-            if (i < p.splits) x += weight[i * kRows + r] * ld_cluster(map_to_rank(smem_u32(acc + e), i));
-          const int qt = (row0 + r) / p.group;
-          const int head = h * p.group + (row0 + r) - qt * p.group;
-          static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + d * p.os2] = from_f32<T>(x);
+          for (int i = 0; i < kMaxCluster; ++i) {
+            if (i >= splits) break;
+            const float f = weight[i * kRows + r];
+            const float4 y = *reinterpret_cast<const float4*>(got + i * share + 4 * e4);
+            x.x += f * y.x;
+            x.y += f * y.y;
+            x.z += f * y.z;
+            x.w += f * y.w;
+          }
+          store4<T>(out + row_out[r], d, p.os2, p.out_vec, x);
         }
         if (p.scores) {
-          for (int i = tid; i < (t1 - t0) * kTok; i += kThreads) {
-            const int tok = t0 * kTok + i;
-            if (tok >= s.n) break;
-            const int64_t id = load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(tok >> p.bs_log2) * p.bts1);
-            if (id < 0 || id >= p.num_blocks) continue;
-            float* dst = p.scores + id * p.scs0 + h * p.scs1 + (tok & mask) * p.scs2;
-            const float old = tok == s.n - 1 ? 0.f : *dst;
+#pragma unroll
+          for (int i = 0; i < kOldMost; ++i) {
+            if (!slot[i]) continue;
             float w = 0.f;
-            for (int r = 0; r < rows; ++r) w += ex2(raw[r * p.raw_tokens + i] - lse[r]);
-            *dst = old + w;
+            for (int r = 0; r < rows; ++r) w += ex2(raw[r * p.raw_tokens + tid + i * kThreads] - lse[r]);
+            *slot[i] = old[i] + w;
           }
         }
-        cluster_arrive();  // the others have read this CTA's partials
-        cluster_wait();
+        if ((rb + p.row_blocks) * kRows < rows_all) {  // the next rows are sent to the same place
+          cluster_arrive();
+          cluster_wait();
+        }
       }
       __syncthreads();
     }
@@ -761,7 +828,8 @@ struct StreamPlan {
   bool prompt;     // many rows: prompt_attention, where it takes the layout
   int64_t max_query;
   int64_t raw_tokens;
-  size_t raw_smem;
+  int rows_most;     // of a cluster's item
+  size_t more_smem;  // of a cluster's CTA
   size_t acc_bytes, ml_bytes, raw_bytes;
   size_t bytes() const { return acc_bytes + ml_bytes + raw_bytes; }
 };
@@ -839,11 +907,12 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
     const int64_t in_cluster = std::min<int64_t>(splits, kMaxCluster);
     const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, 2 * kWarps) * kTok;
     const size_t raw = scored ? static_cast<size_t>(run) * std::min<int64_t>(rows, per) * sizeof(float) : 0;
-    if (run <= 512 && raw <= kRawBytes) {
+    if (run <= kClusterRun && raw <= kRawBytes) {
+      pl.rows_most = static_cast<int>(std::min<int64_t>(rows, per));
       pl.cluster = true;
-      pl.raw_smem = raw;
-      pl.raw_tokens = run;
       pl.splits = static_cast<int>(in_cluster);
+      pl.more_smem = raw + receive_bytes(pl.splits, pl.rows_most, a->head_dim);
+      pl.raw_tokens = run;
       pl.chunk = 2 * kWarps;
       return pl;
     }
@@ -860,9 +929,10 @@ template <typename T, int D, int kM>
 int launch_split(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
   auto kern = stream_split_kernel<T, D, kM>;
   const size_t list = !pl.cluster && p.num_seqs <= kMaxListed ? (p.num_seqs + 1) * sizeof(int) : 0;
-  const size_t smem = split_smem_bytes<D, kM>() + pl.raw_smem + list;
+  const size_t smem = split_smem_bytes<D, kM>() + pl.more_smem + list;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(split_smem_bytes<D, kM>() + kRawBytes));
+                                       static_cast<int>(split_smem_bytes<D, kM>() + kRawBytes +
+                                                        receive_bytes(kMaxCluster, 16 * kM, D)));
   if (e != cudaSuccess) return cuda_status(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = pl.cluster ? dim3(pl.splits, p.hkv * pl.row_blocks, p.num_seqs) : dim3(std::max(pl.ctas, 1));
@@ -948,6 +1018,7 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   }
   p.row_blocks = pl.row_blocks;
   p.splits = pl.splits;
+  p.rows_most = pl.rows_most;
   p.chunk = pl.chunk;
   p.rows_cta = 16 * pl.m16;
   p.score_vec = scored && reinterpret_cast<uintptr_t>(a->scores) % 16 == 0 && a->scores_stride[0] % 4 == 0 &&
