@@ -31,18 +31,21 @@ struct StreamParams {
   int bs_log2, num_blocks, max_blocks;
   int window, sinks;
   int row_blocks;  // of the longest queries announced
-  int splits;      // most splits of a (sequence, KV head, row block)
+  int splits;      // CTAs of a unit (cluster or grid)
   int vec;         // rows of K and V are 16-byte aligned and contiguous
   int q_vec, out_vec;  // the same of q and of out
   float scale_log2;
-  int cluster;      // the splits of a unit form a cluster
-  int chunk;        // tiles of a split (at least, in a cluster)
+  int mode;         // how the split kernel's CTAs share the units (fd_stream_attention.cu)
+  int first_seq;    // of this launch's num_seqs
   int rows_cta;     // rows of a row block
   int rows_most;    // rows of a cluster's row block
   int score_vec;    // four scores of a page: one 16-byte access
-  float* part_acc;  // [row = token * hq + head][split][D]
-  float* part_ml;   // [row][split][2]: max (base 2), sum
-  float* raw;       // [row][raw_tokens]: scaled scores (base 2)
+  int3* share_unit; // [share] where it starts: {sequence of the launch, row block x KV head, tile}
+  int* shares;      // number of shares
+  float* part_acc;  // [place][row of the unit][D]
+  float* part_ml;   // [place][row of the unit][2]: max (base 2), sum
+  float* row_lse;   // [query x head]: max + log2(sum), with scores
+  float* raw;       // [query x head][raw_tokens]: scaled scores (base 2)
   int64_t raw_tokens;  // row length of raw, or of its copy in shared memory
   int* status;
 };

@@ -14,12 +14,16 @@
 namespace fd {
 namespace {
 
+constexpr int kCluster = 0, kGrid = 1, kShares = 2;  // StreamParams::mode, see stream_split_kernel
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTok = 16;    // tokens per warp tile
 constexpr int kStages = 3;  // tiles in flight per warp
 constexpr int kMaxCluster = 8;      // splits that merge inside a cluster
-constexpr int kMaxListed = 1024;    // sequences whose items a CTA counts
+constexpr int kMaxListed = 512;     // sequences of a launch
+constexpr int kMinShare = 16;       // tiles of a CTA's share, at least
+constexpr int kGridRun = 64;        // tiles of a CTA in kGrid, at most
+constexpr int kSnap = 4;            // tiles: a cut this near to a unit's end moves there
 constexpr int kRawBytes = 10 << 10; // scores a CTA may keep in shared memory
 constexpr int kClusterRun = 512;    // tokens of a split of a cluster, at most
 constexpr int kOldMost = kClusterRun / kThreads;
@@ -55,14 +59,27 @@ __device__ __forceinline__ void store4(T* row, int d, int64_t stride, int vec, f
   }
 }
 
-// Splits of a sequence's row blocks (of `rows` rows each): what the last block
-// sees, in runs of p.chunk tiles.
-__device__ __forceinline__ int splits_of(const StreamParams& p, const StreamSeq& s, int rows) {
+// Tiles that a unit (row block x KV head) of a sequence is counted with: what
+// its last row block sees, one at least (rows that see nothing are written too).
+__device__ __forceinline__ int unit_tiles(const StreamParams& p, const StreamSeq& s, int rows) {
   const int all = s.qlen * p.group;
-  if (all == 0 || p.splits == 1) return 1;
+  if (all == 0) return 1;
   const StreamRange rg(s, (all - 1) / rows * rows, all, p.group, p.window, p.sinks, p.bs_log2);
-  const int tiles = ((rg.pages << p.bs_log2) + kTok - 1) / kTok;
-  return min(max((tiles + p.chunk - 1) / p.chunk, 1), p.splits);
+  return max(((rg.pages << p.bs_log2) + kTok - 1) / kTok, 1);
+}
+
+// Last i of [0, n) with first[i] <= x (first[0] <= x).
+__device__ __forceinline__ int last_up_to(const int64_t* first, int n, int64_t x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) {
+      lo = mid;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
 }
 
 // Byte offset of 16-byte chunk `c` of row `r` in a [rows][D] 16-bit tile: the
@@ -74,21 +91,24 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 }
 
 // ---------------------------------------------------------------------------
-// One item: rows [16 kM rb, +16 kM) of a (sequence, KV head) against one split
-// of the pages they see.  Row r is head r % group of query r / group, so K and
-// V are read once for the whole group.  Tile i of 16 tokens goes to warp i % 4;
-// each warp keeps three tiles in flight with cp.async and its own maximum and
-// sum (base 2, the maximum followed only when a score passes it by 2^8), and
-// the four merge at the end.
+// Works on segments: rows [16 kM rb, +16 kM) of a (sequence, KV head), a unit,
+// against a run of the pages they see.  Row r is head r % group of query r /
+// group, so K and V are read once for the whole group.  Tile i of 16 tokens
+// goes to warp i % 4; each warp keeps three tiles in flight with cp.async and
+// its own maximum and sum (base 2, the maximum followed only when a score
+// passes it by 2^8), and the four merge at the end.
 //
-// p.cluster: the CTAs of a cluster have one item each, the splits of a (rows,
-// KV head), and merge through distributed shared memory.  Else a CTA takes
-// every gridDim.x-th item of the batch: a sequence has as many splits as its
-// length asks for, which the CTA counts from the lengths, so a ragged batch
-// launches no idle CTA (as a grid over the longest sequence's splits, 24
-// sequences of 512 to 32768 tokens took 147 us, a third of it for CTAs that
-// found nothing to do).  Splits then leave fp32 partials to
-// stream_finish_kernel.
+// p.mode:
+//   kCluster  a unit per cluster, a segment per CTA; they merge through
+//             distributed shared memory.
+//   kGrid     a unit per p.splits CTAs, a segment each, as partials.
+//   kShares   the tiles of all units in a row are cut into equal shares, one
+//             per CTA, whatever the lengths: a CTA has a few segments, of which
+//             only the first and the last can be parts of a unit and leave
+//             partials.  As many shares as CTAs fit: with four times as many,
+//             one long sequence of 131071 tokens took 117 us (97), 64 sequences
+//             of up to 4100 visible tokens 180 us (162).
+// Partials go to stream_finish_kernel.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int kM>
 __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_constant__ StreamParams p) {
@@ -103,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   float* inv_sum = lse + kRows;                                        // [row], one split
   float* got_ml = reinterpret_cast<float*>(smem + split_smem_bytes<D, kM>());  // [split][rows_most][2]
   float* got = got_ml + 2 * p.splits * p.rows_most;                            // [split][share]
-  float* raw = p.cluster ? got_ml + receive_bytes(p.splits, p.rows_most, D) / sizeof(float) : got_ml;  // [row][raw_tokens]
+  float* raw = p.mode == kCluster ? got_ml + receive_bytes(p.splits, p.rows_most, D) / sizeof(float) : got_ml;  // [row][raw_tokens]
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -112,7 +132,8 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   const int mi = lane >> 3;
   const int r8 = lane & 7;
   const int mask = (1 << p.bs_log2) - 1;
-  int* const upto = reinterpret_cast<int*>(raw);  // [num_seqs + 1] items before a sequence's
+  int64_t* const upto = reinterpret_cast<int64_t*>(got_ml);  // [num_seqs + 1] tiles before a sequence's (no cluster)
+  int* const unit = reinterpret_cast<int*>(upto + p.num_seqs + 1);  // [num_seqs] tiles of its units
   // a scale of 0 (uniform weights) stays above it: -inf * 0 is NaN; its sign goes to q
   const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
@@ -127,22 +148,29 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   const uint32_t k_off = tile_chunk<D>((mi >> 1) * 8 + r8, mi & 1);
   const uint32_t v_off = tile_chunk<D>((mi & 1) * 8 + r8, mi >> 1);
 
-  const bool listed = !p.cluster && p.num_seqs <= kMaxListed;
-  int items = p.cluster ? 1 : p.num_seqs * p.row_blocks * p.splits * p.hkv;
-  if (listed) {
-    // items of every sequence, then their running sum (warp 0)
+  const bool cluster = p.mode == kCluster, grid = p.mode == kGrid;
+  int b = 0, h = 0, rb = 0;
+  StreamSeq s;
+  int64_t at = 0, end = 0;  // this CTA's share of the tiles
+  if (cluster || grid) {
+    b = p.first_seq + blockIdx.z;
+    h = blockIdx.y % p.hkv;
+    rb = blockIdx.y / p.hkv;
+    s = sequence_of(p, b);
+  } else {
     for (int i = tid; i < p.num_seqs; i += kThreads) {
-      const StreamSeq s = sequence_of(p, i);
-      upto[i + 1] = ((s.qlen * p.group + kRows - 1) / kRows) * splits_of(p, s, kRows) * p.hkv;
+      s = sequence_of(p, p.first_seq + i);
+      unit[i] = unit_tiles(p, s, kRows);
+      upto[i + 1] = static_cast<int64_t>((s.qlen * p.group + kRows - 1) / kRows) * p.hkv * unit[i];
     }
     __syncthreads();
     if (warp == 0) {
-      int sum = 0;
+      int64_t sum = 0;
       for (int i = 0; i < p.num_seqs; i += 32) {
-        int x = i + lane < p.num_seqs ? upto[i + lane + 1] : 0;
+        int64_t x = i + lane < p.num_seqs ? upto[i + lane + 1] : 0;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, x, d);
+          const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
           if (lane >= d) x += y;
         }
         if (i + lane < p.num_seqs) upto[i + lane + 1] = sum + x;
@@ -151,59 +179,65 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       if (lane == 0) upto[0] = 0;
     }
     __syncthreads();
-    items = upto[p.num_seqs];
+    const int64_t total = upto[p.num_seqs];
+    const int shares = static_cast<int>(min(max(total / kMinShare, int64_t(1)), static_cast<int64_t>(gridDim.x)));
+    if (static_cast<int>(blockIdx.x) >= shares || total == 0) {
+      if (blockIdx.x == 0 && tid == 0) *p.shares = 0;
+      return;
+    }
+    auto cut = [&](int i) -> int64_t {
+      int64_t x = total * i / shares;
+      if (i == 0 || i == shares) return x;
+      const int q = last_up_to(upto, p.num_seqs, x);
+      const int past = static_cast<int>((x - upto[q]) % unit[q]);
+      if (past < kSnap) return x - past;
+      return unit[q] - past < kSnap ? x + unit[q] - past : x;
+    };
+    at = cut(blockIdx.x);
+    end = cut(blockIdx.x + 1);
+    if (tid == 0) {  // where the share starts
+      const int i = last_up_to(upto, p.num_seqs, at);
+      const int64_t past = at - upto[i];
+      const int u = static_cast<int>(past / unit[i]);
+      p.share_unit[blockIdx.x] = make_int3(i, u, static_cast<int>(past - static_cast<int64_t>(u) * unit[i]));
+    }
+    if (blockIdx.x == 0 && tid == 0) *p.shares = shares;
   }
-  for (int item = p.cluster ? 0 : blockIdx.x; item < items; item += gridDim.x) {
-    // ---- the item: heads of a split are neighbours, then splits, row blocks, sequences ----
-    int b, h, split, rb0, splits = p.splits;
-    StreamSeq s;
-    if (p.cluster) {
-      b = blockIdx.z;
-      h = blockIdx.y % p.hkv;
-      split = blockIdx.x;
-      rb0 = blockIdx.y / p.hkv;
+  for (;;) {
+    int from = 0, to = 0, all = 0;  // the segment: tiles [from, to) of the unit's `all`
+    if (!cluster && !grid) {
+      if (at >= end) break;
+      const int i = last_up_to(upto, p.num_seqs, at);
+      b = p.first_seq + i;
+      all = unit[i];
+      const int64_t past = at - upto[i];
+      const int u = static_cast<int>(past / all);
+      from = static_cast<int>(past - static_cast<int64_t>(u) * all);
+      to = static_cast<int>(min(static_cast<int64_t>(all), from + (end - at)));
+      at += to - from;
+      h = u % p.hkv;
+      rb = u / p.hkv;
       s = sequence_of(p, b);
-    } else {
-      int x = item, of;
-      if (listed) {
-        int lo = 0, hi = p.num_seqs;  // upto[lo] <= item < upto[hi]
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (upto[mid] <= item) {
-            lo = mid;
-          } else {
-            hi = mid;
-          }
-        }
-        b = lo;
-        x -= upto[lo];
-        s = sequence_of(p, b);
-        of = splits = splits_of(p, s, kRows);
-      } else {
-        const int per_seq = p.row_blocks * p.splits * p.hkv;
-        b = x / per_seq;
-        x -= b * per_seq;
-        s = sequence_of(p, b);
-        splits = splits_of(p, s, kRows);
-        of = p.splits;
-      }
-      h = x % p.hkv;
-      x /= p.hkv;
-      split = x % of;
-      rb0 = x / of;
     }
     const int rows_all = s.qlen * p.group;
-    if (split >= splits) continue;
-    // more than one row block where the grid or the list of items is sized by
-    // the longest queries announced, and they are longer
-    for (int rb = rb0; rb * kRows < rows_all; rb += listed ? rows_all : p.row_blocks) {
+    if (rb * kRows >= rows_all) break;  // of a cluster or grid: the last row block is done
+    // (grid: row blocks past the announced ones have no place for partials)
+    const bool whole_unit = cluster ? false : grid ? rb >= p.row_blocks || p.splits == 1 : from == 0 && to == all;
+    if (grid && whole_unit && blockIdx.x > 0) break;
+    const int part = grid ? (blockIdx.z * gridDim.y + blockIdx.y) * p.splits + blockIdx.x
+                          : 2 * blockIdx.x + (from == 0 ? 1 : 0);  // place of a partial
+    {
       const int row0 = rb * kRows;
       const int rows = min(kRows, rows_all - row0);
       const StreamRange rg(s, row0, row0 + rows, p.group, p.window, p.sinks, p.bs_log2);
       const int tiles = ((rg.pages << p.bs_log2) + kTok - 1) / kTok;
-      const int per = max((tiles + splits - 1) / splits, p.cluster ? p.chunk : 1);
-      const int t0 = min(split * per, tiles);
-      const int t1 = min(t0 + per, tiles);
+      const int splits = p.splits, split = blockIdx.x;  // of a cluster
+      const int per = max((tiles + splits - 1) / splits, 2 * kWarps);
+      int t0 = min(from, tiles), t1 = to == all ? tiles : min(to, tiles);
+      if (cluster || (grid && !whole_unit)) {
+        t0 = min(split * per, tiles);
+        t1 = min(t0 + per, tiles);
+      }
 
       // lanes 0 and 1 hold the (at most two) pages of a tile: {block, position of its first token}
       auto fetch = [&](int t, int& blk, int& pos) {
@@ -413,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
               }
         }
         if (p.scores) {  // one query: row = head of the group; list place = position
-          float* dst = p.cluster ? raw + (t - t0) * kTok
+          float* dst = cluster ? raw + (t - t0) * kTok
                                  : p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens + t * kTok;
 #pragma unroll
           for (int a = 0; a < kM; ++a)
@@ -547,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       // with scores: the slots and old values of this thread's tokens, on their way
       float* slot[kOldMost];
       float old[kOldMost];
-      if (p.cluster && p.scores) {
+      if (cluster && p.scores) {
 #pragma unroll
         for (int i = 0; i < kOldMost; ++i) {
           const int tok = t0 * kTok + tid + i * kThreads;
@@ -604,18 +638,20 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
         const int qt = (row0 + r) / p.group;
         const int head = h * p.group + (row0 + r) - qt * p.group;
         const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
-        row_out[r] = p.cluster || splits == 1 ? (s.q0 + qt) * p.os0 + head * p.os1 : (row * p.splits + split) * D;
+        row_out[r] = cluster || whole_unit ? (s.q0 + qt) * p.os0 + head * p.os1 : (static_cast<int64_t>(part) * kRows + r) * D;
         inv_sum[r] = sum == 0.f ? 0.f : 1.f / sum;
-        if (p.cluster) {
+        if (cluster) {
           for (int i = 0; i < splits; ++i)
             st_cluster_v2(map_to_rank(smem_u32(got_ml + (split * p.rows_most + r) * 2), i), mx, sum);
-        } else if (p.part_ml) {
-          *reinterpret_cast<float2*>(p.part_ml + (row * p.splits + split) * 2) = make_float2(mx, sum);
+        } else if (!whole_unit) {
+          *reinterpret_cast<float2*>(p.part_ml + (static_cast<int64_t>(part) * kRows + r) * 2) = make_float2(mx, sum);
+        } else if (p.scores) {
+          p.row_lse[row] = sum == 0.f ? INFINITY : base + log2f(sum);
         }
       }
       __syncthreads();
       // elements 4 e4 .. + 3 of the rows' [rows][D]; rank i of a cluster gets [share i, + share)
-      const int share = p.cluster ? (rows * (D / 4) + splits - 1) / splits * 4 : 0;
+      const int share = cluster ? (rows * (D / 4) + splits - 1) / splits * 4 : 0;
       T* const out = static_cast<T*>(p.out);
       for (int e4 = tid; e4 < rows * (D / 4); e4 += kThreads) {
         const int r = e4 / (D / 4), d = 4 * (e4 % (D / 4));
@@ -629,17 +665,17 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
           x.z += f * y.z;
           x.w += f * y.w;
         }
-        if (p.cluster) {
+        if (cluster) {
           const int to = 4 * e4 / share;
           st_cluster_v4(map_to_rank(smem_u32(got + split * share + 4 * e4 - to * share), to), x.x, x.y, x.z, x.w);
-        } else if (splits == 1) {
+        } else if (whole_unit) {
           const float f = inv_sum[r];
           store4<T>(out + row_out[r], d, p.os2, p.out_vec, make_float4(x.x * f, x.y * f, x.z * f, x.w * f));
         } else {
           *reinterpret_cast<float4*>(p.part_acc + row_out[r] + d) = x;
         }
       }
-      if (p.cluster) {
+      if (cluster) {
         // ---- merge the cluster's splits: everything needed has been sent here ----
         cluster_arrive();
         cluster_wait();
@@ -696,108 +732,132 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
           cluster_wait();
         }
       }
+      if (cluster || grid) rb += p.row_blocks;
       __syncthreads();
     }
   }
 }
 
-// What remains after the split kernel: rows whose splits are partials are
-// merged (one row a CTA at a time), and with scores every token gets the sum
-// over the group of exp2(raw - lse), four neighbouring tokens a thread.
+// What remains after the split kernel where units were cut: one row a CTA, the
+// segments of the row's unit shared out over the warps.  kGrid: CTA (unit, row);
+// kShares: CTA (c, row) has the unit that share c + 1 is the first to start
+// inside, if it is.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_constant__ StreamParams p) {
-  extern __shared__ float lse[];  // [group], with scores
+__global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_constant__ StreamParams p) {
   __shared__ float part[kWarps][D];
+  __shared__ float part_ml[kWarps][2];
   constexpr int kPer = D / 32;
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  int64_t place0, place1, step;  // places of the first and the second segment, and from there on
+  int count, b, h, r = blockIdx.y;
+  if (p.mode == kGrid) {
+    const int units = p.row_blocks * p.hkv, u = blockIdx.x;
+    b = u / units;
+    h = u % p.hkv;
+    place0 = (static_cast<int64_t>(u) * p.splits) * p.rows_cta + r;
+    step = p.rows_cta;
+    place1 = place0 + step;
+    count = p.splits;
+    r += u % units / p.hkv * p.rows_cta;
+  } else {
+    const int c = blockIdx.x + 1, shares = *p.shares;
+    if (c >= shares) return;
+    const int3 at = p.share_unit[c], before = p.share_unit[c - 1];
+    if (at.z == 0 || (before.x == at.x && before.y == at.y && before.z > 0)) return;  // no cut, or not its first
+    count = 1;  // the share before c, and those from c on that start inside the unit
+    for (int i = c;; i += 32) {
+      int3 x = make_int3(-1, 0, 0);
+      if (i + lane < shares) x = p.share_unit[i + lane];
+      const uint32_t same = __ballot_sync(0xffffffffu, x.x == at.x && x.y == at.y && x.z > 0);
+      count += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+      if (same != 0xffffffffu) break;
+    }
+    b = at.x;
+    h = at.y % p.hkv;
+    place0 = static_cast<int64_t>(2 * (c - 1) + 1) * p.rows_cta + r;
+    place1 = static_cast<int64_t>(2 * c) * p.rows_cta + r;
+    step = 2 * p.rows_cta;
+    r += at.y / p.hkv * p.rows_cta;
+  }
+  const StreamSeq s = sequence_of(p, p.first_seq + b);
+  if (r >= s.qlen * p.group) return;
+  // warp w: segments w, w + 4, ... with its own maximum; lane: D / 32 dims
+  float m = -INFINITY, l = 0.f, x[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) x[j] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < count; i += kWarps) {
+    const int64_t at = i == 0 ? place0 : place1 + (i - 1) * step;
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * at);
+    float y[kPer];
+    if constexpr (kPer == 4) {
+      *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(p.part_acc + at * D + lane * 4);
+    } else {
+      *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(p.part_acc + at * D + lane * 2);
+    }
+    const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;
+    const float f = ex2(m - base), w = ex2(ml.x - base);
+    m = mn;
+    l = l * f + ml.y * w;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = x[j] * f + y[j] * w;
+  }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) part[warp][lane * kPer + j] = x[j];
+  if (lane == 0) {
+    part_ml[warp][0] = m;
+    part_ml[warp][1] = l;
+  }
+  __syncthreads();
+  if (tid >= D) return;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, part_ml[w][0]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f, y = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const float f = ex2(part_ml[w][0] - base);
+    sum += f * part_ml[w][1];
+    y += f * part[w][tid];
+  }
+  const int qt = r / p.group, head = h * p.group + r - qt * p.group;
+  static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + tid * p.os2] = from_f32<T>(sum == 0.f ? 0.f : y / sum);
+  if (p.scores && tid == 0)
+    p.row_lse[static_cast<int64_t>(s.q0 + qt) * p.hq + head] = sum == 0.f ? INFINITY : base + log2f(sum);
+}
+
+// Every token's score gets the sum over the group of exp2(raw - lse), four
+// neighbouring tokens a thread.
+__global__ void __launch_bounds__(kThreads) stream_scores_kernel(const __grid_constant__ StreamParams p) {
+  extern __shared__ float lse[];  // [group]
+  const int tid = threadIdx.x;
   const int h = blockIdx.y;
-  const int b = blockIdx.z;
+  const int b = p.first_seq + blockIdx.z;
   pdl_wait();
   pdl_launch_dependents();
   const StreamSeq s = sequence_of(p, b);
-  const int rows_all = s.qlen * p.group;
-  const int splits = splits_of(p, s, p.rows_cta);
-  const int t = 4 * (blockIdx.x * kThreads + tid);  // this thread's first tokens
-  const bool scores_here = p.scores && 4 * static_cast<int>(blockIdx.x) * kThreads < s.n;
-  if (!scores_here && (splits == 1 || static_cast<int>(blockIdx.x) >= rows_all)) return;
-  // the tokens' slot and old scores, on their way while the rows are merged
-  float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
-  float* slot = nullptr;
-  auto look = [&](int at) {  // four tokens: one page
-    slot = nullptr;
-    if (at >= s.n) return;
-    const int64_t id =
-        load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(at >> p.bs_log2) * p.bts1);
-    if (id < 0 || id >= p.num_blocks) return;
-    slot = p.scores + id * p.scs0 + h * p.scs1 + (at & ((1 << p.bs_log2) - 1)) * p.scs2;
-    if (p.score_vec) {
-      old = *reinterpret_cast<const float4*>(slot);
-    } else {
-      old = make_float4(slot[0], slot[p.scs2], slot[2 * p.scs2], slot[3 * p.scs2]);
-    }
-  };
-  if (scores_here) look(t);
-  // max and sum over the splits of a row, by one warp
-  auto row_stats = [&](const float* ml, float& base, float& sum) {
-    float mx = -INFINITY;
-    for (int i = lane; i < splits; i += 32) mx = fmaxf(mx, ml[2 * i]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-    base = mx == -INFINITY ? 0.f : mx;
-    sum = 0.f;
-    for (int i = lane; i < splits; i += 32) sum += ex2(ml[2 * i] - base) * ml[2 * i + 1];
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  };
-  if (splits > 1) {
-    for (int r = blockIdx.x; r < rows_all; r += gridDim.x) {
-      const int qt = r / p.group;
-      const int head = h * p.group + r - qt * p.group;
-      const int64_t row = static_cast<int64_t>(s.q0 + qt) * p.hq + head;
-      const float* ml = p.part_ml + row * p.splits * 2;
-      float base, sum;
-      row_stats(ml, base, sum);
-      // warp w takes splits w, w + 4, ...; lane: D / 32 neighbouring dims
-      float x[kPer];
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) x[j] = 0.f;
-#pragma unroll 8
-      for (int i = warp; i < splits; i += kWarps) {
-        const float w = ex2(ml[2 * i] - base);
-        float y[kPer];
-        if constexpr (kPer == 4) {
-          *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(p.part_acc + (row * p.splits + i) * D + lane * 4);
-        } else {
-          *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(p.part_acc + (row * p.splits + i) * D + lane * 2);
-        }
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) x[j] += w * y[j];
-      }
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) part[warp][lane * kPer + j] = x[j];
-      __syncthreads();
-      if (tid < D) {
-        const float y = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-        static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + tid * p.os2] =
-            from_f32<T>(sum == 0.f ? 0.f : y / sum);
-      }
-      __syncthreads();
-    }
-  }
-  if (!scores_here) return;
-  for (int g = warp; g < p.group; g += kWarps) {
-    float base, sum;
-    row_stats(p.part_ml + (static_cast<int64_t>(b) * p.hq + h * p.group + g) * p.splits * 2, base, sum);
-    if (lane == 0) lse[g] = sum == 0.f ? INFINITY : base + log2f(sum);
-  }
+  if (4 * static_cast<int>(blockIdx.x) * kThreads >= s.n) return;
+  const int64_t row0 = static_cast<int64_t>(b) * p.hq + h * p.group;
+  for (int g = tid; g < p.group; g += kThreads) lse[g] = p.row_lse[row0 + g];
   __syncthreads();
-  const float* raw = p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group) * p.raw_tokens;
-  for (int at = t; at < s.n; at += 4 * gridDim.x * kThreads) {
-    if (at != t) look(at);
-    if (!slot) continue;
-    float w[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* raw = p.raw + row0 * p.raw_tokens;
+  for (int at = 4 * (blockIdx.x * kThreads + tid); at < s.n; at += 4 * gridDim.x * kThreads) {
+    const int64_t id =  // four tokens: one page
+        load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(at >> p.bs_log2) * p.bts1);
+    if (id < 0 || id >= p.num_blocks) continue;
+    float* slot = p.scores + id * p.scs0 + h * p.scs1 + (at & ((1 << p.bs_log2) - 1)) * p.scs2;
+    float old[4], w[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.score_vec) {
+      *reinterpret_cast<float4*>(old) = *reinterpret_cast<const float4*>(slot);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) old[i] = slot[i * p.scs2];
+    }
 #pragma unroll 4
     for (int g = 0; g < p.group; ++g) {
       const float4 x = *reinterpret_cast<const float4*>(raw + g * p.raw_tokens + at);
@@ -807,31 +867,32 @@ __global__ void __launch_bounds__(kThreads) stream_finish_kernel(const __grid_co
       w[2] += ex2(x.z - y);
       w[3] += ex2(x.w - y);
     }
-    const float before[4] = {old.x, old.y, old.z, old.w};
     if (p.score_vec && at + 4 < s.n) {
-      *reinterpret_cast<float4*>(slot) = make_float4(old.x + w[0], old.y + w[1], old.z + w[2], old.w + w[3]);
+      *reinterpret_cast<float4*>(slot) = make_float4(old[0] + w[0], old[1] + w[1], old[2] + w[2], old[3] + w[3]);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (at + i < s.n) slot[i * p.scs2] = at + i == s.n - 1 ? w[i] : before[i] + w[i];
+        if (at + i < s.n) slot[i * p.scs2] = at + i == s.n - 1 ? w[i] : old[i] + w[i];
     }
   }
 }
 
 struct StreamPlan {
   int m16;         // 16-row tiles per CTA: 1 or 2
-  int row_blocks;  // grid extent
-  int splits;
-  int chunk;       // tiles of a split (at least, in a cluster)
-  int ctas;        // grid, without clusters
-  bool cluster;    // the splits are a cluster
+  int row_blocks;  // of the longest queries announced
   bool prompt;     // many rows: prompt_attention, where it takes the layout
   int64_t max_query;
   int64_t raw_tokens;
-  int rows_most;     // of a cluster's item
+  int mode;          // kCluster, kGrid or kShares
+  int splits;        // CTAs of a unit, of a cluster or grid
+  int rows_most;     // of a cluster's unit
   size_t more_smem;  // of a cluster's CTA
-  size_t acc_bytes, ml_bytes, raw_bytes;
-  size_t bytes() const { return acc_bytes + ml_bytes + raw_bytes; }
+  int ctas;          // grid of kShares
+  int parts;         // places of partials
+  // scratch: (kShares) where each CTA's share starts, and their number; the
+  // partials; for scores the rows' lse and raw scores
+  size_t meta_bytes, ml_bytes, acc_bytes, lse_bytes, raw_bytes;
+  size_t bytes() const { return meta_bytes + ml_bytes + acc_bytes + lse_bytes + raw_bytes; }
 };
 
 int check(const fd_stream_attention_args* a, bool scored) {
@@ -887,55 +948,61 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   }
   const int64_t tiles = (seen + kTok - 1) / kTok;
   const int64_t units = static_cast<int64_t>(a->num_seqs) * a->num_kv_heads * pl.row_blocks;
-  // Two CTAs fit an SM.  Splits of 1024 tokens or a few more, so that whole
-  // waves of them make up a uniform batch; fewer tokens when that is less than
-  // one wave, down to two tiles per warp.
-  const int64_t slots = 2 * sms, work = units * tiles;
-  const int64_t waves = std::max<int64_t>(work / (64 * slots), 1);
-  pl.chunk = static_cast<int>(std::max<int64_t>((work + waves * slots - 1) / (waves * slots), 2 * kWarps));
-  int64_t splits = std::max<int64_t>((tiles + pl.chunk - 1) / pl.chunk, 1);
-  // items are counted in 32 bits
-  const int64_t most = (tokens * group / per + a->num_seqs) * a->num_kv_heads + units;
-  if (most * splits > 0x7fffffff) {
-    splits = 1;
-    pl.chunk = static_cast<int>(tiles);
-  }
+  const int64_t slots = 2 * sms;  // two CTAs fit an SM
   const size_t q_rows = static_cast<size_t>(tokens) * a->num_q_heads;
   pl.raw_tokens = (cap + kTok - 1) / kTok * kTok;
-  // One wave of short splits merges inside clusters: no second launch.
-  if (splits > 1 && waves == 1) {
-    const int64_t in_cluster = std::min<int64_t>(splits, kMaxCluster);
+  const int64_t row_most = std::min<int64_t>(rows, per);
+  // Few units with short runs: the splits of each merge inside a cluster, with
+  // no second launch (one token of one sequence: 8.9 us, 14.4 with partials).
+  const int64_t in_cluster = std::min<int64_t>(tiles / (2 * kWarps), kMaxCluster);
+  if (in_cluster > 1 && units * in_cluster <= slots) {
     const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, 2 * kWarps) * kTok;
-    const size_t raw = scored ? static_cast<size_t>(run) * std::min<int64_t>(rows, per) * sizeof(float) : 0;
+    const size_t raw = scored ? static_cast<size_t>(run) * row_most * sizeof(float) : 0;
     if (run <= kClusterRun && raw <= kRawBytes) {
-      pl.rows_most = static_cast<int>(std::min<int64_t>(rows, per));
-      pl.cluster = true;
+      pl.mode = kCluster;
+      pl.rows_most = static_cast<int>(row_most);
       pl.splits = static_cast<int>(in_cluster);
       pl.more_smem = raw + receive_bytes(pl.splits, pl.rows_most, a->head_dim);
       pl.raw_tokens = run;
-      pl.chunk = 2 * kWarps;
       return pl;
     }
   }
-  pl.splits = static_cast<int>(splits);
-  pl.ctas = static_cast<int>(std::min<int64_t>(units * splits, slots));
-  if (pl.splits > 1) pl.acc_bytes = q_rows * pl.splits * a->head_dim * sizeof(float);
-  if (pl.splits > 1 || scored) pl.ml_bytes = (q_rows * pl.splits * 2 * sizeof(float) + 15) & ~size_t(15);
-  if (scored) pl.raw_bytes = q_rows * static_cast<size_t>(pl.raw_tokens) * sizeof(float);
+  // A wave of CTAs with kGridRun tiles each at most: a grid of equal splits, which
+  // needs no count of the batch's tiles first (24 sequences' drafts: 22 us,
+  // 31 as shares).  More: shares.
+  const int64_t even = std::max<int64_t>(std::min<int64_t>(slots / units, tiles / (2 * kWarps)), 1);
+  if (units <= slots && (tiles + even - 1) / even <= kGridRun && a->num_seqs <= kMaxListed) {
+    pl.mode = kGrid;
+    pl.splits = static_cast<int>(even);
+    pl.parts = static_cast<int>(units * even);
+  } else {
+    pl.mode = kShares;
+    pl.splits = 1;
+    pl.ctas = static_cast<int>(std::min<int64_t>(std::max<int64_t>(units * tiles / kMinShare, 1), slots));
+    pl.parts = 2 * pl.ctas;
+  }
+  auto padded = [](size_t x) { return (x + 15) & ~size_t(15); };
+  pl.meta_bytes = padded(pl.ctas * sizeof(int3) + sizeof(int));
+  pl.ml_bytes = static_cast<size_t>(pl.parts) * per * 2 * sizeof(float);
+  pl.acc_bytes = static_cast<size_t>(pl.parts) * per * a->head_dim * sizeof(float);
+  if (scored) {
+    pl.lse_bytes = padded(q_rows * sizeof(float));
+    pl.raw_bytes = q_rows * static_cast<size_t>(pl.raw_tokens) * sizeof(float);
+  }
   return pl;
 }
 
 template <typename T, int D, int kM>
 int launch_split(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
   auto kern = stream_split_kernel<T, D, kM>;
-  const size_t list = !pl.cluster && p.num_seqs <= kMaxListed ? (p.num_seqs + 1) * sizeof(int) : 0;
+  const size_t list = pl.mode == kShares ? (p.num_seqs + 1) * (sizeof(int64_t) + sizeof(int)) : 0;
   const size_t smem = split_smem_bytes<D, kM>() + pl.more_smem + list;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        static_cast<int>(split_smem_bytes<D, kM>() + kRawBytes +
                                                         receive_bytes(kMaxCluster, 16 * kM, D)));
   if (e != cudaSuccess) return cuda_status(e);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = pl.cluster ? dim3(pl.splits, p.hkv * pl.row_blocks, p.num_seqs) : dim3(std::max(pl.ctas, 1));
+  cfg.gridDim = pl.mode == kShares ? dim3(pl.ctas) : dim3(pl.splits, p.hkv * pl.row_blocks, p.num_seqs);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -947,22 +1014,27 @@ int launch_split(const StreamParams& p, const StreamPlan& pl, cudaStream_t strea
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = pl.cluster ? 2 : 1;
+  cfg.numAttrs = pl.mode == kCluster ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
 template <typename T, int D>
 int launch_typed(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
-  const int rc = pl.m16 == 1 ? launch_split<T, D, 1>(p, pl, stream) : launch_split<T, D, 2>(p, pl, stream);
-  if (rc != FD_OK || pl.cluster || (pl.splits == 1 && !p.scores)) return rc;
-  // rows to merge, or four tokens a thread
-  const int64_t rows = static_cast<int64_t>(pl.row_blocks) * 16 * pl.m16;
-  const int64_t tokens = p.scores ? (pl.raw_tokens + 4 * kThreads - 1) / (4 * kThreads) : 0;
+  int rc = pl.m16 == 1 ? launch_split<T, D, 1>(p, pl, stream) : launch_split<T, D, 2>(p, pl, stream);
+  if (rc != FD_OK || pl.mode == kCluster) return rc;
+  const int64_t merges = pl.mode == kGrid ? (pl.splits == 1 ? 0 : static_cast<int64_t>(p.num_seqs) * p.hkv * pl.row_blocks)
+                                          : pl.ctas - 1;
+  // rows of a row block: all of them where queries may be longer than announced
+  const int64_t rows = p.qstart ? p.rows_cta : std::min<int64_t>(p.rows_cta, p.group);
+  if (merges > 0)
+    rc = cuda_status(launch_pdl(stream_merge_kernel<T, D>, dim3(static_cast<unsigned>(merges), static_cast<unsigned>(rows)),
+                                dim3(kThreads), 0, stream, p));
+  if (rc != FD_OK || !p.scores) return rc;
+  // a CTA goes over 2 x 512 tokens where there are so many
+  const int64_t chunks = (pl.raw_tokens + 8 * kThreads - 1) / (8 * kThreads);
   const int64_t most = std::max<int64_t>(1, (1 << 20) / (static_cast<int64_t>(p.hkv) * p.num_seqs));
-  const int blocks = static_cast<int>(std::min(std::max(pl.splits > 1 ? std::min<int64_t>(rows, pl.max_query * p.group) : 1, tokens), most));
-  const size_t smem = p.scores ? static_cast<size_t>(p.group) * sizeof(float) : 0;
-  return cuda_status(launch_pdl(stream_finish_kernel<T, D>, dim3(blocks, p.hkv, p.num_seqs), dim3(kThreads),
-                                smem, stream, p));
+  return cuda_status(launch_pdl(stream_scores_kernel, dim3(static_cast<unsigned>(std::min(chunks, most)), p.hkv, p.num_seqs),
+                                dim3(kThreads), static_cast<size_t>(p.group) * sizeof(float), stream, p));
 }
 
 int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
@@ -1019,11 +1091,10 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   p.row_blocks = pl.row_blocks;
   p.splits = pl.splits;
   p.rows_most = pl.rows_most;
-  p.chunk = pl.chunk;
   p.rows_cta = 16 * pl.m16;
   p.score_vec = scored && reinterpret_cast<uintptr_t>(a->scores) % 16 == 0 && a->scores_stride[0] % 4 == 0 &&
                 a->scores_stride[1] % 4 == 0 && a->scores_stride[2] == 1;
-  p.cluster = pl.cluster;
+  p.mode = pl.mode;
   auto aligned = [](const void* base, const int64_t* st) {
     return reinterpret_cast<uintptr_t>(base) % 16 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 &&
            st[2] % 8 == 0 && st[3] == 1;
@@ -1036,17 +1107,31 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   p.out_vec = aligned3(a->out, a->out_stride);
   p.scale_log2 = a->sm_scale * 1.4426950408889634f;
   char* at = static_cast<char*>(a->scratch);
-  if (pl.acc_bytes) p.part_acc = reinterpret_cast<float*>(at);
-  if (pl.ml_bytes) p.part_ml = reinterpret_cast<float*>(at + pl.acc_bytes);
-  if (pl.raw_bytes) p.raw = reinterpret_cast<float*>(at + pl.acc_bytes + pl.ml_bytes);
+  if (pl.mode != kCluster) {
+    p.share_unit = reinterpret_cast<int3*>(at);
+    p.shares = reinterpret_cast<int*>(p.share_unit + pl.ctas);
+    at += pl.meta_bytes;
+    p.part_ml = reinterpret_cast<float*>(at);
+    at += pl.ml_bytes;
+    p.part_acc = reinterpret_cast<float*>(at);
+    at += pl.acc_bytes;
+    p.row_lse = reinterpret_cast<float*>(at);
+    p.raw = reinterpret_cast<float*>(at + pl.lse_bytes);
+  }
   p.raw_tokens = pl.raw_tokens;
   p.status = status;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   const bool bf16 = a->dtype == FD_DTYPE_BF16;
   if (pl.prompt && prompt_attention(p, bf16, a->head_dim, pl.max_query, stream, &rc)) return rc;
-  if (a->head_dim == 128)
-    return bf16 ? launch_typed<__nv_bfloat16, 128>(p, pl, stream) : launch_typed<__half, 128>(p, pl, stream);
-  return bf16 ? launch_typed<__nv_bfloat16, 64>(p, pl, stream) : launch_typed<__half, 64>(p, pl, stream);
+  for (p.first_seq = 0; rc == FD_OK && p.first_seq < a->num_seqs; p.first_seq += kMaxListed) {
+    p.num_seqs = std::min(a->num_seqs - p.first_seq, kMaxListed);
+    if (a->head_dim == 128) {
+      rc = bf16 ? launch_typed<__nv_bfloat16, 128>(p, pl, stream) : launch_typed<__half, 128>(p, pl, stream);
+    } else {
+      rc = bf16 ? launch_typed<__nv_bfloat16, 64>(p, pl, stream) : launch_typed<__half, 64>(p, pl, stream);
+    }
+  }
+  return rc;
 }
 
 int workspace(const fd_stream_attention_args* a, bool scored, size_t* bytes) {

@@ -288,6 +288,33 @@ def test_window_graph_replay():
         close(out, exact, size, "bf16", 260)
 
 
+def test_window_and_scored_batches_of_many_sequences():
+    """More sequences than one launch takes, with empty and long ones among them."""
+    import flashdec_b200 as fd
+
+    rng = np.random.default_rng(21)
+    lens = rng.integers(0, 24, 1100)
+    lens[[0, 511, 512, 1099]] = [700, 0, 900, 300]
+    lens = lens.tolist()
+    c = Cache(20, lens, hkv=1, d=64, bs=8)
+    q, qn = c.queries(len(lens), 2)
+    out = fd.window_attention(q, c.k, c.v, c.table, c.seq, window=200, sinks=2)
+    exact, size = ref.window_attention_ref(qn, c.k_np, c.v_np, c.table_np, lens, 200, 2)
+    close(out, exact, size, "bf16", 202)
+    scores = torch.ones((c.pool, 1, 8), device="cuda")
+    out = fd.scored_decode(q, c.k, c.v, scores, c.table, c.seq)
+    exact, size, want = ref.scored_decode_ref(qn, c.k_np, c.v_np, np.ones((c.pool, 1, 8)), c.table_np, lens)
+    close(out, exact, size, "bf16", 900)
+    assert (np.abs(scores.double().cpu().numpy() - want) <= 1e-4 * np.abs(want - 1) + 1e-6).all()
+    qs = [min(n, 3) for n in lens]
+    q, qn = c.queries(sum(qs), 2)
+    st = starts_of(qs)
+    out = fd.window_attention(q, c.k, c.v, c.table, c.seq, window=30, sinks=1, max_query_len=3,
+                              query_start_loc=torch.from_numpy(st).cuda())
+    exact, size = ref.window_attention_ref(qn, c.k_np, c.v_np, c.table_np, lens, 30, 1, st)
+    close(out, exact, size, "bf16", 31)
+
+
 SCORED = [
     ("bf16", 16, 2, 128, 32, "planes", [1, 2, 33, 300]),
     ("fp16", 32, 8, 128, 16, "nhd", [700, 5, 0, 64]),
