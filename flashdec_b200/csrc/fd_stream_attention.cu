@@ -383,6 +383,20 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
         __syncthreads();
       }
       const float slack = 8.f / scale;
+      // where this thread's rows' scores go (one query: row = head of the group,
+      // list place = position), less the tile's
+      float* raw_row[kM][2];
+#pragma unroll
+      for (int a = 0; a < kM; ++a)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 16 * a + 8 * e + g8;
+          raw_row[a][e] = nullptr;
+          if (p.scores && r < rows)
+            raw_row[a][e] = (cluster ? raw - t0 * kTok
+                                     : p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens) +
+                            r * p.raw_tokens + 2 * t4;
+        }
 
       for (int t = t0 + warp; t < t1; t += kWarps) {
         issue(t + (kStages - 1) * kWarps, blk[kStages - 1], pos[kStages - 1]);
@@ -446,21 +460,16 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
                 vis |= (on ? 1u : 0u) << (a * 8 + j * 4 + e);
               }
         }
-        if (p.scores) {  // one query: row = head of the group; list place = position
-          float* dst = cluster ? raw + (t - t0) * kTok
-                                 : p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens + t * kTok;
+        if (p.scores) {  // rows are padded to whole tiles
 #pragma unroll
           for (int a = 0; a < kM; ++a)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = 16 * a + 8 * e + g8;
-              if (r < rows) {  // rows are padded to whole tiles
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                  *reinterpret_cast<float2*>(dst + r * p.raw_tokens + 8 * j + 2 * t4) =
-                      make_float2(sc[a][j][2 * e] * scale, sc[a][j][2 * e + 1] * scale);
+            for (int e = 0; e < 2; ++e)
+              if (raw_row[a][e]) {
+                float* dst = raw_row[a][e] + static_cast<int64_t>(t) * kTok;
+                *reinterpret_cast<float2*>(dst) = make_float2(sc[a][0][2 * e] * scale, sc[a][0][2 * e + 1] * scale);
+                *reinterpret_cast<float2*>(dst + 8) = make_float2(sc[a][1][2 * e] * scale, sc[a][1][2 * e + 1] * scale);
               }
-            }
         }
         // ---- follow the maximum when it is 2^8 behind ----
         bool behind = false;
