@@ -31,6 +31,7 @@ struct EvictParams {
   int vec;        // rows are 16-byte aligned and contiguous
   int score_vec;  // four scores of a page: one 16-byte load
   int* status;
+  int device;  // host side only
 };
 
 __device__ __forceinline__ int length_of(const EvictParams& p, int b) {
@@ -66,6 +67,7 @@ constexpr int kMaxCluster = 8;
 // cluster, and 48 clusters of 8 took 51 us on that traffic.
 constexpr int kDigits = 4;
 constexpr int kSelectWords = 512 + 256 + 256 + 128;  // their histograms
+constexpr int kKeyMost = 48 * 1024;  // keys a CTA keeps
 constexpr int kShort = 2048;  // keys of the second digit's bin that are listed for the last two
 
 // Exclusive sum over the threads of a CTA (in thread order) and the total.
@@ -422,8 +424,8 @@ template <int D>
 int copy(const EvictParams& p, int num_seqs, int sms, cudaStream_t stream) {
   constexpr size_t smem = copy_smem_bytes<D>();
   constexpr int kPerSm = D == 128 ? 4 : 8;  // rings that fill an SM's shared memory
-  cudaError_t e = cudaFuncSetAttribute(evict_copy_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(done, reinterpret_cast<const void*>(evict_copy_kernel<D>), smem, p.device);
   if (e != cudaSuccess) return cuda_status(e);
   const int64_t most = std::min<int64_t>(
       std::min<int64_t>(p.budget, static_cast<int64_t>(p.max_new_blocks) << p.bs_log2),
@@ -443,10 +445,11 @@ int select(const EvictParams& p, int num_seqs, cudaStream_t stream) {
   while (ranks < kMaxCluster && cap > 4096 * ranks) ranks *= 2;
   const int64_t run = ((cap + ranks - 1) / ranks + 7) & ~int64_t(7);
   // past this the keys are read again for every digit
-  const int key_cap = run <= 48 * 1024 ? static_cast<int>(run) : 0;
+  const int key_cap = run <= kKeyMost ? static_cast<int>(run) : 0;
   const size_t smem = sizeof(int) * (kSelectWords + kShort + static_cast<size_t>(key_cap));
-  cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(done, reinterpret_cast<const void*>(evict_select_kernel),
+                                   sizeof(int) * (kSelectWords + kShort + kKeyMost), p.device);
   if (e != cudaSuccess) return cuda_status(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, p.hkv, num_seqs);
@@ -525,6 +528,7 @@ extern "C" int fd_evict_tokens(const fd_evict_tokens_args* a, void* cuda_stream)
   };
   p.vec = aligned(a->k_cache, a->k_stride) && aligned(a->v_cache, a->v_stride);
   p.status = status;
+  p.device = dev->device;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   p.score_vec = reinterpret_cast<uintptr_t>(a->scores) % 16 == 0 && a->scores_stride[0] % 4 == 0 &&
                 a->scores_stride[1] % 4 == 0 && a->scores_stride[2] == 1;

@@ -3,6 +3,7 @@
 // no link-time libcuda dependency) and a small cache of encoded maps.
 #pragma once
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda.h>
@@ -107,6 +108,18 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// Let `kern` use `bytes` of dynamic shared memory on `device`: asked of the
+// runtime once per kernel and device (`done` is the kernel's own, one bit a
+// device; the call costs about as much as a launch).
+inline cudaError_t allow_smem(std::atomic<uint64_t>& done, const void* kern, size_t bytes, int device) {
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 // The same launch without the attribute, for a kernel whose stream

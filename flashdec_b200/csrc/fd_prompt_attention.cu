@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       uint8_t* const area = smem + g * SM::kOperand + (c >> 3) * SM::kHalf;
       if (p.q_vec) {
         const T* const src = static_cast<const T*>(p.q) + c * 8;
-#pragma unroll 1
+#pragma unroll 4
         for (int r = r0; r < 128; r += kRowStep) {
           const bool in = grow0 + r < rows_all;
           cp_async16(smem_u32(area) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (in ? row_at(r, p.qs0, p.qs1) : 0),
@@ -682,7 +682,8 @@ int launch(const StreamParams& p, const CUtensorMap& mk, const CUtensorMap& mv, 
            const int (&vp)[4], dim3 grid, cudaStream_t stream) {
   auto kern = prompt_kernel<T, D>;
   constexpr size_t smem = PromptSmem<D>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(done, reinterpret_cast<const void*>(kern), smem, p.device);
   if (e == cudaSuccess)
     e = launch_pdl(kern, grid, dim3(kPromptThreads), smem, stream, p, mk, mv, make_int4(kp[0], kp[1], kp[2], 0),
                    make_int4(vp[0], vp[1], vp[2], 0));

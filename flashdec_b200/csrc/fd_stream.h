@@ -48,6 +48,7 @@ struct StreamParams {
   float* raw;       // [query x head][raw_tokens]: scaled scores (base 2)
   int64_t raw_tokens;  // row length of raw, or of its copy in shared memory
   int* status;
+  int device;  // host side only
 };
 
 // The sequence's queries: rows [q0, q0 + qlen) of q, tokens [n - qlen, n).

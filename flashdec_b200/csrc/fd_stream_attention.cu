@@ -329,7 +329,20 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
         cp_async_commit();
       };
 
-      // ---- first tiles on their way, then q ----
+      // ---- q on its way, the first tiles on theirs, then q to shared memory ----
+      constexpr int kQ = kRows * kChunks / kThreads;
+      uint4 qx[kQ];
+#pragma unroll
+      for (int i = 0; i < kQ; ++i) {
+        const int e = tid + i * kThreads, r = e / kChunks, c = e % kChunks;
+        qx[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) {
+          const int qt = (row0 + r) / p.group;
+          const int head = h * p.group + (row0 + r) - qt * p.group;
+          const T* src = static_cast<const T*>(p.q) + (s.q0 + qt) * p.qs0 + head * p.qs1 + c * 8 * p.qs2;
+          qx[i] = p.q_vec ? *reinterpret_cast<const uint4*>(src) : gather8(src, p.qs2);
+        }
+      }
       int blk[kStages], pos[kStages];  // pages of this warp's next tiles
 #pragma unroll
       for (int i = 0; i < kStages; ++i) fetch(t0 + warp + i * kWarps, blk[i], pos[i]);
@@ -340,19 +353,11 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       // with what a cluster's CTA receives.
       uint8_t* const qsm = kM > 1 ? smem + ring_bytes<D>()
                                   : smem + ((t0 / kWarps + kStages - 1) % kStages) * (2 * kTileBytes);
-      for (int e = tid; e < kRows * kChunks; e += kThreads) {
-        const int r = e / kChunks, c = e % kChunks;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows) {
-          const int qt = (row0 + r) / p.group;
-          const int head = h * p.group + (row0 + r) - qt * p.group;
-          const T* src = static_cast<const T*>(p.q) + (s.q0 + qt) * p.qs0 + head * p.qs1 + c * 8 * p.qs2;
-          x = p.qs2 == 1 && (reinterpret_cast<uintptr_t>(src) & 15u) == 0
-                  ? *reinterpret_cast<const uint4*>(src)
-                  : gather8(src, p.qs2);
-          x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-        }
-        *reinterpret_cast<uint4*>(qsm + tile_chunk<D>(r, c)) = x;
+#pragma unroll
+      for (int i = 0; i < kQ; ++i) {
+        const int e = tid + i * kThreads;
+        *reinterpret_cast<uint4*>(qsm + tile_chunk<D>(e / kChunks, e % kChunks)) =
+            make_uint4(qx[i].x ^ flip, qx[i].y ^ flip, qx[i].z ^ flip, qx[i].w ^ flip);
       }
       __syncthreads();
 
@@ -1006,9 +1011,10 @@ int launch_split(const StreamParams& p, const StreamPlan& pl, cudaStream_t strea
   auto kern = stream_split_kernel<T, D, kM>;
   const size_t list = pl.mode == kShares ? (p.num_seqs + 1) * (sizeof(int64_t) + sizeof(int)) : 0;
   const size_t smem = split_smem_bytes<D, kM>() + pl.more_smem + list;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(split_smem_bytes<D, kM>() + kRawBytes +
-                                                        receive_bytes(kMaxCluster, 16 * kM, D)));
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e =
+      allow_smem(done, reinterpret_cast<const void*>(kern),
+                 split_smem_bytes<D, kM>() + kRawBytes + receive_bytes(kMaxCluster, 16 * kM, D), p.device);
   if (e != cudaSuccess) return cuda_status(e);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = pl.mode == kShares ? dim3(pl.ctas) : dim3(pl.splits, p.hkv * pl.row_blocks, p.num_seqs);
@@ -1129,6 +1135,7 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   }
   p.raw_tokens = pl.raw_tokens;
   p.status = status;
+  p.device = dev->device;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   const bool bf16 = a->dtype == FD_DTYPE_BF16;
   if (pl.prompt && prompt_attention(p, bf16, a->head_dim, pl.max_query, stream, &rc)) return rc;
