@@ -164,6 +164,33 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
       for (int i = 0; i < 4; ++i) k[i] = score_key(src[i * p.scs2]);
     }
   };
+  // the keys of two places, all look-ups and loads out before the first use
+  auto load8 = [&](int t, int t2, uint32_t(&k)[2][4]) {
+    const int at[2] = {t, t2};
+    int64_t id[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      id[u] = at[u] < t1 ? load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(at[u] >> p.bs_log2) * p.bts1) : 0;
+    float4 x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (at[u] < t1 && id[u] >= 0 && id[u] < p.num_blocks) {
+        const float* src = p.scores + id[u] * p.scs0 + h * p.scs1 + (at[u] & mask) * p.scs2;
+        x[u] = p.score_vec ? *reinterpret_cast<const float4*>(src)
+                           : make_float4(src[0], src[p.scs2], src[2 * p.scs2], src[3 * p.scs2]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool good = id[u] >= 0 && id[u] < p.num_blocks;
+      if (!good && at[u] < t1) atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
+      k[u][0] = good ? score_key(x[u].x) : 0u;
+      k[u][1] = good ? score_key(x[u].y) : 0u;
+      k[u][2] = good ? score_key(x[u].z) : 0u;
+      k[u][3] = good ? score_key(x[u].w) : 0u;
+    }
+  };
   auto four = [&](int t, uint32_t(&k)[4]) {
     if (cached) {
       const uint4 x = *reinterpret_cast<const uint4*>(keys + (t - t0));
@@ -175,18 +202,31 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
       load4(t, k);
     }
   };
+  auto all_sync = [&] {  // the cluster's threads
+    if (ranks == 1) {
+      __syncthreads();
+    } else {
+      cluster_arrive();
+      cluster_wait();
+    }
+  };
   // ---- the (m - sinks - recent)-th greatest key of [mid0, mid1) ----
   int need = m - sinks - recent;
   const bool any_mid = need > 0;
   uint32_t prefix = 0;
-#pragma unroll 2
-  for (int t = t0 + 4 * tid; t < t1; t += 4 * kSelectThreads) {  // keys, and the first digit's counts
-    uint32_t k[4];
-    load4(t, k);
-    if (cached) *reinterpret_cast<uint4*>(keys + (t - t0)) = make_uint4(k[0], k[1], k[2], k[3]);
+#pragma unroll 1
+  for (int t8 = t0 + 4 * tid; t8 < t1; t8 += 8 * kSelectThreads) {  // keys, and the first digit's counts
+    uint32_t k[2][4];
+    load8(t8, t8 + 4 * kSelectThreads, k);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (t + i >= mid0 && t + i < mid1) atomicAdd(&hist[k[i] >> 23], 1);
+    for (int u = 0; u < 2; ++u) {
+      const int t = t8 + 4 * kSelectThreads * u;
+      if (t >= t1) break;
+      if (cached) *reinterpret_cast<uint4*>(keys + (t - t0)) = make_uint4(k[u][0], k[u][1], k[u][2], k[u][3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i >= mid0 && t + i < mid1) atomicAdd(&hist[k[u][i] >> 23], 1);
+    }
   }
   int above = 0;  // of this CTA's keys, those that a thread's bins put above the threshold
   if (any_mid) {
@@ -219,8 +259,7 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
           if ((x >> width) == found) atomicAdd(&mine[x & (bins - 1)], 1);
         }
       }
-      cluster_arrive();
-      cluster_wait();
+      all_sync();
       // thread i: bin bins - 1 - i, counted over the cluster
       int c = 0;
       if (tid < bins) {
@@ -269,8 +308,7 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
   block_exclusive(above, warp_sums, total_above);
   if (tid == 0)  // with the protected tokens of the run
     counts[0] = total_above + max(min(t1, mid0) - t0, 0) + max(t1 - max(t0, mid1), 0);
-  cluster_arrive();
-  cluster_wait();
+  all_sync();
   int base = 0, ties = 0;  // sure keeps and threshold keys before this CTA's run
   for (int r = 0; r < rank; ++r) {
     int x, y;
@@ -302,7 +340,7 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
 constexpr int kCopyWarps = 4;
 constexpr int kCopyThreads = kCopyWarps * 32;
 constexpr int kCopyRows = 8;    // rows of a batch
-constexpr int kCopyStages = 3;  // batches a warp has in flight
+constexpr int kCopyStages = 2;  // batches a warp has in flight
 
 template <int D>
 constexpr size_t copy_smem_bytes() {
@@ -423,7 +461,10 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_c
 template <int D>
 int copy(const EvictParams& p, int num_seqs, int sms, cudaStream_t stream) {
   constexpr size_t smem = copy_smem_bytes<D>();
-  constexpr int kPerSm = D == 128 ? 4 : 8;  // rings that fill an SM's shared memory
+  // Six CTAs fit an SM (their registers); four times as many even out the
+  // SMs (537 MB: 123 us with a third stage and four CTAs an SM, 114 with two
+  // and six, 109 with 24, selection included)
+  constexpr int kPerSm = 24;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(done, reinterpret_cast<const void*>(evict_copy_kernel<D>), smem, p.device);
   if (e != cudaSuccess) return cuda_status(e);
