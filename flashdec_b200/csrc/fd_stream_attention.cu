@@ -517,7 +517,10 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
               for (int i = 0; i < 2; ++i) {
                 float& x = sc[a][j][2 * e + i];
                 x = ex2(fmaf(x, scale, -base));
-                l[a][e] += x;
+                // The sum takes the weights as the product takes them, so that a
+                // row with one great weight is not off by its rounding.  With
+                // scores it is the exact sum: their weights are not rounded.
+                l[a][e] += p.scores ? x : to_f32<T>(from_f32<T>(x));
               }
           }
           pf[a][0] = pack2<T>(sc[a][0][0], sc[a][0][1]);
