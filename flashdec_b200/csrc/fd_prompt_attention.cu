@@ -14,7 +14,7 @@
 namespace fd {
 namespace {
 
-// One CTA: 256 query rows (row = query x head of the group) of a (sequence, KV
+// One item: 256 query rows (row = query x head of the group) of a (sequence, KV
 // head) as two groups of 128, against the list of cache pages they see in
 // tiles of 128 keys.  Per group: S = Q K^T (M 128, N 128) into TMEM, one thread
 // per row takes it from there and writes P = exp2(S - m) back over it in the
@@ -24,6 +24,12 @@ namespace {
 // softmax.  With two S buffers of 64 keys a group never waits for its own
 // products, but a product of N 64 takes nearly as long as one of N 128 (it
 // reads the same Q operand): 428 us on an 8k prompt against 378 at that point.
+//
+// One CTA an SM takes every gridDim.x-th item: while the softmax threads finish
+// one, the K and V tiles and the queries of the next are on their way: 58 us for
+// ragged prompts of 9 tiles an item, against 65 with a CTA for each item (whose
+// start and end were a sixth of its time or more); 314 against 306 us for an 8k
+// prompt of 17 tiles an item, which pays for the longer code instead.
 //
 //   warp 0      TMA producer: K and V tiles alternate through a ring of slots
 //   warp 1      issues the tcgen05.mma (one thread)
@@ -37,6 +43,7 @@ namespace {
 constexpr int kPromptThreads = 384;
 constexpr int kRows = 256;
 constexpr int kKeys = 128;  // of a tile
+constexpr int kMostSeqs = 256;  // of a launch
 
 template <int D>
 struct PromptSmem {
@@ -45,7 +52,9 @@ struct PromptSmem {
   static constexpr uint32_t kOperand = (D / 64) * kHalf;   // a Q group or a K or V tile
   static constexpr uint32_t kRing = 2 * kOperand;          // offset: two Q groups first
   static constexpr uint32_t kBars = kRing + kSlots * kOperand;
-  static constexpr size_t kBytes = kBars + 512 + 1024;     // barriers; alignment
+  static constexpr uint32_t kList = kBars + 512;           // row blocks before each sequence's
+  static constexpr uint32_t kStage = kList + 4 * (kMostSeqs + 4);  // output rows, 4 KB a softmax warp
+  static constexpr size_t kBytes = kStage + 8 * 4096 + 1024;       // and alignment
 };
 
 // 64 consecutive fp32 columns of this thread's TMEM lane.
@@ -252,12 +261,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* drained = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  volatile int* careful = abort_flag + 1;  // [2], by parity of the row block
+  // [8] by the CTA's count of items with keys, which the ring lets the loads be
+  // four ahead at most: count + 1 where such an item needs the plain way
+  volatile int* careful = abort_flag + 1;
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
-  const int h = blockIdx.y;
-  const int b = blockIdx.z;
+  int* const upto = reinterpret_cast<int*>(smem + SM::kList);  // [num_seqs + 1] items before a sequence's
 
   if (tid == 0) {
     for (int i = 0; i < kSlots; ++i) {
@@ -274,7 +284,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     mbar_init(smem_u32(drained), 1);
     fence_mbar_init();
     *abort_flag = 0;
-    careful[0] = careful[1] = 0;
+    for (int i = 0; i < 8; ++i) careful[i] = 0;
   }
   if (warp == 3) tmem_alloc(smem_u32(tmem_slot), 512);
   if (warp == 0 && lane == 0) {
@@ -288,12 +298,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   pdl_wait();
   pdl_launch_dependents();
 
-  const StreamSeq s = sequence_of(p, b);
-  const int rows_all = s.qlen * p.group;
+  // ---- the items: row blocks of a (sequence, KV head) are neighbours ----
+  for (int i = tid; i < p.num_seqs; i += kPromptThreads)
+    upto[i + 1] = (sequence_of(p, p.first_seq + i).qlen * p.group + kRows - 1) / kRows * p.hkv;
+  __syncthreads();
+  if (warp == 0) {
+    int sum = 0;
+    for (int i = 0; i < p.num_seqs; i += 32) {
+      int x = i + lane < p.num_seqs ? upto[i + lane + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
+      }
+      if (i + lane < p.num_seqs) upto[i + lane + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) upto[0] = 0;
+  }
+  __syncthreads();
+  const int items = upto[p.num_seqs];
+  struct Item {
+    int b, h, rb, rows_all;
+    StreamSeq s;
+  };
+  auto item_at = [&](int i) {
+    Item im;
+    int lo = 0, hi = p.num_seqs;  // upto[lo] <= i < upto[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (upto[mid] <= i) {
+        lo = mid;
+      } else {
+        hi = mid;
+      }
+    }
+    im.b = p.first_seq + lo;
+    im.s = sequence_of(p, im.b);
+    im.rows_all = im.s.qlen * p.group;
+    const int blocks = (im.rows_all + kRows - 1) / kRows;
+    im.h = (i - upto[lo]) / blocks;
+    im.rb = (i - upto[lo]) - im.h * blocks;
+    return im;
+  };
   const int bs = 1 << p.bs_log2;
   const int tile_pages = kKeys >> p.bs_log2;
-  auto range_of = [&](int rb) {
-    return StreamRange(s, rb * kRows, min(rb * kRows + kRows, rows_all), p.group, p.window, p.sinks, p.bs_log2);
+  auto range_of = [&](const Item& im) {
+    return StreamRange(im.s, im.rb * kRows, min(im.rb * kRows + kRows, im.rows_all), p.group, p.window, p.sinks,
+                       p.bs_log2);
   };
   // every row of the block sees list places [at, at + n)
   auto interior = [&](const StreamRange& rg, int at, int n) {
@@ -310,13 +362,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const int my_page = lane / kHalves;
     uint32_t n = 0;  // tiles of either kind issued so far
     bool ok = true;
-    for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
-      const StreamRange rg = range_of(rb);
+    for (int item = blockIdx.x, live = -1; ok && item < items; item += gridDim.x) {
+      const Item im = item_at(item);
+      const StreamRange rg = range_of(im);
       const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      live += tiles > 0 ? 1 : 0;
       auto look = [&](int t) -> int64_t {  // -2: no page there
         const int i = t * tile_pages + my_page;
         if (my_page >= tile_pages || i >= rg.pages) return -2;
-        return load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(rg.page(i)) * p.bts1);
+        return load_index(p.bt, p.bt64, im.b * p.bts0 + static_cast<int64_t>(rg.page(i)) * p.bts1);
       };
       int64_t next = look(0);
       for (int t = 0; ok && t < tiles; ++t) {
@@ -324,7 +378,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (t + 1 < tiles) next = look(t + 1);
         const bool valid = id >= 0 && id < p.num_blocks;
         if (id != -2 && !valid) {
-          careful[round & 1] = round + 1;
+          careful[live & 7] = live + 1;
           atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
         }
         const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, valid));
@@ -339,8 +393,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const int4 perm = kind ? vperm : kperm;
             const int blk = static_cast<int>(id);
             tma_load_4d(smem_u32(smem + SM::kRing + slot * SM::kOperand + my_half * SM::kHalf) + my_page * (bs * 128),
-                        kind ? &tmap_v : &tmap_k, bar, my_half * 64, tmap_coord(perm.x, h, blk),
-                        tmap_coord(perm.y, h, blk), tmap_coord(perm.z, h, blk), policy);
+                        kind ? &tmap_v : &tmap_k, bar, my_half * 64, tmap_coord(perm.x, im.h, blk),
+                        tmap_coord(perm.y, im.h, blk), tmap_coord(perm.z, im.h, blk), policy);
           }
         }
       }
@@ -361,17 +415,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const uint64_t q_desc = umma_smem_desc(base, 16, 1024, 2);
       const uint64_t k_desc = umma_smem_desc(base + SM::kRing, 16, 1024, 2);
       const uint64_t v_desc = umma_smem_desc(base + SM::kRing, SM::kHalf, 1024, 2);
-      uint32_t n = 0, it = 0;  // next slot, tiles done (per group)
+      uint32_t n = 0;                 // next slot
+      uint32_t it[2] = {0, 0};        // tiles done, per group
+      uint32_t q_round[2] = {0, 0};   // items so far that have the group
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, p.status, abort_flag));
         return ok;
       };
-      for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
-        const StreamRange rg = range_of(rb);
+      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const Item im = item_at(item);
+        const StreamRange rg = range_of(im);
         const int keys = uniform(rg.pages << p.bs_log2);
         const int tiles = (keys + kKeys - 1) / kKeys;
-        const int groups = uniform(rows_all - rb * kRows > 128 ? 2 : 1);
+        const int groups = uniform(im.rows_all - im.rb * kRows > 128 ? 2 : 1);
+        const uint32_t q_parity[2] = {q_round[0] & 1, q_round[1] & 1};
+        q_round[0] += 1;
+        q_round[1] += groups == 2 ? 1 : 0;
         if (tiles == 0) continue;
         auto keys16 = [&](int t) { return (min(kKeys, keys - t * kKeys) + 15) >> 4; };  // of tile t
         auto issue_s = [&](int g, int t, uint32_t slot) {
@@ -385,22 +445,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
           umma_done(on, smem_u32(&s_full[g]));
         };
-        for (int g = 0; ok && g < groups; ++g) wait(&q_ready[g], round & 1);
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (g < groups) wait(&q_ready[g], q_parity[g]);
         if (!wait(&full[n % kSlots], (n / kSlots) & 1)) break;
         tc_fence_after();
         for (int g = 0; g < groups; ++g) issue_s(g, 0, n % kSlots);
         umma_done(on, smem_u32(&empty[n % kSlots]));
         ++n;
-        for (int t = 0; t < tiles; ++t, ++it, n += 2) {  // n: V of tile t
+        for (int t = 0; t < tiles; ++t, n += 2) {  // n: V of tile t
           const uint32_t vs = n % kSlots, ks = (n + 1) % kSlots;
           const bool more = t + 1 < tiles;
           if (!wait(&v_ready[vs], (n / kSlots) & 1)) break;
           if (more && !wait(&full[ks], ((n + 1) / kSlots) & 1)) break;
           const uint64_t va = v_desc + vs * (SM::kOperand >> 4);
           const int k16 = keys16(t);
-          for (int g = 0; g < groups; ++g) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            if (g >= groups || !ok) continue;
             const uint32_t pa = tm + 128 * g, oa = tm + 256 + 128 * g;
-            if (!wait(&p_ready[g], it & 1)) break;
+            if (!wait(&p_ready[g], it[g] & 1)) continue;
+            ++it[g];
             tc_fence_after();
             umma_ts(on, oa, pa, va, kIdO, t > 0);
 #pragma unroll
@@ -428,9 +493,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     constexpr uint32_t kExp = kBf16 ? 0x7f80u : 0x7c00u;
     uint32_t n = 0;
     bool ok = true;
-    for (int rb = blockIdx.x, round = 0; ok && rb * kRows < rows_all; rb += gridDim.x, ++round) {
-      const StreamRange rg = range_of(rb);
+    for (int item = blockIdx.x, live = -1; ok && item < items; item += gridDim.x) {
+      const Item im = item_at(item);
+      const StreamRange rg = range_of(im);
       const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      live += tiles > 0 ? 1 : 0;
       const int shift = (rg.sink_pages - rg.win_page) << p.bs_log2;
       const int list = rg.pages << p.bs_log2;
       // list places that some row of the block sees: [0, s1) and [w0, w1)
@@ -470,7 +537,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               }
             }
           }
-          if (__any_sync(0xffffffffu, nonfinite16(top, kExp)) && lane == 0) careful[round & 1] = round + 1;
+          if (__any_sync(0xffffffffu, nonfinite16(top, kExp)) && lane == 0) careful[live & 7] = live + 1;
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -488,46 +555,67 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // a scale of 0 (uniform weights) stays above it: -inf * 0 is NaN
     const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
     const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // the scale's sign goes to q
-    uint32_t it = 0;
-    for (int rb = blockIdx.x, round = 0; rb * kRows + 128 * g < rows_all; rb += gridDim.x, ++round) {
-      bool ok = true;
-      const StreamRange rg = range_of(rb);
-      const int grow0 = rb * kRows + 128 * g;
-      // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane.
-      // A rolled loop: this code runs once per row block, and unrolled sixteen
-      // times its instruction fetches took 14k cycles of a 90k-cycle block ----
-      constexpr int kChunks = D / 8, kRowStep = 128 / kChunks;
+    constexpr int kChunks = D / 8, kRowStep = 128 / kChunks;
+    uint8_t* const q_area = smem + g * SM::kOperand + ((gt % kChunks) >> 3) * SM::kHalf;
+    // element offset of row r of an item's group, whose first row is the one of
+    // query qt0 and head rem0 (a small dividend: one multiplication)
+    auto row_at = [&](const Item& x, int qt0, int rem0, int r, int64_t s0, int64_t s1) -> int64_t {
+      const int add = p.group == 1 ? r : __umulhi(static_cast<uint32_t>(rem0 + r), p.group_magic);
+      return (x.s.q0 + qt0 + add) * s0 + (x.h * p.group + rem0 + r - add * p.group) * s1;
+    };
+    // The group's queries of item x to its q area: cp.async where they are
+    // aligned.  Hardly unrolled: it runs once per item, and unrolled sixteen
+    // times its instruction fetches took 14k cycles.
+    auto load_q = [&](const Item& x) {
+      const int grow0 = x.rb * kRows + 128 * g;
       const int c = gt % kChunks, r0 = gt / kChunks;
       const int qt0 = grow0 / p.group, rem0 = grow0 - qt0 * p.group;
-      // element offset of row r of the group (a small dividend: one multiplication)
-      auto row_at = [&](int r, int64_t s0, int64_t s1) -> int64_t {
-        const int add = p.group == 1 ? r : __umulhi(static_cast<uint32_t>(rem0 + r), p.group_magic);
-        return (s.q0 + qt0 + add) * s0 + (h * p.group + rem0 + r - add * p.group) * s1;
-      };
-      uint8_t* const area = smem + g * SM::kOperand + (c >> 3) * SM::kHalf;
       if (p.q_vec) {
         const T* const src = static_cast<const T*>(p.q) + c * 8;
 #pragma unroll 4
         for (int r = r0; r < 128; r += kRowStep) {
-          const bool in = grow0 + r < rows_all;
-          cp_async16(smem_u32(area) + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (in ? row_at(r, p.qs0, p.qs1) : 0),
-                     in ? 16 : 0);
+          const bool in = grow0 + r < x.rows_all;
+          cp_async16(smem_u32(q_area) + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                     src + (in ? row_at(x, qt0, rem0, r, p.qs0, p.qs1) : 0), in ? 16 : 0);
         }
-        cp_async_commit();
-        cp_async_wait<0>();
       } else {
 #pragma unroll 1
         for (int r = r0; r < 128; r += kRowStep) {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (grow0 + r < rows_all)
-            x = gather8(static_cast<const T*>(p.q) + row_at(r, p.qs0, p.qs1) + c * 8 * p.qs2, p.qs2);
-          *reinterpret_cast<uint4*>(area + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+          uint4 y = make_uint4(0u, 0u, 0u, 0u);
+          if (grow0 + r < x.rows_all)
+            y = gather8(static_cast<const T*>(p.q) + row_at(x, qt0, rem0, r, p.qs0, p.qs1) + c * 8 * p.qs2, p.qs2);
+          *reinterpret_cast<uint4*>(q_area + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = y;
         }
       }
+      cp_async_commit();
+    };
+    uint32_t it = 0;
+    int live = -1;
+    bool here = false;  // the queries of this item are on their way
+    Item im = {0, 0, 0, 0, {0, 0, 0}};
+    if (static_cast<int>(blockIdx.x) < items) im = item_at(blockIdx.x);
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      bool ok = true;
+      const Item cur = im;
+      const StreamRange rg = range_of(cur);
+      const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      live += tiles > 0 ? 1 : 0;
+      const bool more = item + static_cast<int>(gridDim.x) < items;
+      if (cur.rb * kRows + 128 * g >= cur.rows_all) {  // not a row of this group's
+        if (more) im = item_at(item + gridDim.x);
+        continue;
+      }
+      const int rows_all = cur.rows_all;
+      const int grow0 = cur.rb * kRows + 128 * g;
+      // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane ----
+      const int c = gt % kChunks, r0 = gt / kChunks;
+      if (!here) load_q(cur);
+      here = false;
+      cp_async_wait<0>();
       if (flip) {  // the chunks this thread brought itself
 #pragma unroll 1
         for (int r = r0; r < 128; r += kRowStep) {
-          uint4* x = reinterpret_cast<uint4*>(area + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+          uint4* x = reinterpret_cast<uint4*>(q_area + r * 128 + (((c & 7) ^ (r & 7)) << 4));
           *x = make_uint4(x->x ^ flip, x->y ^ flip, x->z ^ flip, x->w ^ flip);
         }
       }
@@ -536,8 +624,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
       const int row = grow0 + gt;
       const int qt = min(row, rows_all - 1) / p.group;
-      const RowView view = view_of(p, rg, s.n - s.qlen + qt);
-      const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
+      const RowView view = view_of(p, rg, cur.s.n - cur.s.qlen + qt);
       // list places that every row sees: [0, all_s) and [all_0, all_1)
       const RowView row_0 = view_of(p, rg, rg.pos0), row_n = view_of(p, rg, rg.pos1);
       const int all_s = rg.pos0 < 0 ? 0 : row_0.sink_end, all_0 = row_n.w0, all_1 = rg.pos0 < 0 ? 0 : row_0.w1 + 1;
@@ -621,53 +708,67 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tc_fence_before();
         mbar_arrive(smem_u32(&p_ready[g]));
       }
+      // The last S of this item is done, so its queries make room for the next
+      // item's while its last product and its epilogue run.
+      if (more) im = item_at(item + gridDim.x);
+      if (ok && tiles > 0 && more && im.rb * kRows + 128 * g < im.rows_all) {
+        load_q(im);
+        here = true;
+      }
       if (ok && tiles > 0) ok = pv_wait();
-      // all warps of the group go on or none: the barriers below have no limit
+      // all warps of the group go on or none
       if (barrier_any(1 + g, 128, !ok)) break;
       const float l = l2.x + l2.y;
       tc_fence_after();
-      if (careful[round & 1] == round + 1) {
+      if (tiles > 0 && careful[live & 7] == live + 1) {
         const int w0 = grow0 + (warp & 3) * 32;
-        careful_rows<T, D>(p, s, b, h, w0, max(0, min(32, rows_all - w0)), lane);
-        continue;
-      }
-      // ---- O / l through the group's q area (its products are done), so that
-      // 16 (or 8) lanes write a row: stored from TMEM rows directly, a lane
-      // each, the epilogue took 11k cycles of a 100k-cycle row block ----
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint8_t* const rows_out = smem + g * SM::kOperand;
+        careful_rows<T, D>(p, cur.s, cur.b, cur.h, w0, max(0, min(32, rows_all - w0)), lane);
+      } else {
+        // ---- O / l, 64 dims at a time through 4 KB of the warp's own, so that
+        // 8 lanes write 128 bytes of a row: stored from TMEM rows directly, a
+        // lane each, the epilogue took 11k cycles of a 100k-cycle row block ----
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int w0 = 32 * (warp & 3);  // the warp's first row of the group
+        const int qt0 = grow0 / p.group, rem0 = grow0 - qt0 * p.group;
+        uint8_t* const stage = smem + SM::kStage + (warp - 4) * 4096;
+        T* const out = static_cast<T*>(p.out);
 #pragma unroll 1
-      for (int q4 = 0; q4 < D / 32; ++q4) {
-        float o[32];
-        if (tiles > 0) {
-          tmem_ld32(o_addr + 32 * q4, o);
-        } else {
+        for (int hf = 0; hf < D / 64; ++hf) {
+#pragma unroll 1
+          for (int q4 = 0; q4 < 2; ++q4) {
+            float o[32];
+            if (tiles > 0) {
+              tmem_ld32(o_addr + 64 * hf + 32 * q4, o);
+            } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        }
+              for (int i = 0; i < 32; ++i) o[i] = 0.f;
+            }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
+            for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(rows_out + gt * (D * 2) + (((4 * q4 + i) ^ (gt & 7)) << 4)) =
-              make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
-                         pack2<T>(o[8 * i + 4], o[8 * i + 5]), pack2<T>(o[8 * i + 6], o[8 * i + 7]));
-      }
-      named_barrier(1 + g, 128);
-      T* const out = static_cast<T*>(p.out);
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * q4 + i) ^ (lane & 7)) << 4)) =
+                  make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
+                             pack2<T>(o[8 * i + 4], o[8 * i + 5]), pack2<T>(o[8 * i + 6], o[8 * i + 7]));
+          }
+          __syncwarp();
+          const int cc = lane & 7;
 #pragma unroll 4
-      for (int r = r0; r < min(128, rows_all - grow0); r += kRowStep) {
-        const uint4 x = *reinterpret_cast<const uint4*>(rows_out + r * (D * 2) + ((c ^ (r & 7)) << 4));
-        if (p.out_vec) {
-          *reinterpret_cast<uint4*>(out + row_at(r, p.os0, p.os1) + c * 8) = x;
-        } else {
-          T* dst = out + row_at(r, p.os0, p.os1);
-          const T* y = reinterpret_cast<const T*>(rows_out + r * (D * 2) + ((c ^ (r & 7)) << 4));
+          for (int i = lane >> 3; i < 32; i += 4) {
+            if (grow0 + w0 + i >= rows_all) break;
+            const T* y = reinterpret_cast<const T*>(stage + i * 128 + ((cc ^ (i & 7)) << 4));
+            T* dst = out + row_at(cur, qt0, rem0, w0 + i, p.os0, p.os1);
+            const int d = 64 * hf + 8 * cc;
+            if (p.out_vec) {
+              *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(y);
+            } else {
 #pragma unroll 1
-          for (int k = 0; k < 8; ++k) dst[(c * 8 + k) * p.os2] = y[k];
+              for (int k = 0; k < 8; ++k) dst[(d + k) * p.os2] = y[k];
+            }
+          }
+          __syncwarp();
         }
       }
-      named_barrier(1 + g, 128);  // the q area is free
       tc_fence_before();
     }
   }
@@ -692,8 +793,8 @@ int launch(const StreamParams& p, const CUtensorMap& mk, const CUtensorMap& mv, 
 
 }  // namespace
 
-bool prompt_attention(const StreamParams& p, bool bf16, int D, int64_t max_query_len, cudaStream_t stream,
-                      int* rc) {
+bool prompt_attention(const StreamParams& p, bool bf16, int D, int64_t max_query_len, int64_t sms,
+                      cudaStream_t stream, int* rc) {
   CacheDesc kd;
   kd.base = p.k;
   kd.elem_bytes = 2;
@@ -711,14 +812,21 @@ bool prompt_attention(const StreamParams& p, bool bf16, int D, int64_t max_query
   CUtensorMap mk, mv;
   int kp[4], vp[4];
   if (!get_cache_tensor_map(kd, &mk, kp) || !get_cache_tensor_map(vd, &mv, vp)) return false;
-  const int64_t blocks = (max_query_len * p.group + kRows - 1) / kRows;
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, 1 << 20)), p.hkv, p.num_seqs);
-  if (D == 128) {
-    *rc = bf16 ? launch<__nv_bfloat16, 128>(p, mk, mv, kp, vp, grid, stream)
-               : launch<__half, 128>(p, mk, mv, kp, vp, grid, stream);
-  } else {
-    *rc = bf16 ? launch<__nv_bfloat16, 64>(p, mk, mv, kp, vp, grid, stream)
-               : launch<__half, 64>(p, mk, mv, kp, vp, grid, stream);
+  StreamParams part = p;
+  *rc = FD_OK;
+  for (part.first_seq = 0; *rc == FD_OK && part.first_seq < p.num_seqs; part.first_seq += kMostSeqs) {
+    part.num_seqs = std::min(p.num_seqs - part.first_seq, kMostSeqs);
+    // row blocks of the announced queries, or of all rows of q where those are fewer
+    const int64_t each = (max_query_len * p.group + kRows - 1) / kRows * part.num_seqs;
+    const int64_t all = static_cast<int64_t>(p.num_tokens) * p.group / kRows + part.num_seqs;
+    const dim3 grid(static_cast<unsigned>(std::max<int64_t>(std::min(std::min(each, all) * p.hkv, sms), 1)));
+    if (D == 128) {
+      *rc = bf16 ? launch<__nv_bfloat16, 128>(part, mk, mv, kp, vp, grid, stream)
+                 : launch<__half, 128>(part, mk, mv, kp, vp, grid, stream);
+    } else {
+      *rc = bf16 ? launch<__nv_bfloat16, 64>(part, mk, mv, kp, vp, grid, stream)
+                 : launch<__half, 64>(part, mk, mv, kp, vp, grid, stream);
+    }
   }
   return true;
 }

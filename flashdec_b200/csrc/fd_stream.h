@@ -91,7 +91,7 @@ struct StreamRange {
 // fd_window_attention on tcgen05, for many rows per (sequence, KV head).  False
 // when no tensor map describes the caches (nothing is launched); else *rc is
 // the launch's status.
-bool prompt_attention(const StreamParams& p, bool bf16, int head_dim, int64_t max_query_len,
+bool prompt_attention(const StreamParams& p, bool bf16, int head_dim, int64_t max_query_len, int64_t sms,
                       cudaStream_t stream, int* rc);
 
 }  // namespace fd

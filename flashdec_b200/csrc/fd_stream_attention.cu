@@ -1141,7 +1141,7 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
   p.device = dev->device;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   const bool bf16 = a->dtype == FD_DTYPE_BF16;
-  if (pl.prompt && prompt_attention(p, bf16, a->head_dim, pl.max_query, stream, &rc)) return rc;
+  if (pl.prompt && prompt_attention(p, bf16, a->head_dim, pl.max_query, dev->num_sms, stream, &rc)) return rc;
   for (p.first_seq = 0; rc == FD_OK && p.first_seq < a->num_seqs; p.first_seq += kMaxListed) {
     p.num_seqs = std::min(a->num_seqs - p.first_seq, kMaxListed);
     if (a->head_dim == 128) {
