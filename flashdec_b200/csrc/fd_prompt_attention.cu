@@ -261,9 +261,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* drained = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  // [8] by the CTA's count of items with keys, which the ring lets the loads be
-  // four ahead at most: count + 1 where such an item needs the plain way
+  // [8] by the CTA's count of items with keys: count + 1 where such an item
+  // needs the plain way.  The loads are a few items ahead of the group that
+  // works; the other one may lag (items of one group go past it), so a group
+  // says how many it has `seen`, and a place that is taken again before both
+  // have read it sends all later items the plain way.
   volatile int* careful = abort_flag + 1;
+  volatile int* seen = careful + 8;  // [group]
+  volatile int* all_careful = seen + 2;
+  auto need_care = [&](int count) {
+    if (count >= 8 && (seen[0] < count - 7 || seen[1] < count - 7)) {
+      *all_careful = 1;
+      __threadfence_block();
+    }
+    careful[count & 7] = count + 1;
+  };
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -285,6 +297,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     fence_mbar_init();
     *abort_flag = 0;
     for (int i = 0; i < 8; ++i) careful[i] = 0;
+    seen[0] = seen[1] = *all_careful = 0;
   }
   if (warp == 3) tmem_alloc(smem_u32(tmem_slot), 512);
   if (warp == 0 && lane == 0) {
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (t + 1 < tiles) next = look(t + 1);
         const bool valid = id >= 0 && id < p.num_blocks;
         if (id != -2 && !valid) {
-          careful[live & 7] = live + 1;
+          need_care(live);
           atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
         }
         const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, valid));
@@ -417,7 +430,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const uint64_t v_desc = umma_smem_desc(base + SM::kRing, SM::kHalf, 1024, 2);
       uint32_t n = 0;                 // next slot
       uint32_t it[2] = {0, 0};        // tiles done, per group
-      uint32_t q_round[2] = {0, 0};   // items so far that have the group
+      uint32_t q_round[2] = {0, 0};   // items with keys so far that have the group
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         ok = ok && __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, p.status, abort_flag));
@@ -429,10 +442,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int keys = uniform(rg.pages << p.bs_log2);
         const int tiles = (keys + kKeys - 1) / kKeys;
         const int groups = uniform(im.rows_all - im.rb * kRows > 128 ? 2 : 1);
+        if (tiles == 0) continue;
         const uint32_t q_parity[2] = {q_round[0] & 1, q_round[1] & 1};
         q_round[0] += 1;
         q_round[1] += groups == 2 ? 1 : 0;
-        if (tiles == 0) continue;
         auto keys16 = [&](int t) { return (min(kKeys, keys - t * kKeys) + 15) >> 4; };  // of tile t
         auto issue_s = [&](int g, int t, uint32_t slot) {
           const uint32_t idesc = umma_idesc_f16(kBf16, false, 128, 16 * keys16(t));
@@ -537,7 +550,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               }
             }
           }
-          if (__any_sync(0xffffffffu, nonfinite16(top, kExp)) && lane == 0) careful[live & 7] = live + 1;
+          if (__any_sync(0xffffffffu, nonfinite16(top, kExp)) && lane == 0) need_care(live);
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -602,6 +615,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       live += tiles > 0 ? 1 : 0;
       const bool more = item + static_cast<int>(gridDim.x) < items;
       if (cur.rb * kRows + 128 * g >= cur.rows_all) {  // not a row of this group's
+        if (gt == 0) seen[g] = live + 1;
         if (more) im = item_at(item + gridDim.x);
         continue;
       }
@@ -609,18 +623,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int grow0 = cur.rb * kRows + 128 * g;
       // ---- q rows into the K-major operand (128B swizzle), 16 bytes a lane ----
       const int c = gt % kChunks, r0 = gt / kChunks;
-      if (!here) load_q(cur);
+      if (tiles > 0 && !here) load_q(cur);
       here = false;
       cp_async_wait<0>();
-      if (flip) {  // the chunks this thread brought itself
+      if (flip && tiles > 0) {  // the chunks this thread brought itself
 #pragma unroll 1
         for (int r = r0; r < 128; r += kRowStep) {
           uint4* x = reinterpret_cast<uint4*>(q_area + r * 128 + (((c & 7) ^ (r & 7)) << 4));
           *x = make_uint4(x->x ^ flip, x->y ^ flip, x->z ^ flip, x->w ^ flip);
         }
       }
-      fence_proxy_async_smem();
-      mbar_arrive(smem_u32(&q_ready[g]));
+      // Only for products that wait for it: a phase nobody waits for would let
+      // the wait for the next one return at once.
+      if (tiles > 0) {
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&q_ready[g]));
+      }
 
       const int row = grow0 + gt;
       const int qt = min(row, rows_all - 1) / p.group;
@@ -716,11 +734,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         here = true;
       }
       if (ok && tiles > 0) ok = pv_wait();
+      bool plain = false;
+      if (tiles > 0) {
+        plain = careful[live & 7] == live + 1;
+        __threadfence_block();
+        plain = plain || *all_careful != 0;
+      }
       // all warps of the group go on or none
       if (barrier_any(1 + g, 128, !ok)) break;
+      if (gt == 0) seen[g] = live + 1;
       const float l = l2.x + l2.y;
       tc_fence_after();
-      if (tiles > 0 && careful[live & 7] == live + 1) {
+      if (plain) {
         const int w0 = grow0 + (warp & 3) * 32;
         careful_rows<T, D>(p, cur.s, cur.b, cur.h, w0, max(0, min(32, rows_all - w0)), lane);
       } else {
