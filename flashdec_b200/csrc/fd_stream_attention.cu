@@ -951,7 +951,6 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
                          : std::min<int64_t>(a->max_query_len, std::max<int64_t>(tokens, 1));
   const int64_t rows = mq * group;
   pl.max_query = mq;
-  pl.prompt = rows >= 256;
   pl.m16 = rows > 16 ? 2 : 1;
   const int per = 16 * pl.m16;
   pl.row_blocks = static_cast<int>(
@@ -966,6 +965,24 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   const int64_t tiles = (seen + kTok - 1) / kTok;
   const int64_t units = static_cast<int64_t>(a->num_seqs) * a->num_kv_heads * pl.row_blocks;
   const int64_t slots = 2 * sms;  // two CTAs fit an SM
+  // Which kernel: by their times in us, as measured with 2 to 32 query heads a
+  // KV head, 1 to 16 sequences and 4 to 256 queries at a window of 2048.  The
+  // prompt kernel takes 6 + 1.9 a tile of 128 keys for each round of 256-row
+  // blocks over the SMs (16 sequences, 8 KV heads: 41 us for 64 rows, 93 for
+  // 512); this one 12 + 2.4 for every 16-token tile of its busiest warp (88 and
+  // 490 there), 1.7 with heads of 64 (24 sequences' drafts: 20, 27 by the prompt
+  // kernel).  Few rows of few sequences against a long window go to this one,
+  // which splits the keys (1 sequence, 2 KV heads, 128 rows: 17 us, 38).
+  if (!scored && rows > 16) {
+    const int64_t blocks = (rows + 255) / 256 * a->num_kv_heads * a->num_seqs;
+    const int64_t keys = std::min(cap, std::min<int64_t>(a->window, cap) +
+                                           std::min<int64_t>(a->sinks, cap) + 256 / group + 2 * a->block_size);
+    const double prompt_us =
+        static_cast<double>((blocks + sms - 1) / sms) * (6 + 1.9 * static_cast<double>((keys + 127) / 128));
+    const double split_us = 12 + (a->head_dim == 128 ? 2.4 : 1.7) * static_cast<double>(units * tiles) /
+                                     static_cast<double>(kWarps * slots);
+    pl.prompt = prompt_us < split_us;
+  }
   const size_t q_rows = static_cast<size_t>(tokens) * a->num_q_heads;
   pl.raw_tokens = (cap + kTok - 1) / kTok * kTok;
   const int64_t row_most = std::min<int64_t>(rows, per);
@@ -975,11 +992,17 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   if (in_cluster > 1 && units * in_cluster <= slots) {
     const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, 2 * kWarps) * kTok;
     const size_t raw = scored ? static_cast<size_t>(run) * row_most * sizeof(float) : 0;
-    if (run <= kClusterRun && raw <= kRawBytes) {
+    // one CTA an SM if two do not fit: then clusters of 8 leave some SMs of a
+    // GPC idle, and three quarters of them have to do
+    const size_t base = a->head_dim == 128 ? (pl.m16 == 1 ? split_smem_bytes<128, 1>() : split_smem_bytes<128, 2>())
+                                           : (pl.m16 == 1 ? split_smem_bytes<64, 1>() : split_smem_bytes<64, 2>());
+    const size_t more = raw + receive_bytes(static_cast<int>(in_cluster), static_cast<int>(row_most), a->head_dim);
+    const bool fits = 2 * (base + more + 1024) <= 228 * 1024 || units * in_cluster <= sms * 3 / 4;
+    if (fits && run <= kClusterRun && raw <= kRawBytes) {
       pl.mode = kCluster;
       pl.rows_most = static_cast<int>(row_most);
       pl.splits = static_cast<int>(in_cluster);
-      pl.more_smem = raw + receive_bytes(pl.splits, pl.rows_most, a->head_dim);
+      pl.more_smem = more;
       pl.raw_tokens = run;
       return pl;
     }
