@@ -42,8 +42,11 @@ constexpr size_t split_smem_bytes() {
 }
 // what the other CTAs of a cluster send: (max, sum) per row and their part of
 // this CTA's share of the rows' elements
-constexpr size_t receive_bytes(int splits, int rows, int D) {
-  return sizeof(float) * (static_cast<size_t>(splits) * rows * 2 + static_cast<size_t>(rows) * D + 4 * splits);
+__host__ __device__ constexpr int receive_ml(int splits, int rows) {  // floats; what follows starts on 16 bytes
+  return (2 * splits * rows + 3) & ~3;
+}
+__host__ __device__ constexpr size_t receive_bytes(int splits, int rows, int D) {
+  return sizeof(float) * (static_cast<size_t>(receive_ml(splits, rows)) + static_cast<size_t>(rows) * D + 4 * splits);
 }
 
 // Elements d .. d + 3 of a row.
@@ -108,7 +111,7 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 //             partials.  As many shares as CTAs fit: with four times as many,
 //             one long sequence of 131071 tokens took 117 us (97), 64 sequences
 //             of up to 4100 visible tokens 180 us (162).
-// Partials go to stream_finish_kernel.
+// Partials go to stream_merge_kernel.
 // ---------------------------------------------------------------------------
 template <typename T, int D, int kM>
 __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_constant__ StreamParams p) {
@@ -122,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   float* lse = weight + kMaxCluster * kRows;                           // [row]
   float* inv_sum = lse + kRows;                                        // [row], one split
   float* got_ml = reinterpret_cast<float*>(smem + split_smem_bytes<D, kM>());  // [split][rows_most][2]
-  float* got = got_ml + 2 * p.splits * p.rows_most;                            // [split][share]
+  float* got = got_ml + receive_ml(p.splits, p.rows_most);                            // [split][share]
   float* raw = p.mode == kCluster ? got_ml + receive_bytes(p.splits, p.rows_most, D) / sizeof(float) : got_ml;  // [row][raw_tokens]
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -138,6 +141,8 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   const float scale = fmaxf(fabsf(p.scale_log2), 1e-30f);
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
 
+  const bool cluster = p.mode == kCluster, grid = p.mode == kGrid;
+  if (cluster) cluster_arrive_relaxed();  // all its CTAs run before one of them is sent anything
   pdl_wait();
   pdl_launch_dependents();
   uint8_t* const kring = smem + warp * (kStages * 2 * kTileBytes);
@@ -148,7 +153,9 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
   const uint32_t k_off = tile_chunk<D>((mi >> 1) * 8 + r8, mi & 1);
   const uint32_t v_off = tile_chunk<D>((mi & 1) * 8 + r8, mi >> 1);
 
-  const bool cluster = p.mode == kCluster, grid = p.mode == kGrid;
+  // what a cluster receives has room for as many rows as were announced: where
+  // there are more, they are taken that many at a time
+  const int block_rows = cluster ? p.rows_most : kRows;
   int b = 0, h = 0, rb = 0;
   StreamSeq s;
   int64_t at = 0, end = 0;  // this CTA's share of the tiles
@@ -203,6 +210,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
     }
     if (blockIdx.x == 0 && tid == 0) *p.shares = shares;
   }
+  if (cluster) cluster_wait();
   for (;;) {
     int from = 0, to = 0, all = 0;  // the segment: tiles [from, to) of the unit's `all`
     if (!cluster && !grid) {
@@ -220,15 +228,15 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       s = sequence_of(p, b);
     }
     const int rows_all = s.qlen * p.group;
-    if (rb * kRows >= rows_all) break;  // of a cluster or grid: the last row block is done
+    if (rb * block_rows >= rows_all) break;  // of a cluster or grid: the last row block is done
     // (grid: row blocks past the announced ones have no place for partials)
     const bool whole_unit = cluster ? false : grid ? rb >= p.row_blocks || p.splits == 1 : from == 0 && to == all;
     if (grid && whole_unit && blockIdx.x > 0) break;
     const int part = grid ? (blockIdx.z * gridDim.y + blockIdx.y) * p.splits + blockIdx.x
                           : 2 * blockIdx.x + (from == 0 ? 1 : 0);  // place of a partial
     {
-      const int row0 = rb * kRows;
-      const int rows = min(kRows, rows_all - row0);
+      const int row0 = rb * block_rows;
+      const int rows = min(block_rows, rows_all - row0);
       const StreamRange rg(s, row0, row0 + rows, p.group, p.window, p.sinks, p.bs_log2);
       const int tiles = ((rg.pages << p.bs_log2) + kTok - 1) / kTok;
       const int splits = p.splits, split = blockIdx.x;  // of a cluster
@@ -744,7 +752,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
             *slot[i] = old[i] + w;
           }
         }
-        if ((rb + p.row_blocks) * kRows < rows_all) {  // the next rows are sent to the same place
+        if ((rb + p.row_blocks) * block_rows < rows_all) {  // the next rows are sent to the same place
           cluster_arrive();
           cluster_wait();
         }

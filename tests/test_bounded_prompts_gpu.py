@@ -117,3 +117,39 @@ def test_both_sides_of_the_choice_of_kernel(d, hq, hkv, seqs, ql):
                               query_start_loc=torch.from_numpy(st).cuda(), max_query_len=ql)
     exact, size = ref.window_attention_ref(qn, c.k_np, c.v_np, c.table_np, lens, window, sinks, st)
     close(out, exact, size, "bf16", window + sinks)
+
+
+@pytest.mark.parametrize("ql", [2, 7, 16, 50])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(1, 1, 128, 16), (3, 1, 64, 8), (16, 2, 128, 32), (20, 1, 64, 16)])
+def test_more_queries_than_announced_over_a_long_window(hq, hkv, d, bs, ql):
+    """One query announced, and more there: what the parts of a window send to
+    one another has its place for the announced rows only."""
+    import flashdec_b200 as fd
+
+    lens, qs = [3000, 40], [ql, ql - 1]
+    c = Cache(35, lens, hkv=hkv, d=d, bs=bs)
+    q, qn = c.queries(sum(qs), hq)
+    st = starts_of(qs)
+    for window in (700, 2900):
+        out = fd.window_attention(q, c.k, c.v, c.table, c.seq, window=window, sinks=3,
+                                  query_start_loc=torch.from_numpy(st).cuda(), max_query_len=1)
+        exact, size = ref.window_attention_ref(qn, c.k_np, c.v_np, c.table_np, lens, window, 3, st)
+        close(out, exact, size, "bf16", window + 3)
+
+
+@pytest.mark.parametrize("tokens", [250, 390, 500, 640, 800, 900, 1100])
+@pytest.mark.parametrize("hq,hkv,d", [(1, 1, 128), (2, 2, 64), (3, 1, 128), (5, 1, 64)])
+def test_any_number_of_parts_and_rows(tokens, hq, hkv, d):
+    """One sequence in two to eight parts, with few heads: odd counts of both."""
+    import flashdec_b200 as fd
+
+    c = Cache(36, [tokens], hkv=hkv, d=d, bs=16)
+    q, qn = c.queries(1, hq)
+    out = fd.window_attention(q, c.k, c.v, c.table, c.seq, window=tokens)
+    exact, size = ref.window_attention_ref(qn, c.k_np, c.v_np, c.table_np, [tokens], tokens)
+    close(out, exact, size, "bf16", tokens)
+    scores = torch.ones((c.pool, hkv, 16), device="cuda")
+    out = fd.scored_decode(q, c.k, c.v, scores, c.table, c.seq)
+    exact, size, want = ref.scored_decode_ref(qn, c.k_np, c.v_np, np.ones((c.pool, hkv, 16)), c.table_np, [tokens])
+    close(out, exact, size, "bf16", tokens)
+    assert (np.abs(scores.double().cpu().numpy() - want) <= 1e-4 * np.abs(want - 1) + 1e-6).all()
