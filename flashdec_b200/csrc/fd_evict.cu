@@ -101,7 +101,9 @@ __device__ __forceinline__ int block_exclusive(int x, int* warp_sums, int& total
 // finds the same digit.  Then one pass in order keeps the protected tokens
 // (sinks and recent), the keys above the threshold and the first of the keys
 // equal to it.  The counts are whole numbers: no order of the atomics changes
-// the result.
+// the result.  A chain bounds it: the keys' two look-ups, then a cluster
+// barrier and a scan for every digit and one for the counts (17 us for 16
+// sequences of 4400 tokens and 8 heads, 4 MB).
 __global__ void __launch_bounds__(kSelectThreads, 3)
     evict_select_kernel(const __grid_constant__ EvictParams p, int key_cap) {
   extern __shared__ __align__(16) int dyn[];
@@ -352,7 +354,7 @@ constexpr size_t copy_smem_bytes() {
 // and they go out from there two batches later.  Reads and writes both random
 // 256-byte rows: what bounds it is the bytes in flight.  Rows held in registers
 // instead (20 warps an SM, 4 KB each, and nothing in flight while they store)
-// took 119 us for 537 MB.
+// took 119 us for 537 MB; this takes 88, 6.1 TB/s read and written together.
 template <int D>
 __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ __align__(16) uint8_t ring_all[];

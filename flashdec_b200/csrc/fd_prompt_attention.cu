@@ -31,6 +31,12 @@ namespace {
 // start and end were a sixth of its time or more); 314 against 306 us for an 8k
 // prompt of 17 tiles an item, which pays for the longer code instead.
 //
+// What bounds it: the softmax.  A tile costs a thread 128 scores to scale,
+// exponentiate and pack, which its issue slots take longer for than the tensor
+// pipe for both products (8k queries, window 2048, 32/8 heads: 241 GFLOP in
+// 315-325 us, 0.46 of the rate of a large library product; the tensor pipe is busy a
+// third to a half of the time).
+//
 //   warp 0      TMA producer: K and V tiles alternate through a ring of slots
 //   warp 1      issues the tcgen05.mma (one thread)
 //   warps 2, 3  V tiles with keys that some row does not see: rows that no row

@@ -112,6 +112,14 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 //             one long sequence of 131071 tokens took 117 us (97), 64 sequences
 //             of up to 4100 visible tokens 180 us (162).
 // Partials go to stream_merge_kernel.
+//
+// Bounds: long windows, the reads of K and V, once each (64 sequences of up to
+// 131072 tokens, window 4096, 32/8 heads of 128: 892 MB in 166 us, 5.4 TB/s; one
+// sequence of 131071 tokens: 537 MB in 95 us, 5.7 TB/s); a short one, a chain of
+// dependent steps - table, first tile, its product, two merges (one token,
+// window 1024, 16/2 heads: 9.2 us, of which 0.16 are bytes).  Above 16 rows the
+// instructions a tile weigh as much (24 sequences of up to 7 drafts, window 1500,
+// 16/4 heads of 64: 20 us for 27 MB, merge included; DRAM 17 % busy).
 // ---------------------------------------------------------------------------
 template <typename T, int D, int kM>
 __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_constant__ StreamParams p) {
@@ -857,7 +865,10 @@ __global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_con
 }
 
 // Every token's score gets the sum over the group of exp2(raw - lse), four
-// neighbouring tokens a thread.
+// neighbouring tokens a thread.  Bound by its reads of the raw scores (one
+// sequence of 131071 tokens, 32/8 heads: 25 MB in 10 us, cold).  The weights have
+// to wait for the whole row's sum, so the scores go through memory once; kept in
+// the CTA instead where a cluster holds the row.
 __global__ void __launch_bounds__(kThreads) stream_scores_kernel(const __grid_constant__ StreamParams p) {
   extern __shared__ float lse[];  // [group]
   const int tid = threadIdx.x;
@@ -995,7 +1006,7 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   pl.raw_tokens = (cap + kTok - 1) / kTok * kTok;
   const int64_t row_most = std::min<int64_t>(rows, per);
   // Few units with short runs: the splits of each merge inside a cluster, with
-  // no second launch (one token of one sequence: 8.9 us, 14.4 with partials).
+  // no second launch (one token of one sequence: 9.2 us, 14.4 with partials).
   const int64_t in_cluster = std::min<int64_t>(tiles / (2 * kWarps), kMaxCluster);
   if (in_cluster > 1 && units * in_cluster <= slots) {
     const int64_t run = std::max<int64_t>((tiles + in_cluster - 1) / in_cluster, 2 * kWarps) * kTok;
@@ -1016,7 +1027,7 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
     }
   }
   // A wave of CTAs with kGridRun tiles each at most: a grid of equal splits, which
-  // needs no count of the batch's tiles first (24 sequences' drafts: 22 us,
+  // needs no count of the batch's tiles first (24 sequences' drafts: 20 us,
   // 31 as shares).  More: shares.
   const int64_t even = std::max<int64_t>(std::min<int64_t>(slots / units, tiles / (2 * kWarps)), 1);
   if (units <= slots && (tiles + even - 1) / even <= kGridRun && a->num_seqs <= kMaxListed) {
