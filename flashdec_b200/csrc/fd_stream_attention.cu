@@ -105,16 +105,19 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 //   kCluster  a unit per cluster, a segment per CTA; they merge through
 //             distributed shared memory.
 //   kGrid     a unit per p.splits CTAs, a segment each, as partials.
-//   kShares   the tiles of all units in a row are cut into equal shares, one
-//             per CTA, whatever the lengths: a CTA has a few segments, of which
-//             only the first and the last can be parts of a unit and leave
-//             partials.  As many shares as CTAs fit: with four times as many,
-//             one long sequence of 131071 tokens took 117 us (97), 64 sequences
-//             of up to 4100 visible tokens 180 us (162).
+//   kShares   the tiles of all sequences in a row are cut into equal shares, one
+//             per CTA and KV head, whatever the lengths: a CTA has a few
+//             segments, of which only the first and the last can be parts of a
+//             unit and leave partials.  The heads' CTAs of a share go over the
+//             same pages together: with the heads one after another in the row,
+//             24 sequences with interleaved heads took 151 us (139), 64 with a
+//             plane a head 166 (161).  As many shares as CTAs fit: with four
+//             times as many, one long sequence of 131071 tokens took 117 us
+//             (97), 64 sequences of up to 4100 visible tokens 180 us (162).
 // Partials go to stream_merge_kernel.
 //
 // Bounds: long windows, the reads of K and V, once each (64 sequences of up to
-// 131072 tokens, window 4096, 32/8 heads of 128: 892 MB in 166 us, 5.4 TB/s; one
+// 131072 tokens, window 4096, 32/8 heads of 128: 892 MB in 161 us, 5.5 TB/s; one
 // sequence of 131071 tokens: 537 MB in 95 us, 5.7 TB/s); a short one, a chain of
 // dependent steps - table, first tile, its product, two merges (one token,
 // window 1024, 16/2 heads: 9.2 us, of which 0.16 are bytes).  Above 16 rows the
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
     for (int i = tid; i < p.num_seqs; i += kThreads) {
       s = sequence_of(p, p.first_seq + i);
       unit[i] = unit_tiles(p, s, kRows);
-      upto[i + 1] = static_cast<int64_t>((s.qlen * p.group + kRows - 1) / kRows) * p.hkv * unit[i];
+      upto[i + 1] = static_cast<int64_t>((s.qlen * p.group + kRows - 1) / kRows) * unit[i];
     }
     __syncthreads();
     if (warp == 0) {
@@ -195,8 +198,10 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
     }
     __syncthreads();
     const int64_t total = upto[p.num_seqs];
-    const int shares = static_cast<int>(min(max(total / kMinShare, int64_t(1)), static_cast<int64_t>(gridDim.x)));
-    if (static_cast<int>(blockIdx.x) >= shares || total == 0) {
+    const int shares = static_cast<int>(min(max(total / kMinShare, int64_t(1)), static_cast<int64_t>(gridDim.x / p.hkv)));
+    const int c = blockIdx.x / p.hkv;
+    h = blockIdx.x - c * p.hkv;
+    if (c >= shares || total == 0) {
       if (blockIdx.x == 0 && tid == 0) *p.shares = 0;
       return;
     }
@@ -208,13 +213,13 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       if (past < kSnap) return x - past;
       return unit[q] - past < kSnap ? x + unit[q] - past : x;
     };
-    at = cut(blockIdx.x);
-    end = cut(blockIdx.x + 1);
-    if (tid == 0) {  // where the share starts
+    at = cut(c);
+    end = cut(c + 1);
+    if (h == 0 && tid == 0) {  // where the share starts
       const int i = last_up_to(upto, p.num_seqs, at);
       const int64_t past = at - upto[i];
       const int u = static_cast<int>(past / unit[i]);
-      p.share_unit[blockIdx.x] = make_int3(i, u, static_cast<int>(past - static_cast<int64_t>(u) * unit[i]));
+      p.share_unit[c] = make_int3(i, u, static_cast<int>(past - static_cast<int64_t>(u) * unit[i]));
     }
     if (blockIdx.x == 0 && tid == 0) *p.shares = shares;
   }
@@ -227,12 +232,10 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       b = p.first_seq + i;
       all = unit[i];
       const int64_t past = at - upto[i];
-      const int u = static_cast<int>(past / all);
-      from = static_cast<int>(past - static_cast<int64_t>(u) * all);
+      rb = static_cast<int>(past / all);
+      from = static_cast<int>(past - static_cast<int64_t>(rb) * all);
       to = static_cast<int>(min(static_cast<int64_t>(all), from + (end - at)));
       at += to - from;
-      h = u % p.hkv;
-      rb = u / p.hkv;
       s = sequence_of(p, b);
     }
     const int rows_all = s.qlen * p.group;
@@ -773,8 +776,8 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
 
 // What remains after the split kernel where units were cut: one row a CTA, the
 // segments of the row's unit shared out over the warps.  kGrid: CTA (unit, row);
-// kShares: CTA (c, row) has the unit that share c + 1 is the first to start
-// inside, if it is.
+// kShares: CTA ((c, head), row) has the unit that share c + 1 is the first to
+// start inside, if it is.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_constant__ StreamParams p) {
   __shared__ float part[kWarps][D];
@@ -797,7 +800,7 @@ __global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_con
     count = p.splits;
     r += u % units / p.hkv * p.rows_cta;
   } else {
-    const int c = blockIdx.x + 1, shares = *p.shares;
+    const int c = blockIdx.x / p.hkv + 1, shares = *p.shares;
     if (c >= shares) return;
     const int3 at = p.share_unit[c], before = p.share_unit[c - 1];
     if (at.z == 0 || (before.x == at.x && before.y == at.y && before.z > 0)) return;  // no cut, or not its first
@@ -810,11 +813,11 @@ __global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_con
       if (same != 0xffffffffu) break;
     }
     b = at.x;
-    h = at.y % p.hkv;
-    place0 = static_cast<int64_t>(2 * (c - 1) + 1) * p.rows_cta + r;
-    place1 = static_cast<int64_t>(2 * c) * p.rows_cta + r;
-    step = 2 * p.rows_cta;
-    r += at.y / p.hkv * p.rows_cta;
+    h = blockIdx.x % p.hkv;
+    place0 = (2 * (static_cast<int64_t>(c - 1) * p.hkv + h) + 1) * p.rows_cta + r;
+    place1 = 2 * (static_cast<int64_t>(c) * p.hkv + h) * p.rows_cta + r;
+    step = static_cast<int64_t>(2) * p.hkv * p.rows_cta;
+    r += at.y * p.rows_cta;
   }
   const StreamSeq s = sequence_of(p, p.first_seq + b);
   if (r >= s.qlen * p.group) return;
@@ -1037,7 +1040,10 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   } else {
     pl.mode = kShares;
     pl.splits = 1;
-    pl.ctas = static_cast<int>(std::min<int64_t>(std::max<int64_t>(units * tiles / kMinShare, 1), slots));
+    const int64_t of_head = units / a->num_kv_heads * tiles;
+    pl.ctas = static_cast<int>(std::min<int64_t>(std::max<int64_t>(of_head / kMinShare, 1),
+                                                 std::max<int64_t>(slots / a->num_kv_heads, 1)) *
+                               a->num_kv_heads);
     pl.parts = 2 * pl.ctas;
   }
   auto padded = [](size_t x) { return (x + 15) & ~size_t(15); };
@@ -1083,7 +1089,7 @@ int launch_typed(const StreamParams& p, const StreamPlan& pl, cudaStream_t strea
   int rc = pl.m16 == 1 ? launch_split<T, D, 1>(p, pl, stream) : launch_split<T, D, 2>(p, pl, stream);
   if (rc != FD_OK || pl.mode == kCluster) return rc;
   const int64_t merges = pl.mode == kGrid ? (pl.splits == 1 ? 0 : static_cast<int64_t>(p.num_seqs) * p.hkv * pl.row_blocks)
-                                          : pl.ctas - 1;
+                                          : pl.ctas - p.hkv;
   // rows of a row block: all of them where queries may be longer than announced
   const int64_t rows = p.qstart ? p.rows_cta : std::min<int64_t>(p.rows_cta, p.group);
   if (merges > 0)
