@@ -2,6 +2,7 @@
 // token, or a handful of drafts (fd_window_attention), and one token with the
 // attention weights kept (fd_scored_decode).
 #include <algorithm>
+#include <climits>
 #include <cstring>
 #include <type_traits>
 
@@ -114,10 +115,10 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 //             plane a head 166 (161).  As many shares as CTAs fit: with four
 //             times as many, one long sequence of 131071 tokens took 117 us
 //             (97), 64 sequences of up to 4100 visible tokens 180 us (162).
-// Partials go to stream_merge_kernel.
+// Partials go to stream_merge_kernel, or stream_finish_kernel with scores.
 //
 // Bounds: long windows, the reads of K and V, once each (64 sequences of up to
-// 131072 tokens, window 4096, 32/8 heads of 128: 892 MB in 161 us, 5.5 TB/s; one
+// 131072 tokens, window 4096, 32/8 heads of 128: 892 MB in 160 us, 5.6 TB/s; one
 // sequence of 131071 tokens: 537 MB in 95 us, 5.7 TB/s); a short one, a chain of
 // dependent steps - table, first tile, its product, two merges (one token,
 // window 1024, 16/2 heads: 9.2 us, of which 0.16 are bytes).  Above 16 rows the
@@ -779,19 +780,17 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
 // kShares: CTA ((c, head), row) has the unit that share c + 1 is the first to
 // start inside, if it is.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_constant__ StreamParams p) {
+__device__ __forceinline__ void merge_row(const StreamParams& p, int block, int r) {
   __shared__ float part[kWarps][D];
   __shared__ float part_ml[kWarps][2];
   constexpr int kPer = D / 32;
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
-  pdl_wait();
-  pdl_launch_dependents();
   int64_t place0, place1, step;  // places of the first and the second segment, and from there on
-  int count, b, h, r = blockIdx.y;
+  int count, b, h;
   if (p.mode == kGrid) {
-    const int units = p.row_blocks * p.hkv, u = blockIdx.x;
+    const int units = p.row_blocks * p.hkv, u = block;
     b = u / units;
     h = u % p.hkv;
     place0 = (static_cast<int64_t>(u) * p.splits) * p.rows_cta + r;
@@ -800,7 +799,7 @@ __global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_con
     count = p.splits;
     r += u % units / p.hkv * p.rows_cta;
   } else {
-    const int c = blockIdx.x / p.hkv + 1, shares = *p.shares;
+    const int c = block / p.hkv + 1, shares = *p.shares;
     if (c >= shares) return;
     const int3 at = p.share_unit[c], before = p.share_unit[c - 1];
     if (at.z == 0 || (before.x == at.x && before.y == at.y && before.z > 0)) return;  // no cut, or not its first
@@ -813,7 +812,7 @@ __global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_con
       if (same != 0xffffffffu) break;
     }
     b = at.x;
-    h = blockIdx.x % p.hkv;
+    h = block % p.hkv;
     place0 = (2 * (static_cast<int64_t>(c - 1) * p.hkv + h) + 1) * p.rows_cta + r;
     place1 = 2 * (static_cast<int64_t>(c) * p.hkv + h) * p.rows_cta + r;
     step = static_cast<int64_t>(2) * p.hkv * p.rows_cta;
@@ -863,29 +862,78 @@ __global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_con
   }
   const int qt = r / p.group, head = h * p.group + r - qt * p.group;
   static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + tid * p.os2] = from_f32<T>(sum == 0.f ? 0.f : y / sum);
-  if (p.scores && tid == 0)
-    p.row_lse[static_cast<int64_t>(s.q0 + qt) * p.hq + head] = sum == 0.f ? INFINITY : base + log2f(sum);
+}
+
+// log2 of the sum of exp2 of row g of the unit's `count` partials, by a warp.
+__device__ __forceinline__ float merged_lse(const StreamParams& p, int64_t place0, int64_t place1, int64_t step,
+                                            int count, int lane) {
+  float m = -INFINITY, l = 0.f;
+  for (int i = lane; i < count; i += 32) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + 2 * (i == 0 ? place0 : place1 + (i - 1) * step));
+    const float mn = fmaxf(m, ml.x), base = mn == -INFINITY ? 0.f : mn;
+    l = l * ex2(m - base) + ml.y * ex2(ml.x - base);
+    m = mn;
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, d), l2 = __shfl_xor_sync(0xffffffffu, l, d);
+    const float mn = fmaxf(m, m2), base = mn == -INFINITY ? 0.f : mn;
+    l = l * ex2(m - base) + l2 * ex2(m2 - base);
+    m = mn;
+  }
+  return l == 0.f ? INFINITY : (m == -INFINITY ? 0.f : m) + log2f(l);
 }
 
 // Every token's score gets the sum over the group of exp2(raw - lse), four
 // neighbouring tokens a thread.  Bound by its reads of the raw scores (one
 // sequence of 131071 tokens, 32/8 heads: 25 MB in 10 us, cold).  The weights have
 // to wait for the whole row's sum, so the scores go through memory once; kept in
-// the CTA instead where a cluster holds the row.
-__global__ void __launch_bounds__(kThreads) stream_scores_kernel(const __grid_constant__ StreamParams p) {
-  extern __shared__ float lse[];  // [group]
+// the CTA instead where a cluster holds the row.  A CTA works out the sums of its
+// rows itself, so it does not wait for the merge, which is in the same launch.
+__device__ __forceinline__ void add_scores(const StreamParams& p, int chunk, int chunks, int h, int seq, float* lse) {
   const int tid = threadIdx.x;
-  const int h = blockIdx.y;
-  const int b = p.first_seq + blockIdx.z;
-  pdl_wait();
-  pdl_launch_dependents();
+  const int lane = tid & 31;
+  const int b = p.first_seq + seq;
   const StreamSeq s = sequence_of(p, b);
-  if (4 * static_cast<int>(blockIdx.x) * kThreads >= s.n) return;
+  if (4 * chunk * kThreads >= s.n) return;
   const int64_t row0 = static_cast<int64_t>(b) * p.hq + h * p.group;
-  for (int g = tid; g < p.group; g += kThreads) lse[g] = p.row_lse[row0 + g];
+  for (int rb = 0; rb * p.rows_cta < p.group; ++rb) {
+    int64_t place0 = 0, place1 = 0, step = 0;
+    int count = 0;  // of partials; none: one CTA had the unit
+    if (p.mode == kGrid) {
+      if (p.splits > 1) {
+        place0 = ((static_cast<int64_t>(seq) * p.row_blocks + rb) * p.hkv + h) * p.splits * p.rows_cta;
+        step = p.rows_cta;
+        place1 = place0 + step;
+        count = p.splits;
+      }
+    } else {  // the shares that start inside the unit, and the one before them
+      const int shares = *p.shares;
+      int first = 0, inside = 0;
+      for (int i = 0; i < shares; i += kThreads) {
+        int3 x = make_int3(INT_MAX, 0, 0);
+        if (i + tid < shares) x = p.share_unit[i + tid];
+        const bool in = x.x == seq && x.y == rb && x.z > 0;
+        first += __syncthreads_count(x.x < seq || (x.x == seq && (x.y < rb || (x.y == rb && x.z == 0))));
+        inside += __syncthreads_count(in);
+      }
+      if (inside > 0) {
+        place0 = (2 * (static_cast<int64_t>(first - 1) * p.hkv + h) + 1) * p.rows_cta;
+        place1 = 2 * (static_cast<int64_t>(first) * p.hkv + h) * p.rows_cta;
+        step = static_cast<int64_t>(2) * p.hkv * p.rows_cta;
+        count = 1 + inside;
+      }
+    }
+    const int rows = min(p.rows_cta, p.group - rb * p.rows_cta);
+    for (int r = tid >> 5; r < rows; r += kWarps) {
+      const float x = count > 0 ? merged_lse(p, place0 + r, place1 + r, step, count, lane)
+                                : p.row_lse[row0 + rb * p.rows_cta + r];
+      if (lane == 0) lse[rb * p.rows_cta + r] = x;
+    }
+  }
   __syncthreads();
   const float* raw = p.raw + row0 * p.raw_tokens;
-  for (int at = 4 * (blockIdx.x * kThreads + tid); at < s.n; at += 4 * gridDim.x * kThreads) {
+  for (int at = 4 * (chunk * kThreads + tid); at < s.n; at += 4 * chunks * kThreads) {
     const int64_t id =  // four tokens: one page
         load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(at >> p.bs_log2) * p.bts1);
     if (id < 0 || id >= p.num_blocks) continue;
@@ -914,6 +962,33 @@ __global__ void __launch_bounds__(kThreads) stream_scores_kernel(const __grid_co
         if (at + i < s.n) slot[i * p.scs2] = at + i == s.n - 1 ? w[i] : old[i] + w[i];
     }
   }
+}
+
+// Grid: (`merges` units, rows).
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) stream_merge_kernel(const __grid_constant__ StreamParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  merge_row<T, D>(p, blockIdx.x, blockIdx.y);
+}
+
+// The same with scores, in one launch (one sequence of 131071 tokens: 108 us, 113
+// with a launch each): CTAs for `merges` units x `rows` of them, then for `chunks`
+// x KV heads x sequences.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads)
+    stream_finish_kernel(const __grid_constant__ StreamParams p, int merges, int rows, int chunks) {
+  extern __shared__ float lse[];  // [group]
+  pdl_wait();
+  pdl_launch_dependents();
+  int block = blockIdx.x;
+  if (block < merges * rows) {
+    merge_row<T, D>(p, block / rows, block % rows);
+    return;
+  }
+  block -= merges * rows;
+  const int unit = block / chunks;
+  add_scores(p, block - unit * chunks, chunks, unit % p.hkv, unit / p.hkv, lse);
 }
 
 struct StreamPlan {
@@ -1092,15 +1167,20 @@ int launch_typed(const StreamParams& p, const StreamPlan& pl, cudaStream_t strea
                                           : pl.ctas - p.hkv;
   // rows of a row block: all of them where queries may be longer than announced
   const int64_t rows = p.qstart ? p.rows_cta : std::min<int64_t>(p.rows_cta, p.group);
-  if (merges > 0)
-    rc = cuda_status(launch_pdl(stream_merge_kernel<T, D>, dim3(static_cast<unsigned>(merges), static_cast<unsigned>(rows)),
-                                dim3(kThreads), 0, stream, p));
-  if (rc != FD_OK || !p.scores) return rc;
+  if (!p.scores) {
+    if (merges > 0)
+      rc = cuda_status(launch_pdl(stream_merge_kernel<T, D>,
+                                  dim3(static_cast<unsigned>(merges), static_cast<unsigned>(rows)), dim3(kThreads), 0,
+                                  stream, p));
+    return rc;
+  }
   // a CTA goes over 2 x 512 tokens where there are so many
-  const int64_t chunks = (pl.raw_tokens + 8 * kThreads - 1) / (8 * kThreads);
   const int64_t most = std::max<int64_t>(1, (1 << 20) / (static_cast<int64_t>(p.hkv) * p.num_seqs));
-  return cuda_status(launch_pdl(stream_scores_kernel, dim3(static_cast<unsigned>(std::min(chunks, most)), p.hkv, p.num_seqs),
-                                dim3(kThreads), static_cast<size_t>(p.group) * sizeof(float), stream, p));
+  const int64_t chunks = std::min<int64_t>((pl.raw_tokens + 8 * kThreads - 1) / (8 * kThreads), most);
+  const int64_t blocks = merges * rows + chunks * p.hkv * p.num_seqs;
+  return cuda_status(launch_pdl(stream_finish_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
+                                static_cast<size_t>(p.group) * sizeof(float), stream, p, static_cast<int>(merges),
+                                static_cast<int>(rows), static_cast<int>(chunks)));
 }
 
 int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
