@@ -61,6 +61,9 @@ class BoundedLayer:
         start = self.length[stream]
         while len(self.pages[stream]) * self.block_size < start + tokens:
             self.pages[stream].append(self.free.pop())
+        return self._places(stream, start, tokens)
+
+    def _places(self, stream, start, tokens):
         places = range(start, start + tokens)
         return ([self.pages[stream][t // self.block_size] for t in places], [t % self.block_size for t in places])
 
@@ -91,6 +94,8 @@ class BoundedLayer:
                 m = min(n - step, self.budget + self.slack - self.length[stream])
                 part = slice(at + step, at + step + m)
                 rot = self.append([stream], q[part], k[part], v[part], [m])
+                blocks, offsets = self._places(stream, self.length[stream] - m, m)
+                self.scores[blocks, :, offsets] = 0.0
                 outs.append(fd.window_attention(
                     rot, self.k, self.v, self._table([stream]), self._tensor([self.length[stream]], torch.int32),
                     window=self.budget, sinks=self.sinks, query_start_loc=self._tensor([0, m], torch.int32),

@@ -65,8 +65,12 @@ def scored_decode(q, k_cache, v_cache, scores, block_tables, seq_lens, *, sm_sca
     - scores: [num_blocks, num_kv_heads, block_size] float32, updated in
       place: every token of sequence b gets the softmax weights of the query
       heads that share its KV head added.  The newest token's score is set
-      instead, so a reused page needs no clearing.  No two sequences may share
-      a page.
+      instead, so the slots of tokens that enter the cache one at a time
+      through here need no clearing.  Every other slot does: of a prompt or of
+      drafts, appended several at once, only the last token is ever the
+      newest, and the others' slots hold what their pages' former owner left
+      (set them to zero when the tokens are appended).  No two sequences may
+      share a page.
     - return: like q (``out`` if given); zeros for an empty sequence.
     """
     hp = _lib.load_hostpath()

@@ -300,8 +300,9 @@ int fd_rope_kv_append(const fd_rope_kv_append_args* args, void* cuda_stream);
  * sinks, query_start_loc, max_query_len and num_tokens are not read), and
  * scores[block, kv_head, offset] += the softmax weight the token got, summed
  * over the query heads of the KV head.  The newest token's score is set, not
- * added to: what its slot held before is not read.  No two sequences may share
- * a page (their updates would race). */
+ * added to: what its slot held before is not read.  Slots of tokens appended
+ * several at once (a prompt, drafts) have to be cleared by the caller.  No two
+ * sequences may share a page (their updates would race). */
 typedef struct fd_stream_attention_args {
   int32_t struct_size;   /* = sizeof(fd_stream_attention_args) */
   int32_t dtype;         /* FD_DTYPE_F16 or FD_DTYPE_BF16 */
