@@ -83,14 +83,15 @@ class BoundedLayer:
 
     def prompt(self, stream, q, k, v, chunk=1024):
         """A stream's prompt, windowed by its budget: chunk by chunk, the
-        cache is cut back to the budget before it overflows."""
+        cache is cut back to the sinks and the newest before it overflows."""
+        newest = self.budget - self.sinks
         outs = []
         for at in range(0, q.shape[0], chunk):
             n = min(chunk, q.shape[0] - at)
             step = 0
             while step < n:  # what fits the stream's pages goes in one call
                 if self.length[stream] >= self.budget + self.slack:
-                    self.evict([stream])
+                    self.evict([stream], newest)
                 m = min(n - step, self.budget + self.slack - self.length[stream])
                 part = slice(at + step, at + step + m)
                 rot = self.append([stream], q[part], k[part], v[part], [m])
@@ -101,6 +102,8 @@ class BoundedLayer:
                     window=self.budget, sinks=self.sinks, query_start_loc=self._tensor([0, m], torch.int32),
                     max_query_len=m))
                 step += m
+        if self.length[stream] >= self.budget + self.slack:  # the first decoded token would rank zeros
+            self.evict([stream], newest)
         return torch.cat(outs)
 
     def decode(self, streams, q, k, v):
@@ -112,13 +115,15 @@ class BoundedLayer:
         lens = self._tensor([self.length[s] for s in streams], torch.int32)
         return fd.scored_decode(rot, self.k, self.v, self.scores, self._table(streams), lens)
 
-    def evict(self, streams):
-        """Keep the budget's worth of each stream in fresh pages."""
+    def evict(self, streams, recent=None):
+        """Keep the budget's worth of each stream in fresh pages, the last
+        `recent` tokens (the layer's own number if None) among it."""
+        recent = self.recent if recent is None else recent
         kept = -(-self.budget // self.block_size)
         new = [[self.free.pop() for _ in range(kept)] for _ in streams]
         lens = self._tensor([self.length[s] for s in streams], torch.int32)
         fd.evict_tokens(self.k, self.v, self.scores, self._table(streams), lens, self._tensor(new, torch.int32),
-                        budget=self.budget, sinks=self.sinks, recent=self.recent)
+                        budget=self.budget, sinks=self.sinks, recent=recent)
         for s, pages in zip(streams, new):
             self.free += self.pages[s]
             self.pages[s] = pages

@@ -1,5 +1,6 @@
 """examples/bounded_stream.py where pages change hands: a prompt that gets the
-pages of evicted tokens starts without their scores."""
+pages of evicted tokens starts without their scores, and a prompt longer than
+its cache keeps what its own window attention sees."""
 
 from __future__ import annotations
 
@@ -42,3 +43,19 @@ def test_a_prompt_on_recycled_pages_has_no_scores_yet(poison):
     # one step's weights of the 4 query heads of each KV head
     total = layer.scores[blocks, :, offsets].double().sum(0)
     assert torch.allclose(total, torch.full_like(total, 4.0), rtol=1e-4, atol=0)
+
+
+@pytest.mark.parametrize("tokens", [80, 81, 250, 320])
+def test_a_prompt_longer_than_its_cache_keeps_the_newest(tokens):
+    layer = _example().BoundedLayer(1, q_heads=8, kv_heads=2, head_dim=64, block_size=8, budget=64, slack=16, sinks=2,
+                                    recent=16)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    q, k, v = _drawn(gen, tokens, layer)
+    layer.prompt(0, q, k, v, chunk=50)
+    for _ in range(2):  # the first decoded tokens of a full stream have little to rank by
+        blocks, offsets = _slots(layer, 0)
+        n = layer.length[0]
+        assert torch.equal(layer.v[blocks, :, offsets], torch.cat([v[:2], v[len(v) - (n - 2):]]))
+        step = _drawn(gen, 1, layer)
+        v = torch.cat([v, step[2]])
+        layer.decode([0], *step)
