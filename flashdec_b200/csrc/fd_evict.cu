@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(kSelectThreads, 3)
       static_cast<int*>(p.new_lens)[b] = m;
     }
   }
-  for (int i = m + rank * kSelectThreads + tid; i < p.budget; i += ranks * kSelectThreads) kept[i] = -1;
+  // (64 bits: a budget may be within a step of INT_MAX)
+  for (int64_t i = m + rank * kSelectThreads + tid; i < p.budget; i += ranks * kSelectThreads) kept[i] = -1;
   if (n <= m) {  // the whole cluster
     for (int i = rank * kSelectThreads + tid; i < m; i += ranks * kSelectThreads) kept[i] = i;
     return;
