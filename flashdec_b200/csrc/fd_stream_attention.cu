@@ -28,6 +28,7 @@ constexpr int kSnap = 4;            // tiles: a cut this near to a unit's end mo
 constexpr int kRawBytes = 10 << 10; // scores a CTA may keep in shared memory
 constexpr int kClusterRun = 512;    // tokens of a split of a cluster, at most
 constexpr int kOldMost = kClusterRun / kThreads;
+constexpr int kGroupMost = 16384;   // query heads a KV head, at most
 
 template <int D>
 constexpr size_t ring_bytes() {
@@ -1018,7 +1019,7 @@ int check(const fd_stream_attention_args* a, bool scored) {
   if (a->num_seqs < 0 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->num_blocks <= 0 ||
       a->max_blocks_per_seq <= 0 || a->num_q_heads % a->num_kv_heads != 0)
     return FD_ERR_INVALID_ARGUMENT;
-  if (a->num_seqs > 65535 || a->num_kv_heads > 65535 || a->num_q_heads / a->num_kv_heads > 16384 ||
+  if (a->num_seqs > 65535 || a->num_kv_heads > 65535 || a->num_q_heads / a->num_kv_heads > kGroupMost ||
       static_cast<int64_t>(a->max_blocks_per_seq) * a->block_size > 0x3fffffff)
     return FD_ERR_UNSUPPORTED;
   if (!scored) {
@@ -1161,6 +1162,12 @@ int launch_split(const StreamParams& p, const StreamPlan& pl, cudaStream_t strea
 
 template <typename T, int D>
 int launch_typed(const StreamParams& p, const StreamPlan& pl, cudaStream_t stream) {
+  if (p.scores && pl.mode != kCluster) {  // a sum per head of the group: 64 KB for the greatest one
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(done, reinterpret_cast<const void*>(stream_finish_kernel<T, D>),
+                                     kGroupMost * sizeof(float), p.device);
+    if (e != cudaSuccess) return cuda_status(e);
+  }
   int rc = pl.m16 == 1 ? launch_split<T, D, 1>(p, pl, stream) : launch_split<T, D, 2>(p, pl, stream);
   if (rc != FD_OK || pl.mode == kCluster) return rc;
   const int64_t merges = pl.mode == kGrid ? (pl.splits == 1 ? 0 : static_cast<int64_t>(p.num_seqs) * p.hkv * pl.row_blocks)
