@@ -39,9 +39,11 @@ namespace {
 //
 //   warp 0      TMA producer: K and V tiles alternate through a ring of slots
 //   warp 1      issues the tcgen05.mma (one thread)
-//   warps 2, 3  V tiles with keys that some row does not see: rows that no row
-//               sees are zeroed, and an infinity or NaN in another raises the
-//               CTA's `careful` flag
+//   warps 2, 3  V tiles with keys that some row does not see, or with a page
+//               that is not in the cache: rows that no row sees are zeroed, and
+//               so is an infinity or NaN in another (a weight of 0 times it
+//               would be NaN), which marks the item: its epilogue adds what the
+//               rows that see it get
 //   warps 4-7   softmax and epilogue of rows 0-127
 //   warps 8-11  the same of rows 128-255
 //
@@ -58,7 +60,8 @@ struct PromptSmem {
   static constexpr uint32_t kOperand = (D / 64) * kHalf;   // a Q group or a K or V tile
   static constexpr uint32_t kRing = 2 * kOperand;          // offset: two Q groups first
   static constexpr uint32_t kBars = kRing + kSlots * kOperand;
-  static constexpr uint32_t kList = kBars + 512;           // row blocks before each sequence's
+  static constexpr uint32_t kGood = kBars + 512;           // keys of 16 tiles whose page is in the cache
+  static constexpr uint32_t kList = kGood + 256;           // row blocks before each sequence's
   static constexpr uint32_t kStage = kList + 4 * (kMostSeqs + 4);  // output rows, 4 KB a softmax warp
   static constexpr size_t kBytes = kStage + 8 * 4096 + 1024;       // and alignment
 };
@@ -185,7 +188,25 @@ __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity) {
   }
 }
 
-// What a row sees, in list coordinates (key i of step j is list place 64 j +
+// S of the keys that are not `good` (4 x 32 bits) to -inf, for this thread's
+// row, before the softmax takes it: in the mask there it cost the tiles
+// without such keys 3 to 7 % (registers).
+__device__ __noinline__ void drop_bad_keys(uint32_t s_addr, const uint32_t* good) {
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t on = good[c];
+    if (on == ~0u) continue;
+    float x[32];
+    tmem_ld32(s_addr + 32 * c, x);
+    uint32_t y[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) y[i] = (on >> i) & 1u ? __float_as_uint(x[i]) : 0xff800000u;
+    tmem_st32(s_addr + 32 * c, y);
+  }
+  tmem_wait_st();
+}
+
+// What a row sees, in list coordinates (key i of tile j is list place 128 j +
 // i): [0, sink_end) and [w0, w1].
 struct RowView {
   int sink_end, w0, w1;
@@ -199,49 +220,81 @@ __device__ __forceinline__ RowView view_of(const StreamParams& p, const StreamRa
   return v;
 }
 
-// One row at a time by one warp, key by key, with plain loads: the way out
-// when a page id is bad or a value that part of the rows must not see is not
-// finite.  Same result as the tiles up to rounding.
+// Every row of the block sees list places [at, at + n).
+__device__ __forceinline__ bool interior(const StreamParams& p, const StreamRange& rg, int at, int n) {
+  const RowView first = view_of(p, rg, rg.pos0), last = view_of(p, rg, rg.pos1);
+  return rg.pos0 >= 0 && (at + n <= first.sink_end || (at >= last.w0 && at + n - 1 <= first.w1));
+}
+
+// What the infinities and NaN that were zeroed in the item's V tiles give to
+// the warp's rows [row0, row0 + rows), added to their outputs: only the tiles
+// that some row sees in part are gone over (a few, whatever the window), a
+// token at a time with a lane's D / 32 dims of it.  A weight is above 0 unless
+// its score is -inf, so the outcome is an infinity or NaN whatever its size.
 template <typename T, int D>
-__device__ __noinline__ void careful_rows(const StreamParams& p, const StreamSeq& s, int b, int h, int row0,
-                                          int rows, int lane) {
-  for (int r = row0; r < row0 + rows; ++r) {
-    const int qt = r / p.group;
-    const int head = h * p.group + r - qt * p.group;
-    const int pos = s.n - s.qlen + qt;
-    float q[D / 32], o[D / 32], m = -INFINITY, l = 0.f;
+__device__ __noinline__ void add_nonfinite(const StreamParams& p, int b, int h, int rb, int row0, int rows, int lane) {
+  constexpr int kN = D / 32;
+  const StreamSeq s = sequence_of(p, b);
+  const StreamRange rg(s, rb * kRows, min(rb * kRows + kRows, s.qlen * p.group), p.group, p.window, p.sinks, p.bs_log2);
+  const RowView view = view_of(p, rg, s.n - s.qlen + (row0 + min(lane, rows - 1)) / p.group);  // of row `lane`
+  uint32_t up[kN], down[kN];  // bit r: row r gets +inf, -inf; both: NaN
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      q[i] = to_f32<T>(static_cast<const T*>(p.q)[(s.q0 + qt) * p.qs0 + head * p.qs1 + (lane + 32 * i) * p.qs2]);
-      o[i] = 0.f;
+  for (int i = 0; i < kN; ++i) up[i] = down[i] = 0u;
+  const int list = rg.pages << p.bs_log2;
+#pragma unroll 1
+  for (int place = 0; place < list; ++place) {
+    if (place % kKeys == 0 && interior(p, rg, place, kKeys)) {
+      place += kKeys - 1;
+      continue;
     }
-    const int lo = max(pos - p.window + 1, 0);
-    for (int key = min(p.sinks, lo) > 0 ? 0 : lo; key <= pos; ++key) {
-      if (key >= p.sinks && key < lo) key = lo;
-      const int64_t id =
-          load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(key >> p.bs_log2) * p.bts1);
-      if (id < 0 || id >= p.num_blocks) continue;
-      const int off = key & ((1 << p.bs_log2) - 1);
-      const T* k = static_cast<const T*>(p.k) + id * p.ks0 + h * p.ks1 + off * p.ks2;
-      const T* v = static_cast<const T*>(p.v) + id * p.vs0 + h * p.vs1 + off * p.vs2;
-      float x = 0.f;
+    const bool sees = place < view.sink_end || (place >= view.w0 && place <= view.w1);
+    const uint32_t on = __ballot_sync(0xffffffffu, lane < rows && sees);
+    if (on == 0u) continue;
+    const int64_t id =
+        load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(rg.page(place >> p.bs_log2)) * p.bts1);
+    if (id < 0 || id >= p.num_blocks) continue;
+    const int off = place & ((1 << p.bs_log2) - 1);
+    const T* const k = static_cast<const T*>(p.k) + id * p.ks0 + h * p.ks1 + off * p.ks2;
+    const T* const v = static_cast<const T*>(p.v) + id * p.vs0 + h * p.vs1 + off * p.vs2;
+    float x[kN];
+    bool odd = false;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) x += q[i] * to_f32<T>(k[(lane + 32 * i) * p.ks3]);
+    for (int i = 0; i < kN; ++i) {
+      x[i] = to_f32<T>(v[(lane + 32 * i) * p.vs3]);
+      odd |= !isfinite(x[i]);
+    }
+    if (!__any_sync(0xffffffffu, odd)) continue;
+    uint32_t none = 0u;  // rows where the token's weight is 0
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+      if (!((on >> r) & 1u)) continue;
+      const int qt = (row0 + r) / p.group, head = h * p.group + (row0 + r) - qt * p.group;
+      const T* const q = static_cast<const T*>(p.q) + (s.q0 + qt) * p.qs0 + head * p.qs1;
+      float y = 0.f;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      x *= p.scale_log2;
-      const float mn = fmaxf(m, x);
-      const float base = mn == -INFINITY ? 0.f : mn;
-      const float alpha = exp2f(m - base), w = exp2f(x - base);
-      m = mn;
-      l = l * alpha + w;
+      for (int i = 0; i < kN; ++i) y += to_f32<T>(q[(lane + 32 * i) * p.qs2]) * to_f32<T>(k[(lane + 32 * i) * p.ks3]);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) o[i] = o[i] * alpha + w * to_f32<T>(v[(lane + 32 * i) * p.vs3]);
+      for (int d = 16; d > 0; d >>= 1) y += __shfl_xor_sync(0xffffffffu, y, d);
+      if (y * p.scale_log2 == -INFINITY) none |= 1u << r;
     }
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-      static_cast<T*>(p.out)[(s.q0 + qt) * p.os0 + head * p.os1 + (lane + 32 * i) * p.os2] =
-          from_f32<T>(l == 0.f ? 0.f : o[i] / l);
+    for (int i = 0; i < kN; ++i) {
+      if (isfinite(x[i])) continue;
+      up[i] |= x[i] < 0.f ? none : on;  // NaN: both
+      down[i] |= x[i] > 0.f ? none : on;
+    }
+  }
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r) {
+    const int qt = (row0 + r) / p.group, head = h * p.group + (row0 + r) - qt * p.group;
+    T* const out = static_cast<T*>(p.out) + (s.q0 + qt) * p.os0 + head * p.os1;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const bool u = (up[i] >> r) & 1u, d = (down[i] >> r) & 1u;
+      if (!u && !d) continue;
+      T* const y = out + (lane + 32 * i) * p.os2;
+      *y = from_f32<T>(to_f32<T>(*y) + (u ? INFINITY : 0.f) + (d ? -INFINITY : 0.f));
+    }
   }
 }
 
@@ -267,21 +320,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* drained = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  // [8] by the CTA's count of items with keys: count + 1 where such an item
-  // needs the plain way.  The loads are a few items ahead of the group that
-  // works; the other one may lag (items of one group go past it), so a group
-  // says how many it has `seen`, and a place that is taken again before both
-  // have read it sends all later items the plain way.
-  volatile int* careful = abort_flag + 1;
-  volatile int* seen = careful + 8;  // [group]
-  volatile int* all_careful = seen + 2;
-  auto need_care = [&](int count) {
+  // [8] by the CTA's count of items with keys: count + 1 where values of such an
+  // item were zeroed (add_nonfinite).  The loads are a few items ahead of the
+  // group that works; the other one may lag (items of one group go past it),
+  // so a group says how many it has `seen`, and a place that is taken again
+  // before both have read it marks all later items.
+  volatile int* marked = abort_flag + 1;
+  volatile int* seen = marked + 8;  // [group]
+  volatile int* all_marked = seen + 2;
+  auto mark = [&](int count) {
     if (count >= 8 && (seen[0] < count - 7 || seen[1] < count - 7)) {
-      *all_careful = 1;
+      *all_marked = 1;
       __threadfence_block();
     }
-    careful[count & 7] = count + 1;
+    marked[count & 7] = count + 1;
   };
+  // Raised for good at the first page that is not in the cache: only then the
+  // softmax looks at what good_keys says.
+  volatile int* any_bad = all_marked + 1;
+  // [16][4 x 32 bits] by the CTA's count of tiles: the tile's keys whose page is
+  // in the cache.  A tile's product with V waits for those who read this, and
+  // the producer is kSlots / 2 tiles ahead of them at most.
+  uint32_t* const good_keys = reinterpret_cast<uint32_t*>(smem + SM::kGood);
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
   const int lane = tid & 31;
@@ -302,8 +362,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     mbar_init(smem_u32(drained), 1);
     fence_mbar_init();
     *abort_flag = 0;
-    for (int i = 0; i < 8; ++i) careful[i] = 0;
-    seen[0] = seen[1] = *all_careful = 0;
+    for (int i = 0; i < 8; ++i) marked[i] = 0;
+    seen[0] = seen[1] = *all_marked = *any_bad = 0;
   }
   if (warp == 3) tmem_alloc(smem_u32(tmem_slot), 512);
   if (warp == 0 && lane == 0) {
@@ -366,11 +426,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     return StreamRange(im.s, im.rb * kRows, min(im.rb * kRows + kRows, im.rows_all), p.group, p.window, p.sinks,
                        p.bs_log2);
   };
-  // every row of the block sees list places [at, at + n)
-  auto interior = [&](const StreamRange& rg, int at, int n) {
-    const RowView first = view_of(p, rg, rg.pos0), last = view_of(p, rg, rg.pos1);
-    return rg.pos0 >= 0 && (at + n <= first.sink_end || (at >= last.w0 && at + n - 1 <= first.w1));
-  };
 
   // 128 x 88 + 256 x 208 registers: the launch's 384 x 168
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
@@ -381,11 +436,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const int my_page = lane / kHalves;
     uint32_t n = 0;  // tiles of either kind issued so far
     bool ok = true;
-    for (int item = blockIdx.x, live = -1; ok && item < items; item += gridDim.x) {
+    for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
       const Item im = item_at(item);
       const StreamRange rg = range_of(im);
       const int tiles = (rg.pages + tile_pages - 1) / tile_pages;
-      live += tiles > 0 ? 1 : 0;
       auto look = [&](int t) -> int64_t {  // -2: no page there
         const int i = t * tile_pages + my_page;
         if (my_page >= tile_pages || i >= rg.pages) return -2;
@@ -396,11 +450,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int64_t id = next;
         if (t + 1 < tiles) next = look(t + 1);
         const bool valid = id >= 0 && id < p.num_blocks;
-        if (id != -2 && !valid) {
-          need_care(live);
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, valid));
+        const uint32_t bad = __ballot_sync(0xffffffffu, id != -2 && !valid);
+        if (bad != 0u && lane == 0) {
+          *any_bad = 1;
           atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
         }
-        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, valid));
+        if (lane < 4) {
+          uint32_t good = ~0u;
+          if (bad != 0u) {  // 8 keys: never more than a page
+#pragma unroll 1
+            for (int i = 0; i < 32; i += 8)
+              if ((bad >> (((32 * lane + i) >> p.bs_log2) * kHalves)) & 1u) good &= ~(0xffu << i);
+          }
+          good_keys[4 * ((n >> 1) & 15) + lane] = good;
+        }
+        __syncwarp();
         for (int kind = 0; ok && kind < 2; ++kind, ++n) {
           const int slot = n % kSlots;
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[slot]), ((n / kSlots) & 1) ^ 1, p.status, abort_flag));
@@ -526,7 +591,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int slot = n % kSlots;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[slot]), (n / kSlots) & 1, p.status, abort_flag));
         if (!ok) break;
-        if (!interior(rg, t * kKeys, kKeys)) {
+        const bool edge = !interior(p, rg, t * kKeys, kKeys);
+        const uint4 good4 = *reinterpret_cast<const uint4*>(good_keys + 4 * ((n >> 1) & 15));
+        if (edge || (good4.x & good4.y & good4.z & good4.w) != ~0u) {
           uint8_t* v = smem + SM::kRing + slot * SM::kOperand + (lane >> 3) * 128 + (lane & 7) * 16;
           const int end = min(kKeys, (list - t * kKeys + 15) & ~15);
           uint32_t top = 0;  // the largest magnitudes so far, NaN above all
@@ -537,7 +604,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             const int k0 = (kHalves == 2 ? u >> 1 : u) * 16;
             const int at = t * kKeys + k0;
             uint4* x = reinterpret_cast<uint4*>(v + hf * SM::kHalf + k0 * 128);
-            if (at + 16 <= s1 || (at >= w0 && at + 16 <= w1)) {
+            const uint32_t good = (good_keys[4 * ((n >> 1) & 15) + (k0 >> 5)] >> (k0 & 16)) & 0xffffu;
+            if (good == 0xffffu && (at + 16 <= s1 || (at >= w0 && at + 16 <= w1))) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const uint4 y = x[32 * i];
@@ -547,7 +615,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll 1
               for (int i = 0; i < 4; ++i) {
                 const int place = at + 4 * i + (lane >> 3);
-                if (place < s1 || (place >= w0 && place < w1)) {
+                if ((place < s1 || (place >= w0 && place < w1)) && ((good >> (4 * i)) & 1u)) {
                   const uint4 y = x[32 * i];
                   top = max_abs<T>(max_abs<T>(max_abs<T>(max_abs<T>(top, y.x), y.y), y.z), y.w);
                 } else {
@@ -556,7 +624,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               }
             }
           }
-          if (__any_sync(0xffffffffu, nonfinite16(top, kExp)) && lane == 0) need_care(live);
+          // (a tile that every row sees has its product as it is)
+          if (edge && __any_sync(0xffffffffu, nonfinite16(top, kExp))) {
+            if (lane == 0) mark(live);
+#pragma unroll 1
+            for (int u = warp - 2; u < kHalves * (end >> 4); u += 2) {
+              uint32_t* x = reinterpret_cast<uint32_t*>(v + (kHalves == 2 ? u & 1 : 0) * SM::kHalf +
+                                                        (kHalves == 2 ? u >> 1 : u) * 16 * 128);
+#pragma unroll 1
+              for (int i = 0; i < 16; ++i) {
+                uint32_t* y = x + 128 * (i >> 2) + (i & 3);
+                const uint32_t w = *y;
+                *y = ((w & kExp) == kExp ? 0u : w & 0xffffu) | ((w >> 16 & kExp) == kExp ? 0u : w & 0xffff0000u);
+              }
+            }
+          }
           fence_proxy_async_smem();
           __syncwarp();
         }
@@ -609,6 +691,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       cp_async_commit();
     };
     uint32_t it = 0;
+    uint32_t skipped = 0;  // tiles of items without this group
     int live = -1;
     bool here = false;  // the queries of this item are on their way
     Item im = {0, 0, 0, 0, {0, 0, 0}};
@@ -622,6 +705,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const bool more = item + static_cast<int>(gridDim.x) < items;
       if (cur.rb * kRows + 128 * g >= cur.rows_all) {  // not a row of this group's
         if (gt == 0) seen[g] = live + 1;
+        skipped += tiles;
         if (more) im = item_at(item + gridDim.x);
         continue;
       }
@@ -663,6 +747,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[g]), it & 1, p.status, abort_flag));
         if (!ok) break;
         tc_fence_after();
+        if (__any_sync(0xffffffffu, *any_bad)) drop_bad_keys(s_addr, good_keys + 4 * ((it + skipped) & 15));
         float v[kKeys];
         tmem_ld64(s_addr, *reinterpret_cast<float(*)[64]>(v));
         tmem_ld64(s_addr + 64, *reinterpret_cast<float(*)[64]>(v + 64));
@@ -740,66 +825,64 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         here = true;
       }
       if (ok && tiles > 0) ok = pv_wait();
-      bool plain = false;
+      bool mend = false;
       if (tiles > 0) {
-        plain = careful[live & 7] == live + 1;
+        mend = marked[live & 7] == live + 1;
         __threadfence_block();
-        plain = plain || *all_careful != 0;
+        mend = mend || *all_marked != 0;
       }
+      mend = __any_sync(0xffffffffu, mend);
       // all warps of the group go on or none
       if (barrier_any(1 + g, 128, !ok)) break;
       if (gt == 0) seen[g] = live + 1;
       const float l = l2.x + l2.y;
       tc_fence_after();
-      if (plain) {
-        const int w0 = grow0 + (warp & 3) * 32;
-        careful_rows<T, D>(p, cur.s, cur.b, cur.h, w0, max(0, min(32, rows_all - w0)), lane);
-      } else {
-        // ---- O / l, 64 dims at a time through 4 KB of the warp's own, so that
-        // 8 lanes write 128 bytes of a row: stored from TMEM rows directly, a
-        // lane each, the epilogue took 11k cycles of a 100k-cycle row block ----
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int w0 = 32 * (warp & 3);  // the warp's first row of the group
-        const int qt0 = grow0 / p.group, rem0 = grow0 - qt0 * p.group;
-        uint8_t* const stage = smem + SM::kStage + (warp - 4) * 4096;
-        T* const out = static_cast<T*>(p.out);
+      // ---- O / l, 64 dims at a time through 4 KB of the warp's own, so that
+      // 8 lanes write 128 bytes of a row: stored from TMEM rows directly, a
+      // lane each, the epilogue took 11k cycles of a 100k-cycle row block ----
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int w0 = 32 * (warp & 3);  // the warp's first row of the group
+      const int qt0 = grow0 / p.group, rem0 = grow0 - qt0 * p.group;
+      uint8_t* const stage = smem + SM::kStage + (warp - 4) * 4096;
+      T* const out = static_cast<T*>(p.out);
 #pragma unroll 1
-        for (int hf = 0; hf < D / 64; ++hf) {
+      for (int hf = 0; hf < D / 64; ++hf) {
 #pragma unroll 1
-          for (int q4 = 0; q4 < 2; ++q4) {
-            float o[32];
-            if (tiles > 0) {
-              tmem_ld32(o_addr + 64 * hf + 32 * q4, o);
-            } else {
+        for (int q4 = 0; q4 < 2; ++q4) {
+          float o[32];
+          if (tiles > 0) {
+            tmem_ld32(o_addr + 64 * hf + 32 * q4, o);
+          } else {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * q4 + i) ^ (lane & 7)) << 4)) =
-                  make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
-                             pack2<T>(o[8 * i + 4], o[8 * i + 5]), pack2<T>(o[8 * i + 6], o[8 * i + 7]));
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
           }
-          __syncwarp();
-          const int cc = lane & 7;
-#pragma unroll 4
-          for (int i = lane >> 3; i < 32; i += 4) {
-            if (grow0 + w0 + i >= rows_all) break;
-            const T* y = reinterpret_cast<const T*>(stage + i * 128 + ((cc ^ (i & 7)) << 4));
-            T* dst = out + row_at(cur, qt0, rem0, w0 + i, p.os0, p.os1);
-            const int d = 64 * hf + 8 * cc;
-            if (p.out_vec) {
-              *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(y);
-            } else {
-#pragma unroll 1
-              for (int k = 0; k < 8; ++k) dst[(d + k) * p.os2] = y[k];
-            }
-          }
-          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * q4 + i) ^ (lane & 7)) << 4)) =
+                make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
+                           pack2<T>(o[8 * i + 4], o[8 * i + 5]), pack2<T>(o[8 * i + 6], o[8 * i + 7]));
         }
+        __syncwarp();
+        const int cc = lane & 7;
+#pragma unroll 4
+        for (int i = lane >> 3; i < 32; i += 4) {
+          if (grow0 + w0 + i >= rows_all) break;
+          const T* y = reinterpret_cast<const T*>(stage + i * 128 + ((cc ^ (i & 7)) << 4));
+          T* dst = out + row_at(cur, qt0, rem0, w0 + i, p.os0, p.os1);
+          const int d = 64 * hf + 8 * cc;
+          if (p.out_vec) {
+            *reinterpret_cast<uint4*>(dst + d) = *reinterpret_cast<const uint4*>(y);
+          } else {
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k) dst[(d + k) * p.os2] = y[k];
+          }
+        }
+        __syncwarp();
       }
+      const int left = rows_all - grow0 - w0;
+      if (mend && left > 0) add_nonfinite<T, D>(p, cur.b, cur.h, cur.rb, grow0 + w0, min(32, left), lane);
       tc_fence_before();
     }
   }
