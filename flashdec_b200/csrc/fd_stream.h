@@ -45,8 +45,11 @@ struct StreamParams {
   float* part_acc;  // [place][row of the unit][D]
   float* part_ml;   // [place][row of the unit][2]: max (base 2), sum
   float* row_lse;   // [query x head]: max + log2(sum), with scores
-  float* raw;       // [query x head][raw_tokens]: scaled scores (base 2)
-  int64_t raw_tokens;  // row length of raw, or of its copy in shared memory
+  float* raw;       // scaled scores (base 2): per sequence of the launch [head][its tokens]
+  int64_t* raw_start;  // [sequence of the launch] tokens before its raw scores (kShares)
+  int64_t raw_tokens;  // row length of raw (kGrid), or of its copy in shared memory
+  int64_t raw_room;    // tokens that raw has room for
+  uint64_t blocks_magic;  // ceil(2^64 / row blocks of a group); 0: one
   int* status;
   int device;  // host side only
 };

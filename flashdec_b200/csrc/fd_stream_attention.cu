@@ -73,6 +73,13 @@ __device__ __forceinline__ int unit_tiles(const StreamParams& p, const StreamSeq
   return max(((rg.pages << p.bs_log2) + kTok - 1) / kTok, 1);
 }
 
+// Tokens before a sequence's raw scores, from the tiles of the units before it
+// (one query a sequence: as many units each as the group has row blocks).
+__device__ __forceinline__ int64_t raw_tokens_before(const StreamParams& p, int64_t unit_tiles_before) {
+  const uint64_t x = static_cast<uint64_t>(unit_tiles_before);
+  return static_cast<int64_t>(p.blocks_magic ? __umul64hi(x, p.blocks_magic) : x) * kTok;
+}
+
 // Last i of [0, n) with first[i] <= x (first[0] <= x).
 __device__ __forceinline__ int last_up_to(const int64_t* first, int n, int64_t x) {
   int lo = 0, hi = n;
@@ -200,6 +207,8 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
     }
     __syncthreads();
     const int64_t total = upto[p.num_seqs];
+    if (p.scores && blockIdx.x == 0)  // where a sequence's raw scores start
+      for (int i = tid; i < p.num_seqs; i += kThreads) p.raw_start[i] = raw_tokens_before(p, upto[i]);
     const int shares = static_cast<int>(min(max(total / kMinShare, int64_t(1)), static_cast<int64_t>(gridDim.x / p.hkv)));
     const int c = blockIdx.x / p.hkv;
     h = blockIdx.x - c * p.hkv;
@@ -410,7 +419,23 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
       }
       const float slack = 8.f / scale;
       // where this thread's rows' scores go (one query: row = head of the group,
-      // list place = position), less the tile's
+      // list place = position), less the tile's; nowhere where the tables list more
+      // pages than the cache has
+      int64_t raw_tokens = p.raw_tokens;
+      float* raw_at = nullptr;
+      if (p.scores) {
+        if (cluster) {
+          raw_at = raw - t0 * kTok;
+        } else {
+          int64_t before = blockIdx.z * raw_tokens;
+          if (!grid) {
+            before = raw_tokens_before(p, upto[b - p.first_seq]);
+            raw_tokens = static_cast<int64_t>(all) * kTok;
+          }
+          if (before + raw_tokens <= p.raw_room)
+            raw_at = p.raw + before * p.hq + (h * p.group + row0) * raw_tokens;
+        }
+      }
       float* raw_row[kM][2];
 #pragma unroll
       for (int a = 0; a < kM; ++a)
@@ -418,10 +443,7 @@ __global__ void __launch_bounds__(kThreads, 2) stream_split_kernel(const __grid_
         for (int e = 0; e < 2; ++e) {
           const int r = 16 * a + 8 * e + g8;
           raw_row[a][e] = nullptr;
-          if (p.scores && r < rows)
-            raw_row[a][e] = (cluster ? raw - t0 * kTok
-                                     : p.raw + (static_cast<int64_t>(b) * p.hq + h * p.group + row0) * p.raw_tokens) +
-                            r * p.raw_tokens + 2 * t4;
+          if (raw_at && r < rows) raw_row[a][e] = raw_at + r * raw_tokens + 2 * t4;
         }
 
       for (int t = t0 + warp; t < t1; t += kWarps) {
@@ -933,7 +955,14 @@ __device__ __forceinline__ void add_scores(const StreamParams& p, int chunk, int
     }
   }
   __syncthreads();
-  const float* raw = p.raw + row0 * p.raw_tokens;
+  const bool grid = p.mode == kGrid;
+  const int64_t raw_tokens = grid ? p.raw_tokens : unit_tiles(p, s, p.rows_cta) * kTok;
+  const int64_t raw_at = grid ? seq * raw_tokens : p.raw_start[seq];
+  if (raw_at + raw_tokens > p.raw_room) {
+    if (tid == 0) atomicOr(p.status, FD_STATUS_BAD_BLOCK_ID);
+    return;
+  }
+  const float* raw = p.raw + raw_at * p.hq + h * p.group * raw_tokens;
   for (int at = 4 * (chunk * kThreads + tid); at < s.n; at += 4 * chunks * kThreads) {
     const int64_t id =  // four tokens: one page
         load_index(p.bt, p.bt64, b * p.bts0 + static_cast<int64_t>(at >> p.bs_log2) * p.bts1);
@@ -948,7 +977,7 @@ __device__ __forceinline__ void add_scores(const StreamParams& p, int chunk, int
     }
 #pragma unroll 4
     for (int g = 0; g < p.group; ++g) {
-      const float4 x = *reinterpret_cast<const float4*>(raw + g * p.raw_tokens + at);
+      const float4 x = *reinterpret_cast<const float4*>(raw + g * raw_tokens + at);
       const float y = lse[g];
       w[0] += ex2(x.x - y);
       w[1] += ex2(x.y - y);
@@ -997,7 +1026,8 @@ struct StreamPlan {
   int row_blocks;  // of the longest queries announced
   bool prompt;     // many rows: prompt_attention, where it takes the layout
   int64_t max_query;
-  int64_t raw_tokens;
+  int64_t raw_tokens;  // of a table's row, or of a cluster's CTA
+  int64_t raw_room;    // tokens of all sequences of a launch
   int mode;          // kCluster, kGrid or kShares
   int splits;        // CTAs of a unit, of a cluster or grid
   int rows_most;     // of a cluster's unit
@@ -1005,9 +1035,10 @@ struct StreamPlan {
   int ctas;          // grid of kShares
   int parts;         // places of partials
   // scratch: (kShares) where each CTA's share starts, and their number; the
-  // partials; for scores the rows' lse and raw scores
-  size_t meta_bytes, ml_bytes, acc_bytes, lse_bytes, raw_bytes;
-  size_t bytes() const { return meta_bytes + ml_bytes + acc_bytes + lse_bytes + raw_bytes; }
+  // partials; for scores the rows' lse, (kShares) where each sequence's raw
+  // scores start, and raw scores
+  size_t meta_bytes, ml_bytes, acc_bytes, lse_bytes, start_bytes, raw_bytes;
+  size_t bytes() const { return meta_bytes + ml_bytes + acc_bytes + lse_bytes + start_bytes + raw_bytes; }
 };
 
 int check(const fd_stream_attention_args* a, bool scored) {
@@ -1128,7 +1159,17 @@ StreamPlan plan_of(const fd_stream_attention_args* a, bool scored, int sms) {
   pl.acc_bytes = static_cast<size_t>(pl.parts) * per * a->head_dim * sizeof(float);
   if (scored) {
     pl.lse_bytes = padded(q_rows * sizeof(float));
-    pl.raw_bytes = q_rows * static_cast<size_t>(pl.raw_tokens) * sizeof(float);
+    // Raw scores of the tables' tokens, but of no more than twice the cache's (no
+    // two sequences share a page; whole tiles): block tables are as wide as the
+    // longest context allowed (64 sequences of 500 tokens and 32 heads under
+    // tables for 131072: 14 MB, not 1080).
+    const int64_t seqs = std::min(a->num_seqs, kMaxListed);
+    pl.raw_room = seqs * pl.raw_tokens;
+    if (pl.mode == kShares) {
+      pl.raw_room = std::min(pl.raw_room, 2 * static_cast<int64_t>(a->num_blocks) * a->block_size + seqs * kTok);
+      pl.start_bytes = padded(seqs * sizeof(int64_t));
+    }
+    pl.raw_bytes = static_cast<size_t>(pl.raw_room) * a->num_q_heads * sizeof(float);
   }
   return pl;
 }
@@ -1181,9 +1222,12 @@ int launch_typed(const StreamParams& p, const StreamPlan& pl, cudaStream_t strea
                                   stream, p));
     return rc;
   }
-  // a CTA goes over 2 x 512 tokens where there are so many
-  const int64_t most = std::max<int64_t>(1, (1 << 20) / (static_cast<int64_t>(p.hkv) * p.num_seqs));
-  const int64_t chunks = std::min<int64_t>((pl.raw_tokens + 8 * kThreads - 1) / (8 * kThreads), most);
+  // A CTA goes over 2 x 512 tokens of the longest sequence there can be, or more
+  // where that would be many CTAs (of 64 sequences of 500 tokens under tables for
+  // 131072, 65536 of which nearly all return at once: 106 us, 43 with narrow ones).
+  const int64_t most = std::max<int64_t>(1, (1 << 15) / (static_cast<int64_t>(p.hkv) * p.num_seqs));
+  const int64_t longest = std::min(pl.raw_tokens, static_cast<int64_t>(p.num_blocks) << p.bs_log2);
+  const int64_t chunks = std::min<int64_t>((longest + 8 * kThreads - 1) / (8 * kThreads), most);
   const int64_t blocks = merges * rows + chunks * p.hkv * p.num_seqs;
   return cuda_status(launch_pdl(stream_finish_kernel<T, D>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads),
                                 static_cast<size_t>(p.group) * sizeof(float), stream, p, static_cast<int>(merges),
@@ -1269,9 +1313,14 @@ int run(const fd_stream_attention_args* a, bool scored, void* cuda_stream) {
     p.part_acc = reinterpret_cast<float*>(at);
     at += pl.acc_bytes;
     p.row_lse = reinterpret_cast<float*>(at);
-    p.raw = reinterpret_cast<float*>(at + pl.lse_bytes);
+    at += pl.lse_bytes;
+    p.raw_start = reinterpret_cast<int64_t*>(at);
+    p.raw = reinterpret_cast<float*>(at + pl.start_bytes);
   }
   p.raw_tokens = pl.raw_tokens;
+  p.raw_room = pl.raw_room;
+  const uint64_t group_blocks = (p.group + p.rows_cta - 1) / p.rows_cta;
+  p.blocks_magic = group_blocks > 1 ? UINT64_MAX / group_blocks + 1 : 0;
   p.status = status;
   p.device = dev->device;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);

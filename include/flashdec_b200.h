@@ -302,7 +302,10 @@ int fd_rope_kv_append(const fd_rope_kv_append_args* args, void* cuda_stream);
  * over the query heads of the KV head.  The newest token's score is set, not
  * added to: what its slot held before is not read.  Slots of tokens appended
  * several at once (a prompt, drafts) have to be cleared by the caller.  No two
- * sequences may share a page (their updates would race). */
+ * sequences may share a page (their updates would race; where the sequences
+ * list more than twice the cache's pages, those past that get no scores and
+ * raise FD_STATUS_BAD_BLOCK_ID).  The scratch goes by num_blocks, not by the
+ * width of the block tables. */
 typedef struct fd_stream_attention_args {
   int32_t struct_size;   /* = sizeof(fd_stream_attention_args) */
   int32_t dtype;         /* FD_DTYPE_F16 or FD_DTYPE_BF16 */
