@@ -9,6 +9,10 @@ weight of every cached token.  When a stream has outgrown its budget by
 pages and the old ones are freed, so the stream goes on for ever in
 ``budget + slack`` tokens of cache.
 
+A prompt's tokens have no weights yet: their scores start at zero (their pages
+may have been another stream's), and a prompt longer than the cache keeps the
+sinks and its newest tokens.
+
     python examples/bounded_stream.py --streams 8 --prompt 5000 --tokens 600
 
 Random weights stand for the model: q, k and v of each token are drawn, not

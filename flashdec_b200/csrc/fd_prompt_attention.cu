@@ -29,13 +29,21 @@ namespace {
 // one, the K and V tiles and the queries of the next are on their way: 58 us for
 // ragged prompts of 9 tiles an item, against 65 with a CTA for each item (whose
 // start and end were a sixth of its time or more); 314 against 306 us for an 8k
-// prompt of 17 tiles an item, which pays for the longer code instead.
+// prompt of 17 tiles an item, which pays for the longer code instead (both
+// figures of that time).
 //
-// What bounds it: the softmax.  A tile costs a thread 128 scores to scale,
-// exponentiate and pack, which its issue slots take longer for than the tensor
-// pipe for both products (8k queries, window 2048, 32/8 heads: 241 GFLOP in
-// 315-325 us, 0.46 of the rate of a large library product; the tensor pipe is busy a
-// third to a half of the time).
+// What bounds it: the latency of a tile.  8k queries, window 2048, 32/8 heads:
+// 241 GFLOP in 322-337 us, 0.44-0.46 of the rate of a large library product, with
+// the tensor pipe busy 37 % of the time, the exponentials' pipe 38 % and the issue
+// slots 32 %; 23, 25 and 25 % on ragged prompts of 9 tiles an item.  A group
+// waits for its S, then for both halves of the scores, and has all 128 of them
+// masked and their maximum found before the first exponential, and its
+// products idle meanwhile; two groups do not cover that.  Some 200 bytes of a
+// thread's state are spilled around the tile loop.
+//
+// K and V tiles are loaded again for every row block, from L2 mostly: the 8k
+// prompt moves 1.2 GB through L2 and reads 146 MB of DRAM, where q, K and V are
+// 101.
 //
 //   warp 0      TMA producer: K and V tiles alternate through a ring of slots
 //   warp 1      issues the tcgen05.mma (one thread)

@@ -88,7 +88,8 @@ def evict_tokens(k_cache, v_cache, scores, block_tables, seq_lens, new_block_tab
     scored of the others (equal scores: the lower position first; NaN ranks
     above every number), in their order.  K, V and scores of place i of
     sequence b go to slot ``i % block_size`` of page ``new_block_tables[b, i //
-    block_size]``; the source pages stay as they are (they may be shared with
+    block_size]``, whose rows have room for ``min(budget, max_blocks_per_seq *
+    block_size)`` tokens; the source pages stay as they are (they may be shared with
     other sequences), and the caller frees them afterwards.  New pages must be
     distinct and none of them a source page.
 
